@@ -385,6 +385,55 @@ int b2m_rs_reduce_fp8(const void* codes, const float* scales, int64_t rows, int6
 int b2m_route_topk(const float* logits, int64_t tokens, int32_t experts, int32_t top_k, const float* bias,
                    int32_t* topk_ids, float* topk_weights, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Matrix products over expert segments of any length (no padding to blocks).
+ * `rows` rows sorted by expert; segment e is the rows ends[e-1] <= t < ends[e]
+ * (ends[-1] = 0; int32 [experts], the cumulative row counts, on the device).  Empty
+ * segments are allowed, experts <= 1024.  An end below an earlier one or outside [0, rows]
+ * is replaced by the nearest value in order and recorded as B2M_STATUS_BAD_ROUTING in
+ * dev_status.  Rows behind ends[experts-1] belong to no expert: clear_rest != 0 writes zeros
+ * to their output rows, 0 leaves those as they were.
+ * Operands: type codes below; unit stride along the last axis; ld*, w_stride in elements,
+ * multiples of 16 bytes (the extents need not be); base pointers 16-byte aligned.
+ * Outputs: the input type or fp32, any row stride.  Sums are fp32 over the whole axis
+ * and rounded once.  Extents <= 2^30. */
+#define B2M_BF16 0
+#define B2M_FP16 1
+#define B2M_FP32 2
+
+/* out[t, :] = x[t, :] w[e]^T.  x [rows, k], w [experts, n, k], out [rows, n]. */
+int b2m_grouped_mm(const void* x, int64_t rows, int64_t ldx, const void* w, int32_t experts, int64_t n, int64_t k,
+                   int64_t ldw, int64_t w_stride, const int32_t* ends, int32_t in_type, void* out, int64_t ldo,
+                   int32_t out_type, int32_t clear_rest, int32_t* dev_status, void* stream);
+
+/* Gradient of the rows: out[t, :] = dy[t, :] w[e].  dy [rows, n], out [rows, k]. */
+int b2m_grouped_mm_dx(const void* dy, int64_t rows, int64_t lddy, const void* w, int32_t experts, int64_t n, int64_t k,
+                      int64_t ldw, int64_t w_stride, const int32_t* ends, int32_t in_type, void* out, int64_t ldo,
+                      int32_t out_type, int32_t clear_rest, int32_t* dev_status, void* stream);
+
+/* Gradient of the weights: out[e] = dy[segment e]^T x[segment e], zero for an empty segment.
+ * dy [rows, n], x [rows, k], out [experts, n, k] (out_stride elements between experts). */
+int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows, int64_t n, int64_t k,
+                      const int32_t* ends, int32_t experts, int32_t in_type, void* out, int64_t ldo,
+                      int64_t out_stride, int32_t out_type, int32_t* dev_status, void* stream);
+
+/* 8-bit integer codes with one scale for each row of x (type code in_type) [rows, cols]:
+ *   scale[r] = max(amax(|x[r, :]|) / 127, 1e-12)            (IEEE fp32 division)
+ *   q[r, c]  = rne(x[r, c] / scale[r]) clamped to +-127      (IEEE fp32 division)
+ * A NaN in a row makes its scale NaN, an infinity makes it infinite; the codes of such values
+ * are 0, so whatever is multiplied with the row becomes NaN.  Any strides and alignment. */
+int b2m_quant_i8(const void* x, int32_t in_type, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
+                 float* scale, void* stream);
+
+/* 8-bit integer product with scales for each token and channel:
+ *   out[t, n] = (float)(sum_k a[t, k] w[e, n, k]) * a_scale[t] * w_scale[e, n]
+ * with exact int32 sums (k <= 131071, so that no sum can pass 32 bits).  a int8 [rows, k],
+ * w int8 [experts, n, k], a_scale fp32 [rows], w_scale fp32 [experts, n]; out_type any of the
+ * codes.  Segments as above; ends == NULL with experts == 1: one segment of all rows. */
+int b2m_int8_mm(const void* a, const float* a_scale, int64_t rows, int64_t lda, const void* w, const float* w_scale,
+                int32_t experts, int64_t n, int64_t k, int64_t ldw, int64_t w_stride, const int32_t* ends, void* out,
+                int64_t ldo, int32_t out_type, int32_t clear_rest, int32_t* dev_status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -54,6 +54,11 @@ SIGNATURES: dict[str, list] = {
     "b2m_rs_reduce_fp8": [_p, _p, _i64, _i64, _i32, _p, _c.c_uint32, _p, _p, _p, _i32, _p, _i32, _p, _p],
     "b2m_quant_push_sparse": [_p, _i64, _i64, _i64, _i32, _p, _p, _i64, _p, _c.c_uint32, _p, _p, _i32, _p, _i32, _p],
     "b2m_route_topk": [_p, _i64, _i32, _i32, _p, _p, _p, _p],
+    "b2m_grouped_mm": [_p, _i64, _i64, _p, _i32, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _i32, _i32, _p, _p],
+    "b2m_grouped_mm_dx": [_p, _i64, _i64, _p, _i32, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _i32, _i32, _p, _p],
+    "b2m_grouped_mm_dw": [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i32, _i32, _p, _i64, _i64, _i32, _p, _p],
+    "b2m_quant_i8": [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p],
+    "b2m_int8_mm": [_p, _p, _i64, _i64, _p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p, _i64, _i32, _i32, _p, _p],
 }
 
 ERROR_NAMES = {1: "B2M_ERR_ARG", 2: "B2M_ERR_CUDA", 3: "B2M_ERR_UNSUPPORTED"}

@@ -1,0 +1,758 @@
+// Matrix products over expert segments of any length: 16-bit operands (forward, gradient
+// of the rows, gradient of the weights) and 8-bit integers with a scale for each token and
+// channel.  Segment e is the rows ends[e-1] <= t < ends[e] of the row operand.
+//
+//   kFwd  y[t, n]     = sum_k x[t, k] w[e, n, k]        x, w read along k
+//   kDx   dx[t, k]    = sum_n dy[t, n] w[e, n, k]       w read across its rows
+//   kDw   dw[e, n, k] = sum_{t in e} dy[t, n] x[t, k]   both read across their rows
+//
+// The tensor core's M axis is the output's contiguous axis (weight rows n for kFwd, weight
+// columns k for kDx and kDw) and its N axis is the output's rows.  So the ragged axis of
+// kFwd and kDx is N, which an MMA takes in steps of 16: a segment's last tile costs what
+// its rows cost, not a full 128, and one token occupies 16 columns of one 128-row weight
+// tile.  Operands read across their rows are "MN-major": 64 of M or N in a 128-byte
+// swizzled row, one such row for each index of the sum.
+//
+// One persistent CTA per SM: warp 0 feeds a ring of TMA stages, warp 1 issues tcgen05.mma
+// into one of two TMEM accumulators, warps 4-11 turn the other one into output rows.
+// Every sum is one fp32 (or exact int32) accumulator in TMEM from the first product to
+// the last, rounded once.
+//
+// Rows that a tile loads beyond its segment are other output rows in kFwd and kDx, computed
+// and never stored.  In kDw they would enter the sum: warp 1 clears them (in both operands,
+// so an infinity there cannot meet a zero) in the segment's last stage before its MMA.
+#include <cudaTypedefs.h>
+#include <cuda_fp16.h>
+
+#include <atomic>
+
+#include "b2m_common.cuh"
+#include "b2m_host.h"
+
+namespace b2m {
+namespace {
+
+enum Mode { kFwd = 0, kDx = 1, kDw = 2 };
+
+constexpr int kM = 128;            // output columns of a tile (TMEM lanes)
+constexpr int kRowBytes = 128;     // one swizzled shared-memory row
+constexpr int kMaxExperts = 1024;
+constexpr int kThreads = 384;
+constexpr int kEpiWarps = 8;
+constexpr int kABytes = kM * kRowBytes;
+constexpr int kBand = 8;           // row tiles walked together, so that they share a weight tile in L2
+constexpr int kSmallBox = 32;      // rows of one TMA box of a tile that is not full
+
+template <int NT>
+struct Shape {
+  static constexpr int kBBytes = NT * kRowBytes;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = NT >= 256 ? 4 : (NT >= 128 ? 6 : 9);
+  static constexpr uint32_t kTmemCols = 2 * NT;
+};
+
+template <int NT>
+struct Control {
+  uint64_t full[Shape<NT>::kStages];
+  uint64_t empty[Shape<NT>::kStages];
+  uint64_t tfull[2];
+  uint64_t tempty[2];
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort;
+  int32_t warp_max[kThreads / 32];
+  int32_t warp_sum[kThreads / 32];
+  int32_t start[kMaxExperts + 2];  // first row of segment e; [E] = end of the last, [E + 1] = rows
+  int32_t tile0[kMaxExperts + 2];  // row tiles before segment e
+};
+
+template <int NT>
+constexpr size_t smem_bytes() {
+  return size_t(Shape<NT>::kStages) * Shape<NT>::kStageBytes + sizeof(Control<NT>) + 1024;
+}
+
+struct Params {
+  const int32_t* ends;   // nullptr: one segment of all rows
+  int32_t experts;
+  int32_t segments;      // experts, plus one for the rows behind the last segment when they are cleared
+  int64_t rows;
+  int32_t m_dim;         // extent of the output's contiguous axis
+  int32_t m_tiles;
+  int32_t c_dim;         // kDw: output rows of one expert
+  int32_t c_tiles;       // kDw
+  int32_t k_blocks;      // kFwd, kDx: blocks of the sum
+  uint32_t idesc;        // instruction descriptor without N
+  void* out;
+  int64_t ldo;
+  int64_t out_expert;    // kDw: elements between two experts' outputs
+  int32_t out_type;
+  const float* a_scale;  // integers: scale of each row
+  const float* w_scale;  // integers: scale of each weight row, [experts, m_dim]
+  int32_t* status;
+  uint64_t timeout_ns;
+};
+
+// One output tile: rows [row0, row0 + cols) of the output (kDw: of expert e's output),
+// columns [m0, m0 + 128).  k_blocks == 0: all zero, nothing is multiplied.
+struct Tile {
+  int e;
+  int m0;
+  int64_t row0;
+  int cols;
+  int k_blocks;
+  int64_t sum0;  // kDw: first row of the sum
+  int sum_rows;  // kDw: rows of the sum
+};
+
+template <int NT>
+__device__ __forceinline__ int find_segment(const Control<NT>* C, int segments, int slot) {
+  int lo = 0, hi = segments - 1;  // the last segment whose first tile is <= slot
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (C->tile0[mid] <= slot)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+template <int kMode, int NT>
+__device__ __forceinline__ Tile tile_at(const Params& p, const Control<NT>* C, int t) {
+  Tile r;
+  int tiles, i;  // row tiles of the segment, and this tile's index among the segment's tiles
+  if (kMode == kDw) {
+    const int per = p.m_tiles * p.c_tiles;
+    r.e = t / per;
+    i = t - r.e * per;
+    tiles = p.c_tiles;
+  } else {
+    r.e = find_segment(C, p.segments, t / p.m_tiles);
+    i = t - C->tile0[r.e] * p.m_tiles;
+    tiles = C->tile0[r.e + 1] - C->tile0[r.e];
+  }
+  const int band = i / (kBand * p.m_tiles);
+  const int in_band = i - band * kBand * p.m_tiles;
+  const int wide = min(kBand, tiles - band * kBand);
+  const int m = in_band / wide;
+  const int c0 = (band * kBand + in_band - m * wide) * NT;
+  r.m0 = m * kM;
+  if (kMode == kDw) {
+    r.row0 = c0;
+    r.cols = min(NT, p.c_dim - c0);
+    r.sum0 = C->start[r.e];
+    r.sum_rows = C->start[r.e + 1] - C->start[r.e];
+    r.k_blocks = (r.sum_rows + 63) >> 6;
+  } else {
+    r.row0 = static_cast<int64_t>(C->start[r.e]) + c0;
+    r.cols = min(NT, C->start[r.e + 1] - C->start[r.e] - c0);
+    r.k_blocks = r.e < p.experts ? p.k_blocks : 0;
+    r.sum0 = 0;
+    r.sum_rows = 0;
+  }
+  return r;
+}
+
+// Segment starts and row-tile counts from `ends`, by all threads.  An end that is below an
+// earlier one or outside [0, rows] is taken as the nearest one that is in order, and noted
+// in the status word.  Returns the number of tiles.
+template <int kMode, int NT>
+__device__ __forceinline__ int plan_segments(const Params& p, Control<NT>* C) {
+  constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rows = static_cast<int>(p.rows);
+  int v[kPer], top = 0;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = tid * kPer + i;
+    const int raw = e < p.experts ? (p.ends ? __ldg(p.ends + e) : rows) : 0;
+    const int end = min(max(raw, 0), rows);
+    bad |= end != raw || (e < p.experts && end < top);
+    top = max(top, end);
+    v[i] = top;
+  }
+  int scan = top;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, scan, off);
+    if (lane >= off) scan = max(scan, o);
+  }
+  if (lane == 31) C->warp_max[warp] = scan;
+  __syncthreads();
+  int before = __shfl_up_sync(0xffffffffu, scan, 1);
+  if (lane == 0) before = 0;
+  for (int w = 0; w < warp; ++w) before = max(before, C->warp_max[w]);
+  if (tid * kPer < p.experts && p.ends && __ldg(p.ends + tid * kPer) < before) bad = true;
+  if (bad && blockIdx.x == 0) set_status(p.status, B2M_STATUS_BAD_ROUTING);
+  int n[kPer], sum = 0, prev = before;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = tid * kPer + i;
+    const int end = max(v[i], before);
+    if (e < p.experts) C->start[e] = prev;
+    if (e == p.experts - 1) C->start[p.experts] = end;
+    n[i] = e < p.experts ? (end - prev + NT - 1) / NT : 0;
+    sum += n[i];
+    prev = end;
+  }
+  if (tid == 0) C->start[p.experts + 1] = rows;
+  int acc = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, acc, off);
+    if (lane >= off) acc += o;
+  }
+  if (lane == 31) C->warp_sum[warp] = acc;
+  __syncthreads();
+  int at = acc - sum, total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) at += C->warp_sum[w];
+    total += C->warp_sum[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = tid * kPer + i;
+    if (e < p.experts) C->tile0[e] = at;
+    at += n[i];
+  }
+  if (tid == 0) C->tile0[p.experts] = total;
+  if (p.segments > p.experts) {  // the rows behind the last segment, as one more segment
+    total += (rows - C->start[p.experts] + NT - 1) / NT;
+    if (tid == 0) C->tile0[p.experts + 1] = total;
+  }
+  __syncthreads();
+  return kMode == kDw ? p.experts * p.m_tiles * p.c_tiles : total * p.m_tiles;
+}
+
+// Shared-memory descriptor of an operand whose 128-byte swizzled rows run along M or N:
+// 64 elements of M (N) in a row, eight rows (indices of the sum) in a group, groups 1024
+// bytes apart, the next 64 of M (N) `chunk_bytes` further on.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t chunk_bytes) {
+  uint64_t d = smem_desc_sw128(saddr) & ~(static_cast<uint64_t>(0x3FFF) << 16);
+  return d | static_cast<uint64_t>(chunk_bytes >> 4) << 16;
+}
+
+template <bool kI8>
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                    uint32_t accumulate) {
+  if (kI8)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+template <int kMode, bool kI8, int NT>
+__device__ __forceinline__ void producer(const CUtensorMap* map_a, const CUtensorMap* map_b,
+                                         const CUtensorMap* map_b_small, const Params& p, uint8_t* smem,
+                                         Control<NT>* C, int num_tiles) {
+  using S = Shape<NT>;
+  constexpr int kElems = kI8 ? 128 : 64;  // elements in a 128-byte row
+  uint32_t kg = 0;
+  bool alive = true;
+  for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
+    const Tile r = tile_at<kMode, NT>(p, C, t);
+    // 32-row boxes (kDw: 64-column chunks) that the tile's columns need
+    const int boxes = kMode == kDw ? (r.cols + 63) / 64 : (r.cols + kSmallBox - 1) / kSmallBox;
+    const bool whole = kMode != kDw && boxes * kSmallBox == NT;
+    const uint32_t bytes = kABytes + boxes * (kMode == kDw ? 64 : kSmallBox) * kRowBytes;
+    const int row = static_cast<int>(r.row0);
+    for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
+      const int s = kg % S::kStages;
+      if (!mbar_wait(&C->empty[s], ((kg / S::kStages) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_PRODUCER,
+                     &C->abort)) {
+        alive = false;
+        break;
+      }
+      uint8_t* a = smem + s * S::kStageBytes;
+      uint8_t* b = a + kABytes;
+      uint64_t* bar = &C->full[s];
+      mbar_arrive_expect_tx(bar, bytes);
+      if (kMode == kFwd) {
+        tma_load_3d(a, map_a, bar, kb * kElems, r.m0, r.e);
+      } else if (kMode == kDx) {
+        tma_load_3d(a, map_a, bar, r.m0, kb * 64, r.e);
+        tma_load_3d(a + kABytes / 2, map_a, bar, r.m0 + 64, kb * 64, r.e);
+      } else {
+        const int at = static_cast<int>(r.sum0) + kb * 64;
+        tma_load_2d(a, map_a, bar, r.m0, at);
+        tma_load_2d(a + kABytes / 2, map_a, bar, r.m0 + 64, at);
+        for (int i = 0; i < boxes; ++i) tma_load_2d(b + i * 64 * kRowBytes, map_b, bar, row + i * 64, at);
+      }
+      if (kMode != kDw) {
+        if (whole)
+          tma_load_2d(b, map_b, bar, kb * kElems, row);
+        else
+          for (int i = 0; i < boxes; ++i)
+            tma_load_2d(b + i * kSmallBox * kRowBytes, map_b_small, bar, kb * kElems, row + i * kSmallBox);
+      }
+    }
+  }
+  // the copies of the last stages must have landed before the CTA exits
+  const uint32_t first = kg > S::kStages ? kg - S::kStages : 0;
+  for (uint32_t i = first; i < kg; ++i)
+    mbar_wait(&C->full[i % S::kStages], (i / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN,
+              nullptr);
+}
+
+// Warp 1.  All lanes wait (they clear the rows behind a kDw segment together), lane 0 issues.
+template <int kMode, bool kI8, int NT>
+__device__ __forceinline__ void mma_warp(const Params& p, uint8_t* smem, Control<NT>* C, int num_tiles,
+                                         uint32_t tmem_base, int lane) {
+  using S = Shape<NT>;
+  uint32_t kg = 0, used = 0;
+  bool alive = true;
+  for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
+    const Tile r = tile_at<kMode, NT>(p, C, t);
+    if (r.k_blocks == 0) continue;
+    const int buf = used & 1;
+    int ok = mbar_wait(&C->tempty[buf], ((used >> 1) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
+                       &C->abort);
+    if (!__all_sync(0xffffffffu, ok)) break;
+    const uint32_t d = tmem_base + static_cast<uint32_t>(buf * NT);
+    const uint32_t idesc = p.idesc | (static_cast<uint32_t>((r.cols + 15) >> 4 << 1) << 17);
+    for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
+      const int s = kg % S::kStages;
+      ok = mbar_wait(&C->full[s], (kg / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort);
+      if (!__all_sync(0xffffffffu, ok)) {
+        alive = false;
+        break;
+      }
+      uint8_t* a = smem + s * S::kStageBytes;
+      int steps = 4;
+      if (kMode == kDw) {
+        const int left = r.sum_rows - kb * 64;
+        if (left < 64) {
+          steps = (left + 15) >> 4;
+          const int vecs = (steps * 16 - left) * (kRowBytes / 16);  // 16-byte pieces to clear in a chunk
+          const int chunks = 2 + (r.cols + 63) / 64;                // of both operands: B follows A
+          for (int i = lane; i < vecs * chunks; i += 32) {
+            const int chunk = i / vecs, at = i - chunk * vecs;
+            *reinterpret_cast<uint4*>(a + chunk * 64 * kRowBytes + left * kRowBytes + at * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      }
+      if (lane == 0) {
+        tc_fence_after();
+        const uint32_t as = smem_u32(a), bs = as + kABytes;
+        const uint64_t adesc = kMode == kFwd ? smem_desc_sw128(as) : smem_desc_mn(as, kABytes / 2);
+        const uint64_t bdesc = kMode == kDw ? smem_desc_mn(bs, 64 * kRowBytes) : smem_desc_sw128(bs);
+        // 32 bytes of the sum in each step: within the row, or 16 rows further on
+        constexpr uint64_t a_step = kMode == kFwd ? 2 : 128, b_step = kMode == kDw ? 128 : 2;
+        for (int k = 0; k < steps; ++k)
+          mma<kI8>(d, adesc + a_step * k, bdesc + b_step * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
+        mma_commit(&C->empty[s]);
+        if (kb == r.k_blocks - 1) mma_commit(&C->tfull[buf]);
+      }
+      __syncwarp();
+    }
+    ++used;
+  }
+  // every MMA issued here has completed before TMEM is freed
+  if (lane == 0 && kg > 0) {
+    mma_commit(&C->mma_done);
+    mbar_wait(&C->mma_done, 0, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
+  }
+  __syncwarp();
+}
+
+template <typename T>
+__device__ __forceinline__ T round_to(float v);
+template <>
+__device__ __forceinline__ float round_to<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half round_to<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+// Output rows row0 .. row0 + n - 1 at this lane's column: 32 lanes write 32 neighbours.
+template <typename T>
+__device__ __forceinline__ void store_rows(void* out, int64_t at, int64_t ldo, int n, const float (&v)[32]) {
+  T* o = static_cast<T*>(out) + at;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < n) o[j * ldo] = round_to<T>(v[j]);
+}
+
+template <int kMode, bool kI8, int NT>
+__device__ __forceinline__ void epilogue(const Params& p, Control<NT>* C, int num_tiles, uint32_t tmem_base, int warp,
+                                         int lane) {
+  const int q = warp & 3;  // TMEM lane quarter of this warp
+  const int h = (warp - 4) >> 2;
+  const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+  uint32_t used = 0;
+  for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
+    const Tile r = tile_at<kMode, NT>(p, C, t);
+    const int buf = used & 1;
+    const int m = r.m0 + q * 32 + lane;
+    const bool in = m < p.m_dim;
+    float ws = 0.0f;
+    if (kI8 && in && r.k_blocks) ws = __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + m);
+    if (r.k_blocks) {
+      const int ok = mbar_wait(&C->tfull[buf], (used >> 1) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_EPILOGUE,
+                               &C->abort);
+      if (!__all_sync(0xffffffffu, ok)) return;
+      tc_fence_after();
+    }
+    const int64_t base = (kMode == kDw ? r.e * p.out_expert : 0) + r.row0 * p.ldo + m;
+    for (int c = h * 32; c < r.cols; c += 64) {
+      float v[32];
+      const int n = min(32, r.cols - c);
+      if (r.k_blocks) {
+        tmem_ld32(tmem_base + lane_off + static_cast<uint32_t>(buf * NT + c), v);
+        tmem_ld_wait();
+        if (kI8) {
+          const float as = lane < n ? __ldg(p.a_scale + r.row0 + c + lane) : 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            v[j] = __int2float_rn(__float_as_int(v[j])) * __shfl_sync(0xffffffffu, as, j) * ws;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+      }
+      if (in) {
+        const int64_t at = base + c * p.ldo;
+        if (p.out_type == B2M_BF16)
+          store_rows<__nv_bfloat16>(p.out, at, p.ldo, n, v);
+        else if (p.out_type == B2M_FP16)
+          store_rows<__half>(p.out, at, p.ldo, n, v);
+        else
+          store_rows<float>(p.out, at, p.ldo, n, v);
+      }
+      __syncwarp();
+    }
+    if (r.k_blocks) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&C->tempty[buf]);
+      ++used;
+    }
+  }
+}
+
+template <int kMode, bool kI8, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
+    grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_b_small, const __grid_constant__ Params p) {
+  using S = Shape<NT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Control<NT>* C = reinterpret_cast<Control<NT>*>(smem + S::kStages * S::kStageBytes);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&C->full[s], 1);
+      mbar_init(&C->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&C->tfull[b], 1);
+      mbar_init(&C->tempty[b], kEpiWarps);
+    }
+    mbar_init(&C->mma_done, 1);
+    C->abort = 0;
+    fence_mbar_init();
+    if (p.rows > 0) {  // without rows nothing is loaded, and kDw has no maps
+      tma_prefetch_desc(&map_a);
+      tma_prefetch_desc(&map_b);
+      if (kMode != kDw) tma_prefetch_desc(&map_b_small);
+    }
+  }
+  if (warp == 1) tmem_alloc(&C->tmem_base, S::kTmemCols);
+  const int num_tiles = plan_segments<kMode, NT>(p, C);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = C->tmem_base;
+  if (warp == 0) {
+    if (lane == 0) producer<kMode, kI8, NT>(&map_a, &map_b, &map_b_small, p, smem, C, num_tiles);
+    __syncwarp();
+  } else if (warp == 1) {
+    mma_warp<kMode, kI8, NT>(p, smem, C, num_tiles, tmem_base, lane);
+  } else if (warp >= 4) {
+    epilogue<kMode, kI8, NT>(p, C, num_tiles, tmem_base, warp, lane);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, S::kTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+// The SM count of the current device, whose context is made this thread's current one: the
+// tensor maps are made by a driver call, and a thread that has made no runtime call that
+// needs a context (torch's backward threads) has none.
+int device_ready(int* num_sms) {
+  int dev = 0;
+  B2M_TRY(require_sm100(num_sms));
+  B2M_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+  return check_cuda(cudaSetDevice(dev), "cudaSetDevice");
+}
+
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims,
+               const cuuint64_t* strides, const cuuint32_t* box, const char* what) {
+  void* fn = nullptr;
+  B2M_TRY(driver_entry("cuTensorMapEncodeTiled", &fn));
+  const auto encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const CUresult r = encode(map, type, rank, const_cast<void*>(base), dims, strides, box, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(B2M_ERR_ARG, "%s: cuTensorMapEncodeTiled failed (%d)", what, static_cast<int>(r));
+  return B2M_OK;
+}
+
+struct Matrix {  // rows of `cols` elements, ld elements apart
+  const void* ptr;
+  int64_t rows, cols, ld;
+};
+
+struct Weights {  // [experts, n, k], strides in elements
+  const void* ptr;
+  int64_t experts, n, k, ld, expert_stride;
+};
+
+template <int kMode, bool kI8, int NT>
+int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& bs, const Params& p, int64_t tiles_bound,
+           int num_sms, cudaStream_t s) {
+  static_assert(smem_bytes<NT>() <= 227 * 1024, "shared memory budget");
+  static std::atomic<bool> attr_done[64];
+  int dev = 0;
+  B2M_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+  auto kernel = grouped_kernel<kMode, kI8, NT>;
+  if (dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
+    B2M_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            static_cast<int>(smem_bytes<NT>())),
+                       "grouped: cudaFuncSetAttribute"));
+    if (dev < 64) attr_done[dev].store(true, std::memory_order_release);
+  }
+  const int grid = static_cast<int>(tiles_bound < num_sms ? tiles_bound : num_sms);
+  kernel<<<grid, kThreads, smem_bytes<NT>(), s>>>(a, b, bs, p);
+  return check_cuda(cudaGetLastError(), "grouped launch");
+}
+
+constexpr int64_t kMaxDim = int64_t(1) << 30;
+
+int check_matrix(const char* what, const char* name, const Matrix& m, int elem) {
+  if (m.rows < 0 || m.rows > kMaxDim || m.cols < 1 || m.cols > kMaxDim)
+    return fail(B2M_ERR_ARG, "%s: %s is [%lld, %lld]; each extent is at most 2^30 and it has columns", what, name,
+                (long long)m.rows, (long long)m.cols);
+  if (m.ld < m.cols || m.ld * elem % 16 || m.ld > (int64_t(1) << 38))
+    return fail(B2M_ERR_ARG, "%s: rows of %s must be at least %lld elements and a multiple of 16 bytes apart (%lld)",
+                what, name, (long long)m.cols, (long long)m.ld);
+  if (m.rows > 0 && (!m.ptr || !aligned16(m.ptr)))
+    return fail(B2M_ERR_ARG, "%s: %s must not be null and must be 16-byte aligned", what, name);
+  return B2M_OK;
+}
+
+int check_weights(const char* what, const Weights& w, int elem) {
+  if (w.experts < 1 || w.experts > kMaxExperts)
+    return fail(B2M_ERR_ARG, "%s: need 1 <= experts <= %d (%lld)", what, kMaxExperts, (long long)w.experts);
+  B2M_TRY(check_matrix(what, "w", Matrix{w.ptr, w.n, w.k, w.ld}, elem));
+  if (w.n < 1) return fail(B2M_ERR_ARG, "%s: w has no rows", what);
+  if (w.expert_stride < 1 || w.expert_stride * elem % 16 || w.expert_stride > (int64_t(1) << 38))
+    return fail(B2M_ERR_ARG, "%s: experts of w must be a multiple of 16 bytes apart (%lld elements)", what,
+                (long long)w.expert_stride);
+  return B2M_OK;
+}
+
+int check_out(const char* what, const void* out, int64_t cols, int64_t ldo, int32_t out_type, int32_t in_type) {
+  if (!out) return fail(B2M_ERR_ARG, "%s: null output", what);
+  if (ldo < cols) return fail(B2M_ERR_ARG, "%s: output rows are %lld elements apart, need %lld", what, (long long)ldo,
+                              (long long)cols);
+  if (out_type != B2M_FP32 && out_type != in_type)
+    return fail(B2M_ERR_ARG, "%s: output type %d must be the input type or fp32", what, out_type);
+  if (reinterpret_cast<uintptr_t>(out) % (out_type == B2M_FP32 ? 4 : 2))
+    return fail(B2M_ERR_ARG, "%s: misaligned output", what);
+  return B2M_OK;
+}
+
+// kFwd and kDx: `rows` (x, dy or integer codes) times each segment's weights.
+template <int kMode, bool kI8>
+int rows_times_weights(const char* what, const Matrix& x, const Weights& w, const int32_t* ends, int32_t in_type,
+                       void* out, int64_t ldo, int32_t out_type, int32_t clear_rest, const float* a_scale,
+                       const float* w_scale, int32_t* status, void* stream) {
+  const int elem = kI8 ? 1 : 2;
+  const CUtensorMapDataType type = kI8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                       : (in_type == B2M_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16);
+  const cuuint32_t in_row = kRowBytes / elem;  // elements in a shared-memory row
+  const int64_t m_dim = kMode == kFwd ? w.n : w.k;
+  const int64_t sum = kMode == kFwd ? w.k : w.n;
+  Params p{};
+  p.ends = ends;
+  p.experts = static_cast<int32_t>(w.experts);
+  p.segments = p.experts + (clear_rest ? 1 : 0);
+  p.rows = x.rows;
+  p.m_dim = static_cast<int32_t>(m_dim);
+  p.m_tiles = static_cast<int32_t>((m_dim + kM - 1) / kM);
+  p.k_blocks = static_cast<int32_t>((sum + in_row - 1) / in_row);
+  p.out = out;
+  p.ldo = ldo;
+  p.out_type = out_type;
+  p.a_scale = a_scale;
+  p.w_scale = w_scale;
+  p.status = status;
+  p.timeout_ns = 2 * timeout_ns();
+  p.idesc = (kI8 ? (2u << 4) | (1u << 7) | (1u << 10)                                             // S32, both signed
+                 : (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u)) |             // F32
+            (kMode == kDx ? 1u << 15 : 0u) | (static_cast<uint32_t>(kM >> 4) << 24);
+
+  const cuuint64_t w_dims[3] = {static_cast<cuuint64_t>(w.k), static_cast<cuuint64_t>(w.n),
+                                static_cast<cuuint64_t>(w.experts)};
+  const cuuint64_t w_strides[2] = {static_cast<cuuint64_t>(w.ld * elem), static_cast<cuuint64_t>(w.expert_stride * elem)};
+  const cuuint32_t w_box[3] = {in_row, kMode == kFwd ? static_cast<cuuint32_t>(kM) : 64u, 1};
+  const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows)};
+  const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
+  // Row tiles of 32 while segments are short on average: the ring then holds weights, not room for rows.
+  const int64_t mean = (x.rows + w.experts - 1) / w.experts;
+  const int64_t nt = mean <= 32 ? 32 : 256;
+  const int64_t row_tiles = (x.rows + nt - 1) / nt + (x.rows < p.segments ? x.rows : p.segments);
+  if (row_tiles * p.m_tiles > INT32_MAX) return fail(B2M_ERR_ARG, "%s: more than 2^31 tiles", what);
+  int num_sms = 0;
+  B2M_TRY(device_ready(&num_sms));
+  if (x.rows == 0) return B2M_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CUtensorMap ma, mb, ms;
+  B2M_TRY(encode_map(&ma, type, 3, w.ptr, w_dims, w_strides, w_box, what));
+  const cuuint32_t small[2] = {in_row, kSmallBox};
+  B2M_TRY(encode_map(&ms, type, 2, x.ptr, x_dims, x_strides, small, what));
+  const cuuint32_t big[2] = {in_row, static_cast<cuuint32_t>(nt)};
+  B2M_TRY(encode_map(&mb, type, 2, x.ptr, x_dims, x_strides, big, what));
+  if (nt == 32) return launch<kMode, kI8, 32>(ma, mb, ms, p, row_tiles * p.m_tiles, num_sms, s);
+  return launch<kMode, kI8, 256>(ma, mb, ms, p, row_tiles * p.m_tiles, num_sms, s);
+}
+
+int check_16bit(const char* what, int32_t in_type) {
+  if (in_type != B2M_BF16 && in_type != B2M_FP16)
+    return fail(B2M_ERR_ARG, "%s: input type %d is neither bf16 nor fp16", what, in_type);
+  return B2M_OK;
+}
+
+}  // namespace
+}  // namespace b2m
+
+extern "C" int b2m_grouped_mm(const void* x, int64_t rows, int64_t ldx, const void* w, int32_t experts, int64_t n,
+                              int64_t k, int64_t ldw, int64_t w_stride, const int32_t* ends, int32_t in_type, void* out,
+                              int64_t ldo, int32_t out_type, int32_t clear_rest, int32_t* dev_status, void* stream) {
+  using namespace b2m;
+  const Matrix mx{x, rows, k, ldx};
+  const Weights mw{w, experts, n, k, ldw, w_stride};
+  B2M_TRY(check_16bit("grouped_mm", in_type));
+  B2M_TRY(check_weights("grouped_mm", mw, 2));
+  B2M_TRY(check_matrix("grouped_mm", "x", mx, 2));
+  if (!ends) return fail(B2M_ERR_ARG, "grouped_mm: null ends");
+  if (rows > 0) B2M_TRY(check_out("grouped_mm", out, n, ldo, out_type, in_type));
+  return rows_times_weights<kFwd, false>("grouped_mm", mx, mw, ends, in_type, out, ldo, out_type, clear_rest, nullptr,
+                                         nullptr, dev_status, stream);
+}
+
+extern "C" int b2m_grouped_mm_dx(const void* dy, int64_t rows, int64_t lddy, const void* w, int32_t experts, int64_t n,
+                                 int64_t k, int64_t ldw, int64_t w_stride, const int32_t* ends, int32_t in_type,
+                                 void* out, int64_t ldo, int32_t out_type, int32_t clear_rest, int32_t* dev_status,
+                                 void* stream) {
+  using namespace b2m;
+  const Matrix mdy{dy, rows, n, lddy};
+  const Weights mw{w, experts, n, k, ldw, w_stride};
+  B2M_TRY(check_16bit("grouped_mm_dx", in_type));
+  B2M_TRY(check_weights("grouped_mm_dx", mw, 2));
+  B2M_TRY(check_matrix("grouped_mm_dx", "dy", mdy, 2));
+  if (!ends) return fail(B2M_ERR_ARG, "grouped_mm_dx: null ends");
+  if (rows > 0) B2M_TRY(check_out("grouped_mm_dx", out, k, ldo, out_type, in_type));
+  return rows_times_weights<kDx, false>("grouped_mm_dx", mdy, mw, ends, in_type, out, ldo, out_type, clear_rest,
+                                        nullptr, nullptr, dev_status, stream);
+}
+
+extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows, int64_t n,
+                                 int64_t k, const int32_t* ends, int32_t experts, int32_t in_type, void* out,
+                                 int64_t ldo, int64_t out_stride, int32_t out_type, int32_t* dev_status,
+                                 void* stream) {
+  using namespace b2m;
+  const char* what = "grouped_mm_dw";
+  const Matrix mdy{dy, rows, n, lddy}, mx{x, rows, k, ldx};
+  B2M_TRY(check_16bit(what, in_type));
+  B2M_TRY(check_matrix(what, "dy", mdy, 2));
+  B2M_TRY(check_matrix(what, "x", mx, 2));
+  if (experts < 1 || experts > kMaxExperts)
+    return fail(B2M_ERR_ARG, "%s: need 1 <= experts <= %d (%d)", what, kMaxExperts, experts);
+  if (!ends) return fail(B2M_ERR_ARG, "%s: null ends", what);
+  B2M_TRY(check_out(what, out, k, ldo, out_type, in_type));
+  if (out_stride < (n - 1) * ldo + k) return fail(B2M_ERR_ARG, "%s: experts of the output overlap", what);
+  constexpr int NT = 256;
+  Params p{};
+  p.ends = ends;
+  p.experts = experts;
+  p.segments = experts;
+  p.rows = rows;
+  p.m_dim = static_cast<int32_t>(k);
+  p.m_tiles = static_cast<int32_t>((k + kM - 1) / kM);
+  p.c_dim = static_cast<int32_t>(n);
+  p.c_tiles = static_cast<int32_t>((n + NT - 1) / NT);
+  p.out = out;
+  p.ldo = ldo;
+  p.out_expert = out_stride;
+  p.out_type = out_type;
+  p.status = dev_status;
+  p.timeout_ns = 2 * timeout_ns();
+  p.idesc = (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) |
+            (static_cast<uint32_t>(kM >> 4) << 24);
+  const int64_t tiles = int64_t(p.m_tiles) * p.c_tiles * experts;
+  if (tiles > INT32_MAX) return fail(B2M_ERR_ARG, "%s: more than 2^31 tiles", what);
+  int num_sms = 0;
+  B2M_TRY(device_ready(&num_sms));
+  const CUtensorMapDataType type =
+      in_type == B2M_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  // Without rows every segment is empty: nothing is loaded, and a map of no rows cannot be made.
+  const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t dy_dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(ldx * 2)};
+  const cuuint64_t dy_strides[1] = {static_cast<cuuint64_t>(lddy * 2)};
+  const cuuint32_t box[2] = {64, 64};
+  CUtensorMap ma{}, mb{};
+  if (rows > 0) {
+    B2M_TRY(encode_map(&ma, type, 2, x, x_dims, x_strides, box, what));
+    B2M_TRY(encode_map(&mb, type, 2, dy, dy_dims, dy_strides, box, what));
+  }
+  return launch<kDw, false, NT>(ma, mb, mb, p, tiles, num_sms, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int b2m_int8_mm(const void* a, const float* a_scale, int64_t rows, int64_t lda, const void* w,
+                           const float* w_scale, int32_t experts, int64_t n, int64_t k, int64_t ldw, int64_t w_stride,
+                           const int32_t* ends, void* out, int64_t ldo, int32_t out_type, int32_t clear_rest,
+                           int32_t* dev_status, void* stream) {
+  using namespace b2m;
+  const Matrix ma{a, rows, k, lda};
+  const Weights mw{w, experts, n, k, ldw, w_stride};
+  B2M_TRY(check_weights("int8_mm", mw, 1));
+  B2M_TRY(check_matrix("int8_mm", "a", ma, 1));
+  if (k > 131071) return fail(B2M_ERR_ARG, "int8_mm: k=%lld; sums of more than 131071 products can pass 32 bits", (long long)k);
+  if (!w_scale || (rows > 0 && !a_scale)) return fail(B2M_ERR_ARG, "int8_mm: null scales");
+  if (!ends && experts != 1) return fail(B2M_ERR_ARG, "int8_mm: ends may be null for one expert only");
+  if (out_type != B2M_BF16 && out_type != B2M_FP16 && out_type != B2M_FP32)
+    return fail(B2M_ERR_ARG, "int8_mm: unknown output type %d", out_type);
+  if (rows > 0) B2M_TRY(check_out("int8_mm", out, n, ldo, out_type, out_type));
+  return rows_times_weights<kFwd, true>("int8_mm", ma, mw, ends, B2M_BF16, out, ldo, out_type, clear_rest, a_scale,
+                                        w_scale, dev_status, stream);
+}

@@ -1,0 +1,181 @@
+// 8-bit integer codes with one scale for each row (the token scales of the integer products).
+//
+//   scale = max(amax / 127, 1e-12)      IEEE fp32 division
+//   q     = rne(x / scale) within +-127  IEEE fp32 division for each element
+//
+// A group of 32 to 1024 threads owns a row and keeps it in registers (up to four 16-byte
+// vectors in each thread) between the maximum and the codes, so x is read once; wider rows
+// are read a second time, from L2.  Bound by HBM: size + 1 bytes for each element.
+#include <cuda_fp16.h>
+
+#include "b2m_common.cuh"
+#include "b2m_host.h"
+
+namespace b2m {
+namespace {
+
+constexpr int kVecs = 4;     // 16-byte vectors of a row in one thread's registers
+constexpr int kBlock = 256;  // threads of a block that holds several rows
+
+// Larger of the two; NaN when one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
+  return __bfloat162float(v);
+}
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) {
+  return __half2float(v);
+}
+
+// Vector `i` of a row (16 / sizeof(T) elements), zero beyond the row.
+template <typename T, bool kAligned>
+__device__ __forceinline__ void load_vec(const T* __restrict__ row, int64_t cols, int64_t i,
+                                         float (&f)[16 / sizeof(T)]) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t c = i * N;
+  if (kAligned && c + N <= cols) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + c));
+    const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = to_f32<T>(t[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = c + j < cols ? to_f32<T>(row[c + j]) : 0.0f;
+  }
+}
+
+template <typename T, bool kAligned>
+__device__ __forceinline__ void store_codes(int8_t* __restrict__ q, int64_t cols, int64_t i, float scale,
+                                            const float (&f)[16 / sizeof(T)]) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t c = i * N;
+  uint32_t w[N / 4];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int code = max(-127, min(127, __float2int_rn(f[j] / scale)));  // a NaN quotient converts to 0
+    const uint32_t byte = static_cast<uint32_t>(code & 0xFF) << (8 * (j & 3));
+    w[j / 4] = (j & 3) ? w[j / 4] | byte : byte;
+  }
+  if (kAligned && c + N <= cols) {
+    if (N == 8)
+      *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[N / 4 - 1]);
+    else
+      *reinterpret_cast<uint32_t*>(q + c) = w[0];
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (c + j < cols) q[c + j] = static_cast<int8_t>(w[j / 4] >> (8 * (j & 3)));
+  }
+}
+
+// blockDim = rows of the block x group; group = 32 .. 1024 threads of a row.
+template <typename T, bool kAligned, bool kInRegisters>
+__global__ void __launch_bounds__(1024)
+    quant_i8_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int8_t* __restrict__ q,
+                    int64_t ldq, float* __restrict__ scale, int group) {
+  constexpr int N = 16 / sizeof(T);
+  __shared__ float part[32];
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const int in_row = threadIdx.x & (group - 1);
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
+  const int64_t vecs = r < rows ? (cols + N - 1) / N : 0;
+  const T* row = x + r * ldx;
+  float f[kInRegisters ? kVecs : 1][N];
+  float amax = 0.0f;
+  if (kInRegisters) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+      if (in_row + u * group < vecs) load_vec<T, kAligned>(row, cols, in_row + u * group, f[u]);
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+      if (in_row + u * group < vecs) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) amax = max_nan(amax, fabsf(f[u][j]));
+      }
+  } else {
+    for (int64_t i = in_row; i < vecs; i += group) {
+      load_vec<T, kAligned>(row, cols, i, f[0]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) amax = max_nan(amax, fabsf(f[0][j]));
+    }
+  }
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  if (group > 32) {
+    if (lane == 0) part[warp] = amax;
+    __syncthreads();
+    const int first = (threadIdx.x & ~(group - 1)) >> 5;
+    amax = part[first + (lane & (group / 32 - 1))];
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  }
+  const float s = max_nan(amax / 127.0f, 1e-12f);
+  if (r < rows && in_row == 0) scale[r] = s;
+  int8_t* qr = q + r * ldq;
+  if (kInRegisters) {
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+      if (in_row + u * group < vecs) store_codes<T, kAligned>(qr, cols, in_row + u * group, s, f[u]);
+  } else {
+    for (int64_t i = in_row; i < vecs; i += group) {
+      load_vec<T, kAligned>(row, cols, i, f[0]);
+      store_codes<T, kAligned>(qr, cols, i, s, f[0]);
+    }
+  }
+}
+
+template <typename T>
+int launch_quant(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq, float* scale,
+                 cudaStream_t s) {
+  constexpr int N = 16 / sizeof(T);
+  const int64_t vecs = (cols + N - 1) / N;
+  int group = 32;
+  while (group < 1024 && int64_t(group) * kVecs < vecs) group *= 2;
+  const bool fits = int64_t(group) * kVecs >= vecs;
+  const bool aligned = aligned16(x) && ldx * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % N == 0 && ldq % N == 0;
+  const int block = group > kBlock ? group : kBlock;
+  const int64_t per_block = block / group;
+  const int64_t grid = (rows + per_block - 1) / per_block;
+  if (grid > INT32_MAX) return fail(B2M_ERR_ARG, "quant_i8: too many rows (%lld)", (long long)rows);
+  auto kernel = aligned ? (fits ? quant_i8_kernel<T, true, true> : quant_i8_kernel<T, true, false>)
+                        : (fits ? quant_i8_kernel<T, false, true> : quant_i8_kernel<T, false, false>);
+  kernel<<<static_cast<int>(grid), block, 0, s>>>(static_cast<const T*>(x), rows, cols, ldx, static_cast<int8_t*>(q),
+                                                  ldq, scale, group);
+  return check_cuda(cudaGetLastError(), "quant_i8 launch");
+}
+
+}  // namespace
+}  // namespace b2m
+
+extern "C" int b2m_quant_i8(const void* x, int32_t in_type, int64_t rows, int64_t cols, int64_t ldx, void* q,
+                            int64_t ldq, float* scale, void* stream) {
+  using namespace b2m;
+  if (rows < 0 || cols < 1 || cols > (int64_t(1) << 30) || ldx < cols || ldq < cols)
+    return fail(B2M_ERR_ARG, "quant_i8: bad shape [%lld, %lld], row strides %lld and %lld", (long long)rows,
+                (long long)cols, (long long)ldx, (long long)ldq);
+  if (in_type != B2M_BF16 && in_type != B2M_FP16 && in_type != B2M_FP32)
+    return fail(B2M_ERR_ARG, "quant_i8: unknown input type %d", in_type);
+  if (rows > 0 && (!x || !q || !scale)) return fail(B2M_ERR_ARG, "quant_i8: null pointer");
+  if (reinterpret_cast<uintptr_t>(x) % (in_type == B2M_FP32 ? 4 : 2))
+    return fail(B2M_ERR_ARG, "quant_i8: misaligned input");
+  int num_sms = 0;
+  B2M_TRY(require_sm100(&num_sms));
+  if (rows == 0) return B2M_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (in_type == B2M_BF16) return launch_quant<__nv_bfloat16>(x, rows, cols, ldx, q, ldq, scale, s);
+  if (in_type == B2M_FP16) return launch_quant<__half>(x, rows, cols, ldx, q, ldq, scale, s);
+  return launch_quant<float>(x, rows, cols, ldx, q, ldq, scale, s);
+}

@@ -251,3 +251,247 @@ def route_topk(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = Non
     _lib.call("b2m_route_topk", logits.data_ptr(), tokens, experts, top_k, _ptr(bias), ids.data_ptr(), wts.data_ptr(),
               _stream(logits.device))
     return ids, wts
+
+
+# ---------------------------------------------------------------- products over expert segments, 8-bit integers
+TYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _ld(t: torch.Tensor, dim: int, least: int) -> int:
+    """Stride of ``dim``; for an axis of one entry (whose stride says nothing) the smallest that the kernels take."""
+    if t.shape[dim] > 1:
+        return t.stride(dim)
+    per = 16 // t.element_size()
+    return (least + per - 1) // per * per
+
+
+def _ldo(out: torch.Tensor) -> int:
+    """Elements between an output's rows."""
+    return out.stride(-2) if out.shape[-2] > 1 else out.shape[-1]
+
+
+def _on(t: torch.Tensor):
+    """Makes the tensor's device current for a launch."""
+    return torch.cuda.device(t.device)
+
+
+def _operand(t: torch.Tensor, name: str, dim: int, dtype: torch.dtype, device: torch.device) -> None:
+    _need(t.dim() == dim and t.dtype == dtype and t.device == device and (t.shape[-1] <= 1 or t.stride(-1) == 1),
+          f"{name} must be {dim}-D {dtype} on {device} with unit stride along its last axis")
+
+
+def _segments(ends: torch.Tensor, experts: int, device: torch.device) -> None:
+    _need(ends.dtype == torch.int32 and ends.device == device and tuple(ends.shape) == (experts,) and
+          ends.is_contiguous(), f"ends must be contiguous int32 [{experts}] on {device}")
+
+
+def _scale_vec(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> None:
+    _need(t.dtype == torch.float32 and t.device == device and tuple(t.shape) == shape and t.is_contiguous(),
+          f"{name} must be contiguous fp32 {list(shape)} on {device}")
+
+
+def _status_word(status: torch.Tensor | None, device: torch.device) -> None:
+    _need(status is None or (status.dtype == torch.int32 and status.device == device and status.numel() >= 1),
+          f"status must be int32 [1] on {device}")
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """First byte and the byte behind the last one that a tensor reaches."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _output(out: torch.Tensor | None, shape: tuple, dtypes: tuple, out_dtype: torch.dtype | None, like: torch.Tensor,
+            inputs: tuple) -> torch.Tensor:
+    if out is None:
+        dtype = dtypes[0] if out_dtype is None else out_dtype
+        _need(dtype in dtypes, f"out_dtype must be one of {list(dtypes)}")
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    _need(out_dtype is None or out_dtype == out.dtype, "out_dtype differs from out's")
+    _need(tuple(out.shape) == shape and out.dtype in dtypes and out.device == like.device and
+          (shape[-1] <= 1 or out.stride(-1) == 1),
+          f"out must be {list(shape)} of {list(dtypes)} on {like.device} with unit stride along its last axis")
+    lo, hi = _extent(out)
+    for t in inputs:
+        a, b = _extent(t)
+        _need(hi <= a or b <= lo, "out overlaps an input")
+    return out
+
+
+def _grouped_checks(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, axis: int, name: str) -> None:
+    _cuda(x, name)
+    _need(x.dtype in (torch.bfloat16, torch.float16), f"{name} must be bf16 or fp16")
+    _operand(x, name, 2, x.dtype, x.device)
+    _operand(w, "w", 3, x.dtype, x.device)
+    _need(w.shape[axis] == x.shape[1], f"{name} is {list(x.shape)} and w {list(w.shape)}: the summed axes differ")
+    _segments(ends, w.shape[0], x.device)
+
+
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.Tensor | None = None,
+               out_dtype: torch.dtype | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows sorted by expert times that expert's weights: ``y[t] = x[t] @ w[e].T`` for rows ``ends[e-1] <= t < ends[e]``.
+
+    x bf16 / fp16 [T, K], w the same type [E, N, K], ends int32 [E] on the device (cumulative row counts; empty
+    segments allowed, E <= 1024) -> [T, N] of the input type or fp32.  No segment is padded and nothing is read back
+    to the host.  Rows behind ``ends[-1]`` are zero in an output allocated here and left alone in ``out``.  Rows of x
+    and w are a multiple of 16 bytes apart and 16-byte aligned.  ``status`` (``new_status``) records ends that are
+    out of order, which are otherwise taken as the nearest ones in order.
+
+    Differentiable in x and w without ``out`` and ``out_dtype``; a weight gradient covers every expert (zero where a
+    segment is empty).  As with any autograd function, a backward pass is captured into a CUDA graph only when no
+    graph of the same leaves that was recorded outside the capture is still alive."""
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        _need(out is None and out_dtype in (None, x.dtype), "gradients need out=None and the input's type as out_dtype")
+        return _GroupedMM.apply(x, w, ends, status)
+    _grouped_checks(x, w, ends, 2, "x")
+    experts, n, k = w.shape
+    clear = out is None
+    out = _output(out, (x.shape[0], n), (x.dtype, torch.float32), out_dtype, x, (x, w, ends))
+    _status_word(status, x.device)
+    ldw = _ld(w, 1, k)
+    with _on(x):
+        _lib.call("b2m_grouped_mm", x.data_ptr(), x.shape[0], _ld(x, 0, k), w.data_ptr(), experts, n, k, ldw,
+                  w.stride(0) if experts > 1 else n * ldw, ends.data_ptr(), TYPE_CODES[x.dtype], out.data_ptr(),
+                  _ldo(out), TYPE_CODES[out.dtype], int(clear), _ptr(status), _stream(x.device))
+    return out
+
+
+def grouped_mm_dx(dy: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.Tensor | None = None,
+                  out_dtype: torch.dtype | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of ``grouped_mm``'s rows: ``dx[t] = dy[t] @ w[e]``.  dy [T, N], w [E, N, K] -> [T, K]; types, strides,
+    ends, status and the rows behind ``ends[-1]`` as there."""
+    _grouped_checks(dy, w, ends, 1, "dy")
+    experts, n, k = w.shape
+    clear = out is None
+    out = _output(out, (dy.shape[0], k), (dy.dtype, torch.float32), out_dtype, dy, (dy, w, ends))
+    _status_word(status, dy.device)
+    ldw = _ld(w, 1, k)
+    with _on(dy):
+        _lib.call("b2m_grouped_mm_dx", dy.data_ptr(), dy.shape[0], _ld(dy, 0, n), w.data_ptr(), experts, n, k, ldw,
+                  w.stride(0) if experts > 1 else n * ldw, ends.data_ptr(), TYPE_CODES[dy.dtype], out.data_ptr(),
+                  _ldo(out), TYPE_CODES[out.dtype], int(clear), _ptr(status), _stream(dy.device))
+    return out
+
+
+def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: torch.Tensor | None = None,
+                  out_dtype: torch.dtype | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of ``grouped_mm``'s weights: ``dw[e] = dy[seg e].T @ x[seg e]``, zero for an empty segment.
+
+    dy [T, N], x [T, K] -> [E, N, K] of the input type or fp32; types, strides, ends and status as there.  Rows behind
+    ``ends[-1]`` enter no sum, whatever they hold."""
+    _cuda(dy, "dy")
+    _need(dy.dtype in (torch.bfloat16, torch.float16), "dy must be bf16 or fp16")
+    _operand(dy, "dy", 2, dy.dtype, dy.device)
+    _operand(x, "x", 2, dy.dtype, dy.device)
+    rows, n = dy.shape
+    k = x.shape[1]
+    _need(x.shape[0] == rows, f"dy has {rows} rows and x {x.shape[0]}")
+    _need(ends.dim() == 1, "ends must be int32 [E]")
+    _segments(ends, ends.shape[0], dy.device)
+    out = _output(out, (ends.shape[0], n, k), (dy.dtype, torch.float32), out_dtype, dy, (dy, x, ends))
+    _status_word(status, dy.device)
+    ldo = _ldo(out)
+    with _on(dy):
+        _lib.call("b2m_grouped_mm_dw", dy.data_ptr(), _ld(dy, 0, n), x.data_ptr(), _ld(x, 0, k), rows, n, k,
+                  ends.data_ptr(), ends.shape[0], TYPE_CODES[dy.dtype], out.data_ptr(), ldo,
+                  out.stride(0) if ends.shape[0] > 1 else n * ldo, TYPE_CODES[out.dtype], _ptr(status),
+                  _stream(dy.device))
+    return out
+
+
+def _kernel_rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself when the kernels can read its rows, else a copy whose rows are (a gradient that torch hands over
+    may be expanded, transposed or of a width that is no multiple of 16 bytes)."""
+    rows, cols = t.shape
+    if (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or (t.stride(0) >= cols and t.stride(0) % 8 == 0)) and \
+            t.data_ptr() % 16 == 0:
+        return t
+    return torch.empty((rows, (cols + 7) // 8 * 8), dtype=t.dtype, device=t.device)[:, :cols].copy_(t)
+
+
+class _GroupedMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, ends, status):
+        y = grouped_mm(x.detach(), w.detach(), ends, status=status)
+        ctx.save_for_backward(x, w, ends)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, ends = ctx.saved_tensors
+        dy = _kernel_rows(dy)
+        dx = grouped_mm_dx(dy, w, ends) if ctx.needs_input_grad[0] else None
+        dw = grouped_mm_dw(dy, x, ends) if ctx.needs_input_grad[1] else None
+        return dx, dw, None, None
+
+
+def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tensor | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 / fp16 / fp32 [rows, cols] -> (int8 [rows, cols], fp32 [rows]): ``scale = max(amax / 127, 1e-12)``,
+    ``q = rne(x / scale)`` within +-127, both divisions IEEE fp32.
+
+    Token codes of activations, or channel codes of weights (one row for each output channel).  A row that holds a
+    NaN (an infinity) gets a NaN (infinite) scale, and a product with it becomes NaN."""
+    _cuda(x, "x")
+    _need(x.dim() == 2 and x.dtype in TYPE_CODES and (x.shape[1] <= 1 or x.stride(1) == 1),
+          "x must be 2D bf16, fp16 or fp32 with unit column stride")
+    rows, cols = x.shape
+    if q is None:
+        q = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _operand(q, "q", 2, torch.int8, x.device)
+    _need(tuple(q.shape) == (rows, cols) and (rows <= 1 or q.stride(0) >= cols), "bad q buffer")
+    _scale_vec(scale, "scale", (rows,), x.device)
+    with _on(x):
+        _lib.call("b2m_quant_i8", x.data_ptr(), TYPE_CODES[x.dtype], rows, cols, x.stride(0) if rows > 1 else cols,
+                  q.data_ptr(), q.stride(0) if rows > 1 else cols, scale.data_ptr(), _stream(x.device))
+    return q, scale
+
+
+def _int8(a, a_scale, w, w_scale, ends, out, out_dtype, status):
+    _cuda(a, "a")
+    _operand(a, "a", 2, torch.int8, a.device)
+    _operand(w, "w", 3, torch.int8, a.device)
+    experts, n, k = w.shape
+    rows = a.shape[0]
+    _need(a.shape[1] == k, f"a is {list(a.shape)} and w {list(w.shape)}: the summed axes differ")
+    _scale_vec(a_scale, "a_scale", (rows,), a.device)
+    clear = out is None
+    inputs = (a, w, a_scale, w_scale) if ends is None else (a, w, a_scale, w_scale, ends)
+    out = _output(out, (rows, n), (torch.bfloat16, torch.float16, torch.float32), out_dtype, a, inputs)
+    _status_word(status, a.device)
+    ldw = _ld(w, 1, k)
+    with _on(a):
+        _lib.call("b2m_int8_mm", a.data_ptr(), a_scale.data_ptr(), rows, _ld(a, 0, k), w.data_ptr(),
+                  w_scale.data_ptr(), experts, n, k, ldw, w.stride(0) if experts > 1 else n * ldw, _ptr(ends),
+                  out.data_ptr(), _ldo(out), TYPE_CODES[out.dtype], int(clear), _ptr(status), _stream(a.device))
+    return out
+
+
+def int8_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+            out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """8-bit integer product with scales for each token and channel: ``y = (a @ w.T) * a_scale[:, None] * w_scale``.
+
+    a int8 [M, K], w int8 [N, K] (``quant_int8`` of the activations and of the weights), a_scale fp32 [M], w_scale
+    fp32 [N] -> [M, N] in bf16 (default), fp16 or fp32.  The integer sums are exact (K <= 131071); rows of a and w
+    are a multiple of 16 bytes apart and 16-byte aligned."""
+    _need(w.dim() == 2, "w must be 2-D int8 [N, K]")
+    _cuda(a, "a")
+    _scale_vec(w_scale, "w_scale", (w.shape[0],), a.device)
+    return _int8(a, a_scale, w.unsqueeze(0), w_scale, None, out, out_dtype, None)
+
+
+def int8_grouped_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                    ends: torch.Tensor, out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+                    status: torch.Tensor | None = None) -> torch.Tensor:
+    """``int8_mm`` over expert segments: a int8 [T, K], w int8 [E, N, K], a_scale fp32 [T], w_scale fp32 [E, N], ends
+    int32 [E] -> [T, N]; ends, status and the rows behind ``ends[-1]`` as in ``grouped_mm``."""
+    _need(w.dim() == 3, "w must be 3-D int8 [E, N, K]")
+    _cuda(a, "a")
+    _segments(ends, w.shape[0], a.device)
+    _scale_vec(w_scale, "w_scale", tuple(w.shape[:2]), a.device)
+    return _int8(a, a_scale, w, w_scale, ends, out, out_dtype, status)

@@ -1,0 +1,493 @@
+"""Products over expert segments and 8-bit integer products against plain sums in 64 bits.
+
+Tolerances.  A 16-bit output is off by its rounding, half a step of the value (``eps / 2``), and by the fp32 sum before
+it: each of the L additions of a sum loses at most one part in 2^23 of a partial sum (an adder that cuts off instead of
+rounding loses up to a whole step), and no partial sum passes S = sum |x||w|, so L * 2^-23 * S.  Integer sums are exact:
+their outputs are those of the three fp32 roundings that the definition names, bit for bit.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from tests.conftest import cuda_ok  # noqa: E402
+
+if not cuda_ok():
+    pytest.skip("needs an sm_100 GPU", allow_module_level=True)
+
+from td_benchmark_b200 import configs, data, ops  # noqa: E402
+
+DEV = torch.device("cuda", 0)
+TYPES = [torch.bfloat16, torch.float16]
+
+
+def _randn(*shape, seed=0, dtype=torch.bfloat16, std=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * std).to(dtype).to(DEV)
+
+
+def _ends(counts):
+    return torch.tensor(counts, dtype=torch.int64).cumsum(0).to(torch.int32).to(DEV)
+
+
+def _spans(counts):
+    at = 0
+    for e, c in enumerate(counts):
+        yield e, slice(at, at + c)
+        at += c
+
+
+def _close(got, want, mass, length):
+    """want and mass (the sums of absolute products) in 64 bits; length = products in a sum."""
+    assert got.shape == want.shape
+    lost = length * 2.0 ** -23 * mass
+    # fp16 results below its normal range are rounded to half of its smallest step
+    tol = torch.finfo(got.dtype).eps / 2 * (want.abs() + lost) + lost + torch.finfo(got.dtype).smallest_normal * \
+        torch.finfo(got.dtype).eps / 2
+    worst = ((got.double() - want).abs() - tol).max().item() if got.numel() else -1.0
+    assert worst <= 0, f"past the tolerance by {worst}"
+
+
+def _fwd(x, w, counts):
+    y = x.new_zeros((x.shape[0], w.shape[1]), dtype=torch.float64)
+    for e, s in _spans(counts):
+        y[s] = x[s].double() @ w[e].double().T
+    return y
+
+
+def _dx(dy, w, counts):
+    return _fwd(dy, w.transpose(1, 2), counts)
+
+
+def _dw(dy, x, counts):
+    return torch.stack([dy[s].double().T @ x[s].double() for _, s in _spans(counts)])
+
+
+# (rows of each expert, rows behind them, N, K)
+SHAPES = [
+    ([1], 0, 8, 8),
+    ([1], 0, 128, 64),
+    ([16], 3, 256, 72),
+    ([0, 0, 5, 0], 0, 136, 16),
+    ([7, 0, 300, 17, 0, 1], 11, 200, 328),
+    ([33, 257, 0, 31], 0, 520, 136),
+    ([513], 1, 304, 1000),
+    ([0, 0, 0], 9, 64, 64),
+    ([64, 128, 256, 63, 65, 255], 40, 128, 256),
+    ([1] * 200 + [0] * 56 + [3] * 10, 2, 264, 192),
+    ([2, 0, 0, 1] * 256, 0, 64, 128),
+    ([5000, 3, 1200], 5, 640, 704),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("counts,slack,n,k", SHAPES)
+def test_products_over_segments(counts, slack, n, k, dtype):
+    rows = sum(counts) + slack
+    x, dy = _randn(rows, k, seed=1, dtype=dtype), _randn(rows, n, seed=2, dtype=dtype)
+    w = _randn(len(counts), n, k, seed=3, dtype=dtype, std=0.1)
+    ends = _ends(counts)
+    status = ops.new_status(DEV)
+    y = ops.grouped_mm(x, w, ends, status=status)
+    dx = ops.grouped_mm_dx(dy, w, ends, status=status)
+    dw = ops.grouped_mm_dw(dy, x, ends, status=status)
+    torch.cuda.synchronize()
+    ops.check_status(status)
+    _close(y, _fwd(x, w, counts), _fwd(x.abs(), w.abs(), counts), k)
+    _close(dx, _dx(dy, w, counts), _dx(dy.abs(), w.abs(), counts), n)
+    _close(dw, _dw(dy, x, counts), _dw(dy.abs(), x.abs(), counts), max(counts))
+    if slack:
+        assert not y[-slack:].any() and not dx[-slack:].any()
+
+
+@pytest.mark.parametrize("counts,n,k", [([7, 0, 300, 17], 201, 136), ([3, 1], 1, 64), ([40], 127, 24),
+                                        ([300, 2], 1025, 104)])
+def test_odd_widths_and_fp32_outputs(counts, n, k):
+    """N needs no alignment in a product; a summed axis needs it only in its row stride."""
+    rows = sum(counts)
+    pad = torch.full((rows, k + 8), float("nan"), device=DEV, dtype=torch.bfloat16)
+    wide = torch.full((len(counts), n, k + 16), float("nan"), device=DEV, dtype=torch.bfloat16)
+    x, w = pad[:, :k - 3], wide[:, :, :k - 3]
+    x.copy_(_randn(rows, k - 3, seed=4))
+    w.copy_(_randn(len(counts), n, k - 3, seed=5))
+    y = ops.grouped_mm(x, w, _ends(counts), out_dtype=torch.float32)
+    assert y.dtype == torch.float32
+    _close(y, _fwd(x, w, counts), _fwd(x.abs(), w.abs(), counts), k)
+    dy = torch.full((rows, (n + 15) // 8 * 8), float("nan"), device=DEV, dtype=torch.bfloat16)[:, :n]
+    dy.copy_(_randn(rows, n, seed=6))
+    dx = ops.grouped_mm_dx(dy, w, _ends(counts), out_dtype=torch.float32)
+    dw = ops.grouped_mm_dw(dy, x, _ends(counts), out_dtype=torch.float32)
+    _close(dx, _dx(dy, w, counts), _dx(dy.abs(), w.abs(), counts), n)
+    _close(dw, _dw(dy, x, counts), _dw(dy.abs(), x.abs(), counts), max(counts))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_rows_of_no_expert_enter_nothing(bad):
+    """Rows behind the last segment, and another segment's rows, reach no other output whatever they hold."""
+    counts, n, k = [5, 70, 0, 129], 136, 200
+    rows = sum(counts)
+    x, dy = _randn(rows + 30, k, seed=7), _randn(rows + 30, n, seed=8)
+    w = _randn(4, n, k, seed=9)
+    x[rows:], dy[rows:] = bad, bad
+    x[5:75], dy[5:75] = bad, bad            # the second expert's rows
+    ends = _ends(counts)
+    y, dx, dw = ops.grouped_mm(x, w, ends), ops.grouped_mm_dx(dy, w, ends), ops.grouped_mm_dw(dy, x, ends)
+    keep = [0, 2, 3]
+    others = torch.cat([torch.arange(5), torch.arange(75, rows + 30)]).to(DEV)
+    assert torch.isfinite(y[others]).all() and torch.isfinite(dx[others]).all() and torch.isfinite(dw[keep]).all()
+    assert not torch.isfinite(y[5:75]).any() and not torch.isfinite(dw[1]).any()
+    clean = [5, 0, 0, 129]
+    cx, cdy = torch.cat([x[:5], x[75:rows]]), torch.cat([dy[:5], dy[75:rows]])
+    _close(dw[keep], _dw(cdy, cx, clean)[keep], _dw(cdy.abs(), cx.abs(), clean)[keep], 129)
+    _close(y[75:rows], _fwd(cx, w, clean)[5:], _fwd(cx.abs(), w.abs(), clean)[5:], k)
+
+
+def test_given_output_keeps_rows_of_no_expert_and_columns_beside_it():
+    counts, n, k = [3, 40], 72, 64
+    x, w, ends = _randn(50, k, seed=1), _randn(2, n, k, seed=2), _ends(counts)
+    buf = torch.full((50, n + 24), 7.0, device=DEV, dtype=torch.bfloat16)
+    out = buf[:, 8:8 + n]
+    assert ops.grouped_mm(x, w, ends, out=out) is out
+    _close(out[:43], _fwd(x, w, counts)[:43], _fwd(x.abs(), w.abs(), counts)[:43], k)
+    assert (buf[43:] == 7).all() and (buf[:, :8] == 7).all() and (buf[:, 8 + n:] == 7).all()
+    big = torch.full((2, n, k + 8), 7.0, device=DEV, dtype=torch.float32)
+    ops.grouped_mm_dw(_randn(50, n, seed=3), x, ends, out=big[:, :, :k])
+    assert (big[:, :, k:] == 7).all() and not (big[:, :, :k] == 7).any()
+
+
+def test_no_rows():
+    w, ends = _randn(3, 64, 32, seed=1), _ends([0, 0, 0])
+    x, dy = _randn(0, 32), _randn(0, 64)
+    assert ops.grouped_mm(x, w, ends).shape == (0, 64) and ops.grouped_mm_dx(dy, w, ends).shape == (0, 32)
+    dw = ops.grouped_mm_dw(dy, x, ends, out=torch.full((3, 64, 32), 5.0, device=DEV, dtype=torch.bfloat16))
+    torch.cuda.synchronize()
+    assert not dw.any()
+    q, s = ops.quant_int8(_randn(0, 32))
+    assert q.shape == (0, 32) and s.shape == (0,)
+
+
+def test_ends_out_of_order_are_recorded_and_contained():
+    """An end below an earlier one leaves its segment empty, one past the rows ends at the last row."""
+    n, k = 64, 64
+    x, w = _randn(40, k, seed=1), _randn(4, n, k, seed=2)
+    status = ops.new_status(DEV)
+    guard = torch.full((60, n), 7.0, device=DEV, dtype=torch.bfloat16)
+    ends = torch.tensor([10, 4, -3, 1 << 30], dtype=torch.int32, device=DEV)
+    ops.grouped_mm(x, w, ends, out=guard[:40], status=status)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="BAD_ROUTING"):
+        ops.check_status(status)
+    _close(guard[:40], _fwd(x, w, [10, 0, 0, 30]), _fwd(x.abs(), w.abs(), [10, 0, 0, 30]), k)
+    assert (guard[40:] == 7).all()
+    for bad in ([-1, 10, 20, 40], [41, 41, 41, 41], [10, 20, 19, 40]):
+        status.zero_()
+        ops.grouped_mm_dw(_randn(40, n, seed=3), x, torch.tensor(bad, dtype=torch.int32, device=DEV), status=status)
+        assert status.item() == 0x201, bad
+    status.zero_()
+    ops.grouped_mm(x, w, torch.tensor([0, 10, 10, 40], dtype=torch.int32, device=DEV), status=status)
+    assert status.item() == 0
+
+
+def test_offsets_past_32_bits():
+    """The last expert's weights, and the last rows, lie more than 2^32 bytes into their tensors."""
+    n, k, experts = 4096, 8192, 66
+    w = torch.empty((experts, n, k), dtype=torch.bfloat16, device=DEV)      # 4.4 GB
+    w[-1] = _randn(n, k, seed=1)
+    w[0] = 0
+    counts = [2] + [0] * (experts - 2) + [3]
+    x = _randn(5, k, seed=2)
+    y = ops.grouped_mm(x, w, _ends(counts))
+    want = x[2:].double() @ w[-1].double().T
+    _close(y[2:], want, x[2:].abs().double() @ w[-1].abs().double().T, k)
+    dy = _randn(5, n, seed=3)
+    w.zero_()
+    dw = ops.grouped_mm_dw(dy, x, _ends(counts), out=w)
+    _close(dw[-1], dy[2:].double().T @ x[2:].double(), dy[2:].abs().double().T @ x[2:].abs().double(), 3)
+    del w, dw
+    rows = (1 << 31) // 512 + 300
+    big = torch.zeros((rows, 512), dtype=torch.bfloat16, device=DEV)        # rows past 2^31 elements
+    big[-3:] = _randn(3, 512, seed=4)
+    w2 = _randn(2, 1024, 512, seed=5)
+    y = ops.grouped_mm(big, w2, torch.tensor([rows - 2, rows], dtype=torch.int32, device=DEV))
+    _close(y[-2:], big[-2:].double() @ w2[1].double().T, big[-2:].abs().double() @ w2[1].abs().double().T, 512)
+    _close(y[-3:-2], big[-3:-2].double() @ w2[0].double().T, big[-3:-2].abs().double() @ w2[0].abs().double().T, 512)
+
+
+# ---------------------------------------------------------------- gradients
+def test_gradients_through_autograd():
+    """The gradients that torch sees are the formula's, with an expanded, a transposed and a ragged-width dy."""
+    counts, k = [4, 0, 90, 33], 72
+    rows = sum(counts) + 6
+    for n, shape in [(64, "plain"), (64, "transposed"), (64, "expanded"), (61, "plain")]:
+        x, w = _randn(rows, k, seed=1).requires_grad_(), _randn(4, n, k, seed=2).requires_grad_()
+        y = ops.grouped_mm(x, w, _ends(counts))
+        dy = {"plain": lambda: _randn(rows, n, seed=3), "transposed": lambda: _randn(n, rows, seed=3).t(),
+              "expanded": lambda: _randn(1, 1, seed=3).expand(rows, n)}[shape]()
+        gx, gw = torch.autograd.grad(y, (x, w), dy)
+        _close(gx, _dx(dy, w.detach(), counts), _dx(dy.abs(), w.detach().abs(), counts), n)
+        _close(gw, _dw(dy, x.detach(), counts), _dw(dy.abs(), x.detach().abs(), counts), max(counts))
+    only_w = torch.autograd.grad(ops.grouped_mm(x.detach(), w, _ends(counts)), w, dy)
+    assert torch.equal(only_w[0], gw)
+
+
+def test_gradients_against_differences():
+    """<g, v> is the slope of the fp32 output's weighted sum along v: the function is linear in x and in w, so the
+    difference over any step is exact but for the fp32 sums."""
+    counts, n, k = [3, 20, 0, 9], 40, 56
+    rows = sum(counts)
+    ends = _ends(counts)
+    # values on a coarse grid: x + v and w + v are exact in bf16
+    grid = lambda *s, seed: (torch.randint(-8, 9, s, generator=torch.Generator().manual_seed(seed)) / 8).to(  # noqa: E731
+        torch.bfloat16).to(DEV)
+    x, vx, w, vw = grid(rows, k, seed=1), grid(rows, k, seed=2), grid(4, n, k, seed=3), grid(4, n, k, seed=4)
+    dy = grid(rows, n, seed=5)
+    f = lambda a, b: (ops.grouped_mm(a, b, ends, out_dtype=torch.float32).double() * dy.double()).sum()  # noqa: E731
+    dx = ops.grouped_mm_dx(dy, w, ends, out_dtype=torch.float32).double()
+    dw = ops.grouped_mm_dw(dy, x, ends, out_dtype=torch.float32).double()
+    # products are multiples of 2^-6 (outputs) and 2^-9 (sums below), far inside 24 bits: every figure is exact
+    assert (f(x + vx, w) - f(x, w) - (dx * vx.double()).sum()).abs().item() == 0
+    assert (f(x, w + vw) - f(x, w) - (dw * vw.double()).sum()).abs().item() == 0
+
+
+# ---------------------------------------------------------------- 8-bit integers
+def _quant_ref(x):
+    """The definition with IEEE fp32 steps, evaluated in 64 bits and rounded to 32 after each."""
+    x = x.double().cpu()
+    scale = torch.maximum(x.abs().amax(1) / 127, torch.tensor(1e-12, dtype=torch.float64)).float()
+    q = (x / scale.double()[:, None]).float().double().round().clamp(-127, 127)
+    return q.to(torch.int8), scale
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7168), (3, 7), (33, 129), (257, 64), (5, 1000), (64, 4096), (9, 8191),
+                                       (3, 32768), (2, 70001)])
+def test_quant_int8_is_exact(rows, cols, dtype):
+    x = _randn(rows, cols, seed=rows + cols, dtype=dtype, std=3.0)
+    if rows > 2:
+        x[1] = 0
+        x[2, cols // 2] = 3.0e4
+    if cols > 200:                       # quotients on and next to a tie
+        x[0, :201] = torch.arange(-100, 101).to(dtype).to(DEV) / 4
+        x[0, 5] = 127 / 4
+    q, s = ops.quant_int8(x)
+    torch.cuda.synchronize()
+    qr, sr = _quant_ref(x)
+    assert torch.equal(s.cpu(), sr)
+    assert torch.equal(q.cpu(), qr)
+
+
+def test_quant_int8_strides_and_unaligned_rows():
+    big = _randn(20, 700, seed=1)
+    for at, cols in [(0, 256), (8, 513), (3, 100), (1, 699)]:
+        x = big[:, at:at + cols]
+        q = torch.full((20, cols + 5), 99, dtype=torch.int8, device=DEV)
+        ops.quant_int8(x, q[:, 2:2 + cols])
+        qr, _ = _quant_ref(x)
+        assert torch.equal(q[:, 2:2 + cols].cpu(), qr)
+        assert (q[:, :2] == 99).all() and (q[:, 2 + cols:] == 99).all()
+
+
+def test_quant_int8_marks_rows_that_are_not_finite():
+    x = _randn(6, 300, seed=1, dtype=torch.float32)
+    x[1, 7], x[2, 0], x[3, 299] = float("nan"), float("inf"), float("-inf")
+    x[4] = 1e-30
+    q, s = ops.quant_int8(x)
+    assert torch.isnan(s[1]) and torch.isinf(s[2]) and torch.isinf(s[3])
+    assert s[4].item() == torch.tensor(1e-12).item() and not q[4].any()
+    a = torch.zeros((6, 304), dtype=torch.int8, device=DEV)
+    a[:, :300] = q
+    w = torch.ones((16, 304), dtype=torch.int8, device=DEV)
+    y = ops.int8_mm(a, s, w, torch.ones(16, device=DEV))
+    assert torch.isnan(y[1:4]).all() and torch.isfinite(y[[0, 4, 5]]).all()
+
+
+def _codes(*shape, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(-128, 128, shape, generator=g, dtype=torch.int8).to(DEV)
+
+
+def _scales(*shape, seed):
+    return (torch.rand(shape, generator=torch.Generator().manual_seed(seed)) * 0.01 + 1e-4).to(DEV)
+
+
+def _int8_ref(a, a_scale, w, w_scale, dtype):
+    sums = (a.double() @ w.double().T).float()          # exact in 64 bits, one rounding
+    return (sums * a_scale[:, None] * w_scale).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 4096, 512), (2, 129, 64), (17, 255, 1008), (33, 640, 2048),
+                                   (300, 1001, 400), (1000, 384, 7168), (257, 128, 16)])
+def test_int8_mm_is_exact(m, n, k, dtype):
+    a, w = _codes(m, k, seed=1), _codes(n, k, seed=2)
+    sa, sw = _scales(m, seed=3), _scales(n, seed=4)
+    y = ops.int8_mm(a, sa, w, sw, out_dtype=dtype)
+    torch.cuda.synchronize()
+    assert torch.equal(y, _int8_ref(a, sa, w, sw, dtype))
+
+
+def test_int8_sums_at_the_edge_of_32_bits():
+    k = 131056
+    a, w = torch.full((2, k), -128, dtype=torch.int8, device=DEV), torch.full((3, k), -128, dtype=torch.int8, device=DEV)
+    w[1] = 127
+    one = torch.ones(3, device=DEV)
+    y = ops.int8_mm(a, one[:2], w, one, out_dtype=torch.float32)
+    want = torch.tensor([128 * 128 * k, -128 * 127 * k, 128 * 128 * k], dtype=torch.float64).float()
+    assert torch.equal(y.cpu(), want.expand(2, 3))
+
+
+@pytest.mark.parametrize("counts,slack,n,k", [([1], 0, 16, 16), ([7, 0, 300, 17, 0, 1], 11, 201, 336),
+                                              ([0, 0], 4, 64, 64), ([1] * 100 + [0] * 50, 3, 130, 256),
+                                              ([700, 1, 64], 0, 512, 1040)])
+def test_int8_grouped_mm_is_exact(counts, slack, n, k):
+    rows = sum(counts) + slack
+    a, w = _codes(rows, k, seed=1), _codes(len(counts), n, k, seed=2)
+    sa, sw = _scales(rows, seed=3), _scales(len(counts), n, seed=4)
+    y = ops.int8_grouped_mm(a, sa, w, sw, _ends(counts), out_dtype=torch.float32)
+    for e, s in _spans(counts):
+        assert torch.equal(y[s], _int8_ref(a[s], sa[s], w[e], sw[e], torch.float32)), e
+    if slack:
+        assert not y[-slack:].any()
+
+
+def test_strided_integer_operands():
+    wide_a, wide_w = _codes(40, 512, seed=1), _codes(3, 90, 640, seed=2)
+    a, w = wide_a[:, 32:32 + 200], wide_w[:, 5:75, 16:216]
+    sa, sw = _scales(40, seed=3), _scales(3, 70, seed=4)
+    y = ops.int8_grouped_mm(a, sa, w, sw, _ends([11, 0, 29]), out_dtype=torch.float32)
+    assert torch.equal(y[:11], _int8_ref(a[:11], sa[:11], w[0], sw[0], torch.float32))
+    assert torch.equal(y[11:], _int8_ref(a[11:], sa[11:], w[2], sw[2], torch.float32))
+
+
+# ---------------------------------------------------------------- used together
+def _route(tokens, experts, top_k, seed):
+    logits = _randn(tokens, experts, seed=seed, dtype=torch.float32)
+    ids, wts = ops.route_topk(logits, top_k)
+    order, expert_of, _ = ops.moe_align_block_size(ids, 1, experts)       # blocks of one row: sorted, no padding
+    ends = torch.searchsorted(expert_of, torch.arange(experts, device=DEV, dtype=torch.int32), right=True)
+    return ids, wts, order.long(), ends.to(torch.int32)
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 200])
+def test_a_routed_layer_and_its_gradients(tokens):
+    """route -> sort -> gate/up product -> SiLU * up -> down product -> weighted sum, and its gradients, against the
+    same layer with one dense product for each token and expert in 64 bits.
+
+    The layer rounds h to bf16 and each product's output once, and the gradients pass the same roundings back: a chain
+    of at most five roundings of relative size 2^-8, plus fp32 sums far below them.  Each enters a sum whose terms have
+    independent signs, so the 2-norm of the difference stays below five times 2^-8 of the norm of the result."""
+    cfg = configs.preset("tiny").shape
+    e, h, inter, top_k = cfg.E, cfg.K, cfg.n_down, cfg.top_k
+    ids, wts, order, ends = _route(tokens, e, top_k, seed=tokens)
+    x = _randn(tokens, h, seed=1).requires_grad_()
+    w1 = _randn(e, 2 * inter, h, seed=2, std=h ** -0.5).requires_grad_()
+    w2 = _randn(e, h, inter, seed=3, std=inter ** -0.5).requires_grad_()
+
+    gu = ops.grouped_mm(x[order // top_k], w1, ends)
+    gate, up = gu.float().chunk(2, -1)
+    y = ops.grouped_mm((torch.nn.functional.silu(gate) * up).to(torch.bfloat16), w2, ends)
+    pairs = torch.empty_like(y).index_copy(0, order, y)
+    out = (pairs.float().view(tokens, top_k, h) * wts[..., None]).sum(1)
+    dout = _randn(tokens, h, seed=4, dtype=torch.float32)
+    grads = torch.autograd.grad(out, (x, w1, w2), dout)
+
+    xd, w1d, w2d = (t.detach().double().requires_grad_() for t in (x, w1, w2))
+    want = 0
+    for j in range(top_k):
+        g2, u2 = torch.einsum("th,tnh->tn", xd, w1d[ids[:, j].long()]).chunk(2, -1)
+        y2 = torch.einsum("ti,thi->th", torch.nn.functional.silu(g2) * u2, w2d[ids[:, j].long()])
+        want = want + y2 * wts[:, j, None].double()
+    want_grads = torch.autograd.grad(want, (xd, w1d, w2d), dout.double())
+    for got, ref in zip((out, *grads), (want, *want_grads)):
+        assert ((got.double() - ref).norm() / ref.norm()).item() < 5 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("tokens", [1, 130])
+def test_a_routed_integer_layer(tokens):
+    """The same layer with 8-bit weights and activations; the oracle takes the same codes and rounds where it does, so
+    the layer's outputs differ from it by the fp32 SiLU's last bits, which can move a code by one: 1 / 127 of a row's
+    largest value, in one of many terms."""
+    cfg = configs.preset("tiny").shape
+    e, h, inter, top_k = cfg.E, cfg.K, cfg.n_down, cfg.top_k
+    ids, wts, order, ends = _route(tokens, e, top_k, seed=tokens + 50)
+    x = _randn(tokens, h, seed=1)
+    w1, s1 = ops.quant_int8(_randn(e * 2 * inter, h, seed=2))
+    w2, s2 = ops.quant_int8(_randn(e * h, inter, seed=3))
+    w1, s1, w2, s2 = w1.view(e, 2 * inter, h), s1.view(e, 2 * inter), w2.view(e, h, inter), s2.view(e, h)
+
+    q, s = ops.quant_int8(x)
+    rows = order // top_k
+    gu = ops.int8_grouped_mm(q[rows], s[rows], w1, s1, ends, out_dtype=torch.float32)
+    gate, up = gu.chunk(2, -1)
+    hq, hs = ops.quant_int8(torch.nn.functional.silu(gate) * up)
+    y = ops.int8_grouped_mm(hq, hs, w2, s2, ends)
+    pairs = torch.empty_like(y).index_copy(0, order, y)
+    out = ops.combine((pairs.view(tokens, top_k, h) * wts[..., None]).to(torch.bfloat16).view(-1, h), top_k)
+
+    xd = q.double() * s.double()[:, None]
+    want = torch.zeros((tokens, h), dtype=torch.float64, device=DEV)
+    for j in range(top_k):
+        g2, u2 = torch.einsum("th,tnh->tn", xd, (w1.double() * s1.double()[..., None])[ids[:, j].long()]).chunk(2, -1)
+        h2 = torch.nn.functional.silu(g2) * u2
+        hs2 = h2.abs().amax(1, keepdim=True) / 127
+        h2 = (h2 / hs2).round() * hs2
+        want += torch.einsum("ti,thi->th", h2, (w2.double() * s2.double()[..., None])[ids[:, j].long()]) * \
+            wts[:, j, None].double()
+    # bf16 roundings of y and of the weighted rows and of the sum: three times 2^-8
+    assert ((out.double() - want).norm() / want.norm()).item() < 3 * 2.0 ** -8
+
+
+# ---------------------------------------------------------------- streams, graphs
+def test_other_stream_and_replayed_graph():
+    counts = [40, 0, 3, 85]
+    x, w, dy = _randn(128, 128, seed=1), _randn(4, 192, 128, seed=2), _randn(128, 192, seed=3)
+    ends = _ends(counts)
+    qa, sa = ops.quant_int8(x)
+    qw, sw = ops.quant_int8(w.view(-1, 128))
+    qw, sw = qw.view(4, 192, 128), sw.view(4, 192)
+    run = lambda: (ops.grouped_mm(x, w, ends), ops.grouped_mm_dx(dy, w, ends), ops.grouped_mm_dw(dy, x, ends),  # noqa: E731
+                   ops.int8_grouped_mm(qa, sa, qw, sw, ends), *ops.quant_int8(x))
+    eager = run()
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        other = run()
+    torch.cuda.synchronize()
+    for a, b in zip(eager, other):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    # new routing, new rows: the captured calls read both from the device
+    ends.copy_(_ends([1, 100, 0, 20]))
+    x.copy_(_randn(128, 128, seed=11))
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(held, run()):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    counts = [900, 0, 300, 700]
+    x, w = _randn(1900, 512, seed=1), _randn(4, 768, 512, seed=2)
+    ends = _ends(counts)
+    want = ops.grouped_mm(x, w, ends)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(DEV) for _ in range(2)]
+    got = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops.grouped_mm(x, w, ends))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_results_do_not_change_from_run_to_run():
+    counts = [100, 0, 3, 85, 300]
+    x, w, dy = _randn(488, 640, seed=1), _randn(5, 384, 640, seed=2), _randn(488, 384, seed=3)
+    ends = _ends(counts)
+    run = lambda: (ops.grouped_mm(x, w, ends), ops.grouped_mm_dx(dy, w, ends), ops.grouped_mm_dw(dy, x, ends))  # noqa: E731
+    first = run()
+    for _ in range(5):
+        for a, b in zip(first, run()):
+            assert torch.equal(a, b)

@@ -1,0 +1,93 @@
+"""Calls of the expert-segment and integer products that are refused, through the C ABI: no device is touched."""
+import pytest
+
+from td_benchmark_b200 import _lib
+
+BF16, FP16, FP32 = 0, 1, 2
+P = 4096          # stands for an aligned address; every call below is refused before it is used
+
+MM = dict(x=P, rows=8, ldx=64, w=P, experts=4, n=32, k=64, ldw=64, w_stride=2048, ends=P, in_type=BF16, out=P, ldo=64,
+          out_type=BF16, clear=1, status=None, stream=None)
+DW = dict(dy=P, lddy=32, x=P, ldx=64, rows=8, n=32, k=64, ends=P, experts=4, in_type=BF16, out=P, ldo=64,
+          out_stride=2048, out_type=BF16, status=None, stream=None)
+QUANT = dict(x=P, in_type=BF16, rows=4, cols=64, ldx=64, q=P, ldq=64, scale=P, stream=None)
+INT8 = dict(a=P, a_scale=P, rows=8, lda=64, w=P, w_scale=P, experts=4, n=32, k=64, ldw=64, w_stride=2048, ends=P, out=P,
+            ldo=32, out_type=BF16, clear=1, status=None, stream=None)
+
+
+@pytest.fixture(autouse=True)
+def _built():
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("libb2m.so not built")
+
+
+def _refused(fn, base, change, match):
+    with pytest.raises(_lib.B2MError, match=match) as e:
+        _lib.call(fn, *dict(base, **change).values())
+    assert e.value.code == 1          # an argument error, also where there is no GPU
+
+
+COMMON = [
+    (dict(experts=0), "experts"), (dict(experts=1025), "experts"), (dict(n=0), "extent|no rows"), (dict(k=0), "extent"),
+    (dict(rows=-1), "extent"), (dict(rows=(1 << 30) + 1), "extent"), (dict(k=1 << 31, ldx=1 << 31, ldw=1 << 31), "extent"),
+    (dict(ends=None), "ends"), (dict(out=None), "null output"), (dict(out=P + 1), "misaligned"),
+    (dict(ldo=16), "output rows"), (dict(in_type=FP32), "neither"), (dict(in_type=7), "neither"),
+    (dict(out_type=FP16), "output type"), (dict(out_type=9), "output type"),
+]
+
+
+@pytest.mark.parametrize("change,match", COMMON + [
+    (dict(ldx=68), "rows of x"), (dict(ldx=56), "rows of x"), (dict(x=None), "x must not be null"),
+    (dict(x=P + 8), "aligned"), (dict(w=P + 2), "aligned"), (dict(w=None), "w must not be null"),
+    (dict(ldw=60), "rows of w"), (dict(w_stride=0), "experts of w"), (dict(w_stride=2049), "experts of w"),
+    (dict(rows=1 << 30, n=1 << 20, ldo=1 << 20), "tiles")])
+def test_grouped_mm_refuses(change, match):
+    _refused("b2m_grouped_mm", MM, change, match)
+
+
+@pytest.mark.parametrize("change,match", [(dict(ldx=24), "rows of dy"), (dict(x=None), "dy must not be null"),
+                                          (dict(ends=None), "ends"), (dict(ldo=63), "output rows"),
+                                          (dict(ldw=72 + 1), "rows of w")])
+def test_grouped_mm_dx_refuses(change, match):
+    _refused("b2m_grouped_mm_dx", dict(MM, ldx=32), change, match)
+
+
+@pytest.mark.parametrize("change,match", [c for c in COMMON if "ldw" not in c[0]] + [
+    (dict(lddy=36), "rows of dy"), (dict(ldx=68), "rows of x"), (dict(dy=P + 4), "dy must not be null"),
+    (dict(out_stride=2047), "overlap"), (dict(ldo=48), "output rows")])
+def test_grouped_mm_dw_refuses(change, match):
+    _refused("b2m_grouped_mm_dw", DW, change, match)
+
+
+@pytest.mark.parametrize("change,match", [(dict(cols=0), "bad shape"), (dict(rows=-1), "bad shape"),
+                                          (dict(ldx=63), "bad shape"), (dict(ldq=63), "bad shape"),
+                                          (dict(in_type=3), "input type"), (dict(x=None), "null"),
+                                          (dict(q=None), "null"), (dict(scale=None), "null"),
+                                          (dict(x=P + 1), "misaligned")])
+def test_quant_i8_refuses(change, match):
+    _refused("b2m_quant_i8", QUANT, change, match)
+
+
+@pytest.mark.parametrize("change,match", [(dict(k=131072, lda=131072, ldw=131072), "32 bits"), (dict(lda=72), "rows of a"),
+                                          (dict(ldw=65), "rows of w"), (dict(a_scale=None), "scales"),
+                                          (dict(w_scale=None), "scales"), (dict(ends=None), "one expert"),
+                                          (dict(out_type=3), "output type"), (dict(a=P + 8), "aligned"),
+                                          (dict(w=P + 8), "aligned"), (dict(ldo=31), "output rows"),
+                                          (dict(experts=0), "experts")])
+def test_int8_mm_refuses(change, match):
+    _refused("b2m_int8_mm", INT8, change, match)
+
+
+def test_wrappers_refuse_host_tensors_and_wrong_shapes():
+    import torch
+
+    from td_benchmark_b200 import ops
+
+    x, w = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros((2, 32, 64), dtype=torch.bfloat16)
+    ends = torch.tensor([2, 4], dtype=torch.int32)
+    a, s = torch.zeros((4, 64), dtype=torch.int8), torch.zeros(4)
+    for call in (lambda: ops.grouped_mm(x, w, ends), lambda: ops.grouped_mm_dx(x, w, ends),
+                 lambda: ops.grouped_mm_dw(x, x, ends), lambda: ops.quant_int8(x), lambda: ops.int8_mm(a, s, a, s),
+                 lambda: ops.int8_grouped_mm(a, s, a.view(2, 2, 64), s, ends)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
