@@ -254,7 +254,20 @@ def route_topk(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = Non
 
 
 # ---------------------------------------------------------------- products over expert segments, 8-bit integers
+# One-token calls take a few microseconds on the GPU, so these wrappers keep the host's part short: messages are made
+# only when a check fails, and the device is switched only when it is not the current one.
 TYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """The C call on the tensors' device and its current stream."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+        return
+    with torch.cuda.device(index):
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _ld(t: torch.Tensor, dim: int, least: int) -> int:
@@ -270,29 +283,22 @@ def _ldo(out: torch.Tensor) -> int:
     return out.stride(-2) if out.shape[-2] > 1 else out.shape[-1]
 
 
-def _on(t: torch.Tensor):
-    """Makes the tensor's device current for a launch."""
-    return torch.cuda.device(t.device)
-
-
 def _operand(t: torch.Tensor, name: str, dim: int, dtype: torch.dtype, device: torch.device) -> None:
-    _need(t.dim() == dim and t.dtype == dtype and t.device == device and (t.shape[-1] <= 1 or t.stride(-1) == 1),
-          f"{name} must be {dim}-D {dtype} on {device} with unit stride along its last axis")
+    if t.dim() != dim or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise ValueError(f"{name} must be {dim}-D {dtype} on {device} with unit stride along its last axis")
 
 
-def _segments(ends: torch.Tensor, experts: int, device: torch.device) -> None:
-    _need(ends.dtype == torch.int32 and ends.device == device and tuple(ends.shape) == (experts,) and
-          ends.is_contiguous(), f"ends must be contiguous int32 [{experts}] on {device}")
+def _vector(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
+    if t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {dtype} {list(shape)} on {device}")
 
 
-def _scale_vec(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> None:
-    _need(t.dtype == torch.float32 and t.device == device and tuple(t.shape) == shape and t.is_contiguous(),
-          f"{name} must be contiguous fp32 {list(shape)} on {device}")
-
-
-def _status_word(status: torch.Tensor | None, device: torch.device) -> None:
-    _need(status is None or (status.dtype == torch.int32 and status.device == device and status.numel() >= 1),
+def _status_word(status: torch.Tensor | None, device: torch.device) -> int | None:
+    if status is None:
+        return None
+    _need(status.dtype == torch.int32 and status.device == device and status.numel() >= 1,
           f"status must be int32 [1] on {device}")
+    return status.data_ptr()
 
 
 def _extent(t: torch.Tensor) -> tuple[int, int]:
@@ -303,16 +309,17 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
-def _output(out: torch.Tensor | None, shape: tuple, dtypes: tuple, out_dtype: torch.dtype | None, like: torch.Tensor,
-            inputs: tuple) -> torch.Tensor:
+def _output(out: torch.Tensor | None, shape: tuple, dtypes: tuple, out_dtype: torch.dtype | None,
+            device: torch.device, inputs: tuple) -> torch.Tensor:
     if out is None:
         dtype = dtypes[0] if out_dtype is None else out_dtype
-        _need(dtype in dtypes, f"out_dtype must be one of {list(dtypes)}")
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        if dtype not in dtypes:
+            raise ValueError(f"out_dtype must be one of {list(dtypes)}")
+        return torch.empty(shape, dtype=dtype, device=device)
     _need(out_dtype is None or out_dtype == out.dtype, "out_dtype differs from out's")
-    _need(tuple(out.shape) == shape and out.dtype in dtypes and out.device == like.device and
+    _need(tuple(out.shape) == shape and out.dtype in dtypes and out.device == device and
           (shape[-1] <= 1 or out.stride(-1) == 1),
-          f"out must be {list(shape)} of {list(dtypes)} on {like.device} with unit stride along its last axis")
+          f"out must be {list(shape)} of {list(dtypes)} on {device} with unit stride along its last axis")
     lo, hi = _extent(out)
     for t in inputs:
         a, b = _extent(t)
@@ -320,13 +327,28 @@ def _output(out: torch.Tensor | None, shape: tuple, dtypes: tuple, out_dtype: to
     return out
 
 
-def _grouped_checks(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, axis: int, name: str) -> None:
+def _rows_times_weights(entry: str, name: str, x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, summed: int,
+                        out: torch.Tensor | None, out_dtype: torch.dtype | None, status: torch.Tensor | None
+                        ) -> torch.Tensor:
+    """x [T, .] times w [E, N, K] of its segment, summed over axis ``summed`` of w."""
+    dtype, device = x.dtype, x.device
     _cuda(x, name)
-    _need(x.dtype in (torch.bfloat16, torch.float16), f"{name} must be bf16 or fp16")
-    _operand(x, name, 2, x.dtype, x.device)
-    _operand(w, "w", 3, x.dtype, x.device)
-    _need(w.shape[axis] == x.shape[1], f"{name} is {list(x.shape)} and w {list(w.shape)}: the summed axes differ")
-    _segments(ends, w.shape[0], x.device)
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError(f"{name} must be bf16 or fp16")
+    _operand(x, name, 2, dtype, device)
+    _operand(w, "w", 3, dtype, device)
+    experts, n, k = w.shape
+    rows, width = x.shape
+    if width != (k if summed == 2 else n):
+        raise ValueError(f"{name} is {list(x.shape)} and w {list(w.shape)}: the summed axes differ")
+    _vector(ends, "ends", (experts,), torch.int32, device)
+    clear = out is None
+    out = _output(out, (rows, n if summed == 2 else k), (dtype, torch.float32), out_dtype, device, (x, w, ends))
+    ldw = _ld(w, 1, k)
+    _launch(device, entry, x.data_ptr(), rows, _ld(x, 0, width), w.data_ptr(), experts, n, k, ldw,
+            w.stride(0) if experts > 1 else n * ldw, ends.data_ptr(), TYPE_CODES[dtype], out.data_ptr(), _ldo(out),
+            TYPE_CODES[out.dtype], clear, _status_word(status, device))
+    return out
 
 
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.Tensor | None = None,
@@ -342,37 +364,17 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.
     Differentiable in x and w without ``out`` and ``out_dtype``; a weight gradient covers every expert (zero where a
     segment is empty).  As with any autograd function, a backward pass is captured into a CUDA graph only when no
     graph of the same leaves that was recorded outside the capture is still alive."""
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+    if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         _need(out is None and out_dtype in (None, x.dtype), "gradients need out=None and the input's type as out_dtype")
         return _GroupedMM.apply(x, w, ends, status)
-    _grouped_checks(x, w, ends, 2, "x")
-    experts, n, k = w.shape
-    clear = out is None
-    out = _output(out, (x.shape[0], n), (x.dtype, torch.float32), out_dtype, x, (x, w, ends))
-    _status_word(status, x.device)
-    ldw = _ld(w, 1, k)
-    with _on(x):
-        _lib.call("b2m_grouped_mm", x.data_ptr(), x.shape[0], _ld(x, 0, k), w.data_ptr(), experts, n, k, ldw,
-                  w.stride(0) if experts > 1 else n * ldw, ends.data_ptr(), TYPE_CODES[x.dtype], out.data_ptr(),
-                  _ldo(out), TYPE_CODES[out.dtype], int(clear), _ptr(status), _stream(x.device))
-    return out
+    return _rows_times_weights("b2m_grouped_mm", "x", x, w, ends, 2, out, out_dtype, status)
 
 
 def grouped_mm_dx(dy: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.Tensor | None = None,
                   out_dtype: torch.dtype | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of ``grouped_mm``'s rows: ``dx[t] = dy[t] @ w[e]``.  dy [T, N], w [E, N, K] -> [T, K]; types, strides,
     ends, status and the rows behind ``ends[-1]`` as there."""
-    _grouped_checks(dy, w, ends, 1, "dy")
-    experts, n, k = w.shape
-    clear = out is None
-    out = _output(out, (dy.shape[0], k), (dy.dtype, torch.float32), out_dtype, dy, (dy, w, ends))
-    _status_word(status, dy.device)
-    ldw = _ld(w, 1, k)
-    with _on(dy):
-        _lib.call("b2m_grouped_mm_dx", dy.data_ptr(), dy.shape[0], _ld(dy, 0, n), w.data_ptr(), experts, n, k, ldw,
-                  w.stride(0) if experts > 1 else n * ldw, ends.data_ptr(), TYPE_CODES[dy.dtype], out.data_ptr(),
-                  _ldo(out), TYPE_CODES[out.dtype], int(clear), _ptr(status), _stream(dy.device))
-    return out
+    return _rows_times_weights("b2m_grouped_mm_dx", "dy", dy, w, ends, 1, out, out_dtype, status)
 
 
 def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: torch.Tensor | None = None,
@@ -381,23 +383,24 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: to
 
     dy [T, N], x [T, K] -> [E, N, K] of the input type or fp32; types, strides, ends and status as there.  Rows behind
     ``ends[-1]`` enter no sum, whatever they hold."""
+    dtype, device = dy.dtype, dy.device
     _cuda(dy, "dy")
-    _need(dy.dtype in (torch.bfloat16, torch.float16), "dy must be bf16 or fp16")
-    _operand(dy, "dy", 2, dy.dtype, dy.device)
-    _operand(x, "x", 2, dy.dtype, dy.device)
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise ValueError("dy must be bf16 or fp16")
+    _operand(dy, "dy", 2, dtype, device)
+    _operand(x, "x", 2, dtype, device)
     rows, n = dy.shape
     k = x.shape[1]
-    _need(x.shape[0] == rows, f"dy has {rows} rows and x {x.shape[0]}")
+    if x.shape[0] != rows:
+        raise ValueError(f"dy has {rows} rows and x {x.shape[0]}")
     _need(ends.dim() == 1, "ends must be int32 [E]")
-    _segments(ends, ends.shape[0], dy.device)
-    out = _output(out, (ends.shape[0], n, k), (dy.dtype, torch.float32), out_dtype, dy, (dy, x, ends))
-    _status_word(status, dy.device)
+    experts = ends.shape[0]
+    _vector(ends, "ends", (experts,), torch.int32, device)
+    out = _output(out, (experts, n, k), (dtype, torch.float32), out_dtype, device, (dy, x, ends))
     ldo = _ldo(out)
-    with _on(dy):
-        _lib.call("b2m_grouped_mm_dw", dy.data_ptr(), _ld(dy, 0, n), x.data_ptr(), _ld(x, 0, k), rows, n, k,
-                  ends.data_ptr(), ends.shape[0], TYPE_CODES[dy.dtype], out.data_ptr(), ldo,
-                  out.stride(0) if ends.shape[0] > 1 else n * ldo, TYPE_CODES[out.dtype], _ptr(status),
-                  _stream(dy.device))
+    _launch(device, "b2m_grouped_mm_dw", dy.data_ptr(), _ld(dy, 0, n), x.data_ptr(), _ld(x, 0, k), rows, n, k,
+            ends.data_ptr(), experts, TYPE_CODES[dtype], out.data_ptr(), ldo,
+            out.stride(0) if experts > 1 else n * ldo, TYPE_CODES[out.dtype], _status_word(status, device))
     return out
 
 
@@ -436,39 +439,42 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
     Token codes of activations, or channel codes of weights (one row for each output channel).  A row that holds a
     NaN (an infinity) gets a NaN (infinite) scale, and a product with it becomes NaN."""
     _cuda(x, "x")
-    _need(x.dim() == 2 and x.dtype in TYPE_CODES and (x.shape[1] <= 1 or x.stride(1) == 1),
-          "x must be 2D bf16, fp16 or fp32 with unit column stride")
+    code, device = TYPE_CODES.get(x.dtype), x.device
+    if code is None or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError("x must be 2D bf16, fp16 or fp32 with unit column stride")
     rows, cols = x.shape
     if q is None:
-        q = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
+        q = torch.empty((rows, cols), dtype=torch.int8, device=device)
+        ldq = cols
+    else:
+        _operand(q, "q", 2, torch.int8, device)
+        ldq = q.stride(0) if rows > 1 else cols
+        _need(tuple(q.shape) == (rows, cols) and ldq >= cols, "bad q buffer")
+        (lo, hi), (a, b) = _extent(q), _extent(x)
+        _need(hi <= a or b <= lo, "q overlaps x")
     if scale is None:
-        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _operand(q, "q", 2, torch.int8, x.device)
-    _need(tuple(q.shape) == (rows, cols) and (rows <= 1 or q.stride(0) >= cols), "bad q buffer")
-    _scale_vec(scale, "scale", (rows,), x.device)
-    with _on(x):
-        _lib.call("b2m_quant_i8", x.data_ptr(), TYPE_CODES[x.dtype], rows, cols, x.stride(0) if rows > 1 else cols,
-                  q.data_ptr(), q.stride(0) if rows > 1 else cols, scale.data_ptr(), _stream(x.device))
+        scale = torch.empty(rows, dtype=torch.float32, device=device)
+    else:
+        _vector(scale, "scale", (rows,), torch.float32, device)
+    _launch(device, "b2m_quant_i8", x.data_ptr(), code, rows, cols, x.stride(0) if rows > 1 else cols, q.data_ptr(),
+            ldq, scale.data_ptr())
     return q, scale
 
 
-def _int8(a, a_scale, w, w_scale, ends, out, out_dtype, status):
-    _cuda(a, "a")
-    _operand(a, "a", 2, torch.int8, a.device)
-    _operand(w, "w", 3, torch.int8, a.device)
-    experts, n, k = w.shape
+def _int8(a, a_scale, w, w_scale, experts, n, k, w_stride, ends, out, out_dtype, status):
+    device = a.device
+    _operand(a, "a", 2, torch.int8, device)
     rows = a.shape[0]
-    _need(a.shape[1] == k, f"a is {list(a.shape)} and w {list(w.shape)}: the summed axes differ")
-    _scale_vec(a_scale, "a_scale", (rows,), a.device)
+    if a.shape[1] != k:
+        raise ValueError(f"a is {list(a.shape)} and w {list(w.shape)}: the summed axes differ")
+    _vector(a_scale, "a_scale", (rows,), torch.float32, device)
     clear = out is None
-    inputs = (a, w, a_scale, w_scale) if ends is None else (a, w, a_scale, w_scale, ends)
-    out = _output(out, (rows, n), (torch.bfloat16, torch.float16, torch.float32), out_dtype, a, inputs)
-    _status_word(status, a.device)
-    ldw = _ld(w, 1, k)
-    with _on(a):
-        _lib.call("b2m_int8_mm", a.data_ptr(), a_scale.data_ptr(), rows, _ld(a, 0, k), w.data_ptr(),
-                  w_scale.data_ptr(), experts, n, k, ldw, w.stride(0) if experts > 1 else n * ldw, _ptr(ends),
-                  out.data_ptr(), _ldo(out), TYPE_CODES[out.dtype], int(clear), _ptr(status), _stream(a.device))
+    out = _output(out, (rows, n), FLOATS, out_dtype, device,
+                  (a, w, a_scale, w_scale) if ends is None else (a, w, a_scale, w_scale, ends))
+    ldw = _ld(w, -2, k)
+    _launch(device, "b2m_int8_mm", a.data_ptr(), a_scale.data_ptr(), rows, _ld(a, 0, k), w.data_ptr(),
+            w_scale.data_ptr(), experts, n, k, ldw, n * ldw if experts == 1 else w_stride, _ptr(ends), out.data_ptr(),
+            _ldo(out), TYPE_CODES[out.dtype], clear, _status_word(status, device))
     return out
 
 
@@ -479,10 +485,11 @@ def int8_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     a int8 [M, K], w int8 [N, K] (``quant_int8`` of the activations and of the weights), a_scale fp32 [M], w_scale
     fp32 [N] -> [M, N] in bf16 (default), fp16 or fp32.  The integer sums are exact (K <= 131071); rows of a and w
     are a multiple of 16 bytes apart and 16-byte aligned."""
-    _need(w.dim() == 2, "w must be 2-D int8 [N, K]")
     _cuda(a, "a")
-    _scale_vec(w_scale, "w_scale", (w.shape[0],), a.device)
-    return _int8(a, a_scale, w.unsqueeze(0), w_scale, None, out, out_dtype, None)
+    _operand(w, "w", 2, torch.int8, a.device)
+    n, k = w.shape
+    _vector(w_scale, "w_scale", (n,), torch.float32, a.device)
+    return _int8(a, a_scale, w, w_scale, 1, n, k, 0, None, out, out_dtype, None)
 
 
 def int8_grouped_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -490,8 +497,9 @@ def int8_grouped_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
                     status: torch.Tensor | None = None) -> torch.Tensor:
     """``int8_mm`` over expert segments: a int8 [T, K], w int8 [E, N, K], a_scale fp32 [T], w_scale fp32 [E, N], ends
     int32 [E] -> [T, N]; ends, status and the rows behind ``ends[-1]`` as in ``grouped_mm``."""
-    _need(w.dim() == 3, "w must be 3-D int8 [E, N, K]")
     _cuda(a, "a")
-    _segments(ends, w.shape[0], a.device)
-    _scale_vec(w_scale, "w_scale", tuple(w.shape[:2]), a.device)
-    return _int8(a, a_scale, w, w_scale, ends, out, out_dtype, status)
+    _operand(w, "w", 3, torch.int8, a.device)
+    experts, n, k = w.shape
+    _vector(ends, "ends", (experts,), torch.int32, a.device)
+    _vector(w_scale, "w_scale", (experts, n), torch.float32, a.device)
+    return _int8(a, a_scale, w, w_scale, experts, n, k, w.stride(0), ends, out, out_dtype, status)
