@@ -13,13 +13,14 @@
 // tile.  Operands read across their rows are "MN-major": 64 of M or N in a 128-byte
 // swizzled row, one such row for each index of the sum.
 //
-// One persistent CTA per SM: warp 0 feeds a ring of TMA stages, warp 1 issues tcgen05.mma
-// into one of two TMEM accumulators, warps 4-11 turn the other one into output rows.
+// Persistent CTAs, one on each SM, in pairs (M = 256 over both) unless segments are short:
+// warp 0 feeds a ring of TMA stages, warp 1 issues tcgen05.mma into one of two TMEM
+// accumulators, warps 4-11 turn the other one into output rows.
 // Every sum is one fp32 (or exact int32) accumulator in TMEM from the first product to
 // the last, rounded once.
 //
 // Rows that a tile loads beyond its segment are other output rows in kFwd and kDx, computed
-// and never stored.  In kDw they would enter the sum: warp 1 clears them (in both operands,
+// and never stored.  In kDw they would enter the sum: warp 2 clears them (in both operands,
 // so an infinity there cannot meet a zero) in the segment's last stage before its MMA.
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -34,7 +35,7 @@ namespace {
 
 enum Mode { kFwd = 0, kDx = 1, kDw = 2 };
 
-constexpr int kM = 128;            // output columns of a tile (TMEM lanes)
+constexpr int kM = 128;            // output columns of a CTA's part of a tile (TMEM lanes)
 constexpr int kRowBytes = 128;     // one swizzled shared-memory row
 constexpr int kMaxExperts = 1024;
 constexpr int kThreads = 384;
@@ -43,20 +44,31 @@ constexpr int kABytes = kM * kRowBytes;
 constexpr int kBand = 8;           // row tiles walked together, so that they share a weight tile in L2
 constexpr int kSmallBox = 32;      // rows of one TMA box of a tile that is not full
 
-template <int NT>
+// A tile is NT output rows by 128 output columns, or, for a pair of CTAs, by 256: each CTA
+// keeps the operand rows and the accumulator of its own 128 columns and half of the row
+// operand, and the leader's MMAs (cta_group::2) read both halves.
+template <int kRows, bool kTwoCtas>
 struct Shape {
-  static constexpr int kBBytes = NT * kRowBytes;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = NT >= 256 ? 4 : (NT >= 128 ? 6 : 9);
+  static constexpr int NT = kRows;
+  static constexpr bool kPair = kTwoCtas;
+  static constexpr int kCtas = kPair ? 2 : 1;
+  static constexpr int kTileM = kM * kCtas;
+  static constexpr int kBRows = NT / kCtas;         // rows of the row operand in one CTA
+  static constexpr int kStep = 16 * kCtas;          // granularity of N in an MMA
+  static constexpr int kStageBytes = kABytes + kBRows * kRowBytes;
+  static constexpr int kStages = kPair ? 6 : 9;
   static constexpr uint32_t kTmemCols = 2 * NT;
 };
+using Wide = Shape<256, true>;
+using Narrow = Shape<32, false>;
 
-template <int NT>
+template <class S>
 struct Control {
-  uint64_t full[Shape<NT>::kStages];
-  uint64_t empty[Shape<NT>::kStages];
-  uint64_t tfull[2];
-  uint64_t tempty[2];
+  uint64_t full[S::kStages];    // operands landed; of a pair, the leader's counts both CTAs' copies
+  uint64_t empty[S::kStages];   // the stage's MMAs are done
+  uint64_t landed[S::kStages];  // kDw: this CTA's own copies landed (warp 2 passes that on to `full`)
+  uint64_t tfull[2];            // accumulator ready
+  uint64_t tempty[2];           // accumulator read; of a pair, the leader's counts both CTAs' warps
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort;
@@ -66,9 +78,9 @@ struct Control {
   int32_t tile0[kMaxExperts + 2];  // row tiles before segment e
 };
 
-template <int NT>
+template <class S>
 constexpr size_t smem_bytes() {
-  return size_t(Shape<NT>::kStages) * Shape<NT>::kStageBytes + sizeof(Control<NT>) + 1024;
+  return size_t(S::kStages) * S::kStageBytes + sizeof(Control<S>) + 1024;
 }
 
 struct Params {
@@ -77,7 +89,7 @@ struct Params {
   int32_t segments;      // experts, plus one for the rows behind the last segment when they are cleared
   int64_t rows;
   int32_t m_dim;         // extent of the output's contiguous axis
-  int32_t m_tiles;
+  int32_t m_tiles;       // tiles along it
   int32_t c_dim;         // kDw: output rows of one expert
   int32_t c_tiles;       // kDw
   int32_t k_blocks;      // kFwd, kDx: blocks of the sum
@@ -93,7 +105,7 @@ struct Params {
 };
 
 // One output tile: rows [row0, row0 + cols) of the output (kDw: of expert e's output),
-// columns [m0, m0 + 128).  k_blocks == 0: all zero, nothing is multiplied.
+// columns from m0.  k_blocks == 0: all zero, nothing is multiplied.
 struct Tile {
   int e;
   int m0;
@@ -104,8 +116,8 @@ struct Tile {
   int sum_rows;  // kDw: rows of the sum
 };
 
-template <int NT>
-__device__ __forceinline__ int find_segment(const Control<NT>* C, int segments, int slot) {
+template <class S>
+__device__ __forceinline__ int find_segment(const Control<S>* C, int segments, int slot) {
   int lo = 0, hi = segments - 1;  // the last segment whose first tile is <= slot
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -117,8 +129,8 @@ __device__ __forceinline__ int find_segment(const Control<NT>* C, int segments, 
   return lo;
 }
 
-template <int kMode, int NT>
-__device__ __forceinline__ Tile tile_at(const Params& p, const Control<NT>* C, int t) {
+template <int kMode, class S>
+__device__ __forceinline__ Tile tile_at(const Params& p, const Control<S>* C, int t) {
   Tile r;
   int tiles, i;  // row tiles of the segment, and this tile's index among the segment's tiles
   if (kMode == kDw) {
@@ -135,17 +147,17 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Control<NT>* C, i
   const int in_band = i - band * kBand * p.m_tiles;
   const int wide = min(kBand, tiles - band * kBand);
   const int m = in_band / wide;
-  const int c0 = (band * kBand + in_band - m * wide) * NT;
-  r.m0 = m * kM;
+  const int c0 = (band * kBand + in_band - m * wide) * S::NT;
+  r.m0 = m * S::kTileM;
   if (kMode == kDw) {
     r.row0 = c0;
-    r.cols = min(NT, p.c_dim - c0);
+    r.cols = min(S::NT, p.c_dim - c0);
     r.sum0 = C->start[r.e];
     r.sum_rows = C->start[r.e + 1] - C->start[r.e];
     r.k_blocks = (r.sum_rows + 63) >> 6;
   } else {
     r.row0 = static_cast<int64_t>(C->start[r.e]) + c0;
-    r.cols = min(NT, C->start[r.e + 1] - C->start[r.e] - c0);
+    r.cols = min(S::NT, C->start[r.e + 1] - C->start[r.e] - c0);
     r.k_blocks = r.e < p.experts ? p.k_blocks : 0;
     r.sum0 = 0;
     r.sum_rows = 0;
@@ -153,11 +165,18 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Control<NT>* C, i
   return r;
 }
 
+// Columns of a tile as an MMA takes them: N is a multiple of 16 (of 32 for a pair).
+template <class S>
+__device__ __forceinline__ int mma_cols(int cols) {
+  return (cols + S::kStep - 1) / S::kStep * S::kStep;
+}
+
 // Segment starts and row-tile counts from `ends`, by all threads.  An end that is below an
 // earlier one or outside [0, rows] is taken as the nearest one that is in order, and noted
 // in the status word.  Returns the number of tiles.
-template <int kMode, int NT>
-__device__ __forceinline__ int plan_segments(const Params& p, Control<NT>* C) {
+template <int kMode, class S>
+__device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
+  constexpr int NT = S::NT;
   constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = static_cast<int>(p.rows);
@@ -233,40 +252,85 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t chunk_
   return d | static_cast<uint64_t>(chunk_bytes >> 4) << 16;
 }
 
-template <bool kI8>
+template <bool kI8, bool kPair>
 __device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                     uint32_t accumulate) {
-  if (kI8)
+#define B2M_MMA(group, kind)                                                                      \
+  asm volatile(                                                                                   \
+      "{\n\t.reg .pred p;\n\t"                                                                    \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                                 \
+      "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),  \
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)                                         \
+      : "memory")
+  if (kI8 && kPair)
+    B2M_MMA("2", "i8");
+  else if (kI8)
+    B2M_MMA("1", "i8");
+  else if (kPair)
+    B2M_MMA("2", "f16");
+  else
+    B2M_MMA("1", "f16");
+#undef B2M_MMA
+}
+
+// Tiled loads whose bytes are counted on the barrier at `bar`, an address in the cluster's
+// shared memory (of a pair: the leader's barrier).  No multicast.
+template <bool kPair>
+__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
+  if (kPair)
+    tma_load_2d_pair(dst, map, bar, x, y);
+  else
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+template <bool kPair>
+__device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
+                                        int32_t z) {
+  if (kPair)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
   else
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 
-template <int kMode, bool kI8, int NT>
+// Place of this CTA in its pair, and of the pair in the grid.
+struct Where {
+  uint32_t rank;
+  int first;   // first tile
+  int stride;  // tiles between two of this pair (or CTA)
+};
+
+// Warp 0, one lane: this CTA's operands of every stage.
+template <int kMode, bool kI8, class S>
 __device__ __forceinline__ void producer(const CUtensorMap* map_a, const CUtensorMap* map_b,
                                          const CUtensorMap* map_b_small, const Params& p, uint8_t* smem,
-                                         Control<NT>* C, int num_tiles) {
-  using S = Shape<NT>;
+                                         Control<S>* C, int num_tiles, const Where& at) {
   constexpr int kElems = kI8 ? 128 : 64;  // elements in a 128-byte row
+  // kDw: every CTA counts its own bytes, and warp 2 tells the leader
+  uint64_t* const landed = kMode == kDw ? C->landed : C->full;
+  const bool counts = kMode == kDw || at.rank == 0;
+  constexpr int kSources = kMode == kDw ? 1 : S::kCtas;
   uint32_t kg = 0;
   bool alive = true;
-  for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
-    const Tile r = tile_at<kMode, NT>(p, C, t);
-    // 32-row boxes (kDw: 64-column chunks) that the tile's columns need
-    const int boxes = kMode == kDw ? (r.cols + 63) / 64 : (r.cols + kSmallBox - 1) / kSmallBox;
-    const bool whole = kMode != kDw && boxes * kSmallBox == NT;
-    const uint32_t bytes = kABytes + boxes * (kMode == kDw ? 64 : kSmallBox) * kRowBytes;
-    const int row = static_cast<int>(r.row0);
+  for (int t = at.first; t < num_tiles && alive; t += at.stride) {
+    const Tile r = tile_at<kMode, S>(p, C, t);
+    const int half = mma_cols<S>(r.cols) / S::kCtas;  // rows of the row operand in this CTA
+    const int box = kMode == kDw ? 64 : kSmallBox;
+    const int boxes = (half + box - 1) / box;
+    const bool whole = kMode != kDw && half == S::kBRows;
+    const uint32_t bytes = kABytes + boxes * box * kRowBytes;
+    const int row = static_cast<int>(r.row0) + static_cast<int>(at.rank) * half;
+    const int m0 = r.m0 + static_cast<int>(at.rank) * kM;
     for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
       const int s = kg % S::kStages;
       if (!mbar_wait(&C->empty[s], ((kg / S::kStages) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_PRODUCER,
@@ -276,97 +340,117 @@ __device__ __forceinline__ void producer(const CUtensorMap* map_a, const CUtenso
       }
       uint8_t* a = smem + s * S::kStageBytes;
       uint8_t* b = a + kABytes;
-      uint64_t* bar = &C->full[s];
-      mbar_arrive_expect_tx(bar, bytes);
+      uint32_t bar = smem_u32(&landed[s]);
+      if (S::kPair && kMode != kDw) bar = mapa_shared(bar, 0);
+      if (counts) mbar_arrive_expect_tx(&landed[s], kSources * bytes);
       if (kMode == kFwd) {
-        tma_load_3d(a, map_a, bar, kb * kElems, r.m0, r.e);
+        load_3d<S::kPair>(a, map_a, bar, kb * kElems, m0, r.e);
       } else if (kMode == kDx) {
-        tma_load_3d(a, map_a, bar, r.m0, kb * 64, r.e);
-        tma_load_3d(a + kABytes / 2, map_a, bar, r.m0 + 64, kb * 64, r.e);
+        load_3d<S::kPair>(a, map_a, bar, m0, kb * 64, r.e);
+        load_3d<S::kPair>(a + kABytes / 2, map_a, bar, m0 + 64, kb * 64, r.e);
       } else {
-        const int at = static_cast<int>(r.sum0) + kb * 64;
-        tma_load_2d(a, map_a, bar, r.m0, at);
-        tma_load_2d(a + kABytes / 2, map_a, bar, r.m0 + 64, at);
-        for (int i = 0; i < boxes; ++i) tma_load_2d(b + i * 64 * kRowBytes, map_b, bar, row + i * 64, at);
+        const int sum = static_cast<int>(r.sum0) + kb * 64;
+        load_2d<false>(a, map_a, bar, m0, sum);
+        load_2d<false>(a + kABytes / 2, map_a, bar, m0 + 64, sum);
+        for (int i = 0; i < boxes; ++i) load_2d<false>(b + i * 64 * kRowBytes, map_b, bar, row + i * 64, sum);
       }
       if (kMode != kDw) {
         if (whole)
-          tma_load_2d(b, map_b, bar, kb * kElems, row);
+          load_2d<S::kPair>(b, map_b, bar, kb * kElems, row);
         else
           for (int i = 0; i < boxes; ++i)
-            tma_load_2d(b + i * kSmallBox * kRowBytes, map_b_small, bar, kb * kElems, row + i * kSmallBox);
+            load_2d<S::kPair>(b + i * kSmallBox * kRowBytes, map_b_small, bar, kb * kElems, row + i * kSmallBox);
       }
     }
   }
   // the copies of the last stages must have landed before the CTA exits
+  if (!counts) return;
   const uint32_t first = kg > S::kStages ? kg - S::kStages : 0;
   for (uint32_t i = first; i < kg; ++i)
-    mbar_wait(&C->full[i % S::kStages], (i / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN,
-              nullptr);
+    mbar_wait(&landed[i % S::kStages], (i / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
 }
 
-// Warp 1.  All lanes wait (they clear the rows behind a kDw segment together), lane 0 issues.
-template <int kMode, bool kI8, int NT>
-__device__ __forceinline__ void mma_warp(const Params& p, uint8_t* smem, Control<NT>* C, int num_tiles,
-                                         uint32_t tmem_base, int lane) {
-  using S = Shape<NT>;
-  uint32_t kg = 0, used = 0;
-  bool alive = true;
-  for (int t = blockIdx.x; t < num_tiles && alive; t += gridDim.x) {
-    const Tile r = tile_at<kMode, NT>(p, C, t);
-    if (r.k_blocks == 0) continue;
-    const int buf = used & 1;
-    int ok = mbar_wait(&C->tempty[buf], ((used >> 1) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
-                       &C->abort);
-    if (!__all_sync(0xffffffffu, ok)) break;
-    const uint32_t d = tmem_base + static_cast<uint32_t>(buf * NT);
-    const uint32_t idesc = p.idesc | (static_cast<uint32_t>((r.cols + 15) >> 4 << 1) << 17);
+// Warp 2 of kDw: when this CTA's copies of a stage have landed, clears the rows behind the
+// segment and hands the stage to the (leader's) MMA warp.
+template <class S>
+__device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, Control<S>* C, int num_tiles,
+                                            const Where& at, int lane) {
+  uint32_t kg = 0;
+  for (int t = at.first; t < num_tiles; t += at.stride) {
+    const Tile r = tile_at<kDw, S>(p, C, t);
+    const int chunks = 2 + (mma_cols<S>(r.cols) / S::kCtas + 63) / 64;  // 64 columns each, of both operands
     for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
       const int s = kg % S::kStages;
-      ok = mbar_wait(&C->full[s], (kg / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort);
-      if (!__all_sync(0xffffffffu, ok)) {
+      const int ok = mbar_wait(&C->landed[s], (kg / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
+                               &C->abort);
+      if (!__all_sync(0xffffffffu, ok)) return;
+      const int left = r.sum_rows - kb * 64;
+      if (left < 64) {
+        const int vecs = ((left + 15) / 16 * 16 - left) * (kRowBytes / 16);  // 16-byte pieces of a chunk
+        uint8_t* rows = smem + s * S::kStageBytes + left * kRowBytes;
+        for (int i = lane; i < vecs * chunks; i += 32) {
+          const int chunk = i / vecs;
+          *reinterpret_cast<uint4*>(rows + chunk * 64 * kRowBytes + (i - chunk * vecs) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&C->full[s]), 0));
+    }
+  }
+}
+
+// Warp 1 (of a pair: the leader's), one lane issuing.
+template <int kMode, bool kI8, class S>
+__device__ __forceinline__ void mma_thread(const Params& p, uint8_t* smem, Control<S>* C, int num_tiles,
+                                           uint32_t tmem_base, const Where& at) {
+  uint32_t kg = 0, used = 0;
+  bool alive = true;
+  for (int t = at.first; t < num_tiles && alive; t += at.stride) {
+    const Tile r = tile_at<kMode, S>(p, C, t);
+    if (r.k_blocks == 0) continue;
+    const int buf = used & 1;
+    if (!mbar_wait(&C->tempty[buf], ((used >> 1) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort))
+      break;
+    const uint32_t d = tmem_base + static_cast<uint32_t>(buf * S::NT);
+    const uint32_t idesc = p.idesc | (static_cast<uint32_t>(mma_cols<S>(r.cols)) >> 3 << 17);
+    for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
+      const int s = kg % S::kStages;
+      if (!mbar_wait(&C->full[s], (kg / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort)) {
         alive = false;
         break;
       }
-      uint8_t* a = smem + s * S::kStageBytes;
-      int steps = 4;
-      if (kMode == kDw) {
-        const int left = r.sum_rows - kb * 64;
-        if (left < 64) {
-          steps = (left + 15) >> 4;
-          const int vecs = (steps * 16 - left) * (kRowBytes / 16);  // 16-byte pieces to clear in a chunk
-          const int chunks = 2 + (r.cols + 63) / 64;                // of both operands: B follows A
-          for (int i = lane; i < vecs * chunks; i += 32) {
-            const int chunk = i / vecs, at = i - chunk * vecs;
-            *reinterpret_cast<uint4*>(a + chunk * 64 * kRowBytes + left * kRowBytes + at * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-      }
-      if (lane == 0) {
-        tc_fence_after();
-        const uint32_t as = smem_u32(a), bs = as + kABytes;
-        const uint64_t adesc = kMode == kFwd ? smem_desc_sw128(as) : smem_desc_mn(as, kABytes / 2);
-        const uint64_t bdesc = kMode == kDw ? smem_desc_mn(bs, 64 * kRowBytes) : smem_desc_sw128(bs);
-        // 32 bytes of the sum in each step: within the row, or 16 rows further on
-        constexpr uint64_t a_step = kMode == kFwd ? 2 : 128, b_step = kMode == kDw ? 128 : 2;
-        for (int k = 0; k < steps; ++k)
-          mma<kI8>(d, adesc + a_step * k, bdesc + b_step * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
+      tc_fence_after();
+      const uint32_t as = smem_u32(smem + s * S::kStageBytes), bs = as + kABytes;
+      const uint64_t adesc = kMode == kFwd ? smem_desc_sw128(as) : smem_desc_mn(as, kABytes / 2);
+      const uint64_t bdesc = kMode == kDw ? smem_desc_mn(bs, 64 * kRowBytes) : smem_desc_sw128(bs);
+      // 32 bytes of the sum in each step: within the row, or 16 rows further on
+      constexpr uint64_t a_step = kMode == kFwd ? 2 : 128, b_step = kMode == kDw ? 128 : 2;
+      const int steps = kMode == kDw ? min(4, (r.sum_rows - kb * 64 + 15) >> 4) : 4;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (kMode != kDw || k < steps)
+          mma<kI8, S::kPair>(d, adesc + a_step * k, bdesc + b_step * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
+      if (S::kPair)
+        mma_commit_pair(&C->empty[s], 0x3);
+      else
         mma_commit(&C->empty[s]);
-        if (kb == r.k_blocks - 1) mma_commit(&C->tfull[buf]);
-      }
-      __syncwarp();
     }
+    if (!alive) break;
+    if (S::kPair)
+      mma_commit_pair(&C->tfull[buf], 0x3);
+    else
+      mma_commit(&C->tfull[buf]);
     ++used;
   }
   // every MMA issued here has completed before TMEM is freed
-  if (lane == 0 && kg > 0) {
-    mma_commit(&C->mma_done);
+  if (kg > 0) {
+    if (S::kPair)
+      mma_commit_pair(&C->mma_done, 0x1);
+    else
+      mma_commit(&C->mma_done);
     mbar_wait(&C->mma_done, 0, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
   }
-  __syncwarp();
 }
 
 template <typename T>
@@ -393,17 +477,17 @@ __device__ __forceinline__ void store_rows(void* out, int64_t at, int64_t ldo, i
     if (j < n) o[j * ldo] = round_to<T>(v[j]);
 }
 
-template <int kMode, bool kI8, int NT>
-__device__ __forceinline__ void epilogue(const Params& p, Control<NT>* C, int num_tiles, uint32_t tmem_base, int warp,
-                                         int lane) {
+template <int kMode, bool kI8, class S>
+__device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, int num_tiles, uint32_t tmem_base,
+                                         const Where& at, int warp, int lane) {
   const int q = warp & 3;  // TMEM lane quarter of this warp
   const int h = (warp - 4) >> 2;
   const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
   uint32_t used = 0;
-  for (int t = blockIdx.x; t < num_tiles; t += gridDim.x) {
-    const Tile r = tile_at<kMode, NT>(p, C, t);
+  for (int t = at.first; t < num_tiles; t += at.stride) {
+    const Tile r = tile_at<kMode, S>(p, C, t);
     const int buf = used & 1;
-    const int m = r.m0 + q * 32 + lane;
+    const int m = r.m0 + static_cast<int>(at.rank) * kM + q * 32 + lane;
     const bool in = m < p.m_dim;
     float ws = 0.0f;
     if (kI8 && in && r.k_blocks) ws = __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + m);
@@ -418,7 +502,7 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<NT>* C, int nu
       float v[32];
       const int n = min(32, r.cols - c);
       if (r.k_blocks) {
-        tmem_ld32(tmem_base + lane_off + static_cast<uint32_t>(buf * NT + c), v);
+        tmem_ld32(tmem_base + lane_off + static_cast<uint32_t>(buf * S::NT + c), v);
         tmem_ld_wait();
         if (kI8) {
           const float as = lane < n ? __ldg(p.a_scale + r.row0 + c + lane) : 0.0f;
@@ -431,43 +515,50 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<NT>* C, int nu
         for (int j = 0; j < 32; ++j) v[j] = 0.0f;
       }
       if (in) {
-        const int64_t at = base + c * p.ldo;
+        const int64_t o = base + c * p.ldo;
         if (p.out_type == B2M_BF16)
-          store_rows<__nv_bfloat16>(p.out, at, p.ldo, n, v);
+          store_rows<__nv_bfloat16>(p.out, o, p.ldo, n, v);
         else if (p.out_type == B2M_FP16)
-          store_rows<__half>(p.out, at, p.ldo, n, v);
+          store_rows<__half>(p.out, o, p.ldo, n, v);
         else
-          store_rows<float>(p.out, at, p.ldo, n, v);
+          store_rows<float>(p.out, o, p.ldo, n, v);
       }
       __syncwarp();
     }
     if (r.k_blocks) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&C->tempty[buf]);
+      if (lane == 0) {
+        if (S::kPair)
+          mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(&C->tempty[buf]), 0));
+        else
+          mbar_arrive(&C->tempty[buf]);
+      }
       ++used;
     }
   }
 }
 
-template <int kMode, bool kI8, int NT>
+template <int kMode, bool kI8, class S>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_b_small, const __grid_constant__ Params p) {
-  using S = Shape<NT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Control<NT>* C = reinterpret_cast<Control<NT>*>(smem + S::kStages * S::kStageBytes);
+  Control<S>* C = reinterpret_cast<Control<S>*>(smem + S::kStages * S::kStageBytes);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const Where at{S::kPair ? cluster_ctarank() : 0u, static_cast<int>(blockIdx.x) / S::kCtas,
+                 static_cast<int>(gridDim.x) / S::kCtas};
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(&C->full[s], 1);
+      mbar_init(&C->full[s], kMode == kDw ? S::kCtas : 1);
       mbar_init(&C->empty[s], 1);
+      mbar_init(&C->landed[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&C->tfull[b], 1);
-      mbar_init(&C->tempty[b], kEpiWarps);
+      mbar_init(&C->tempty[b], S::kCtas * kEpiWarps);
     }
     mbar_init(&C->mma_done, 1);
     C->abort = 0;
@@ -478,25 +569,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (kMode != kDw) tma_prefetch_desc(&map_b_small);
     }
   }
-  if (warp == 1) tmem_alloc(&C->tmem_base, S::kTmemCols);
-  const int num_tiles = plan_segments<kMode, NT>(p, C);
+  if (warp == 1) {
+    if (S::kPair)
+      tmem_alloc_pair(&C->tmem_base, S::kTmemCols);
+    else
+      tmem_alloc(&C->tmem_base, S::kTmemCols);
+  }
+  const int num_tiles = plan_segments<kMode, S>(p, C);
   tc_fence_before();
-  __syncthreads();
+  if (S::kPair)
+    cluster_sync();  // both CTAs' barriers exist before one CTA signals the other's
+  else
+    __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = C->tmem_base;
   if (warp == 0) {
-    if (lane == 0) producer<kMode, kI8, NT>(&map_a, &map_b, &map_b_small, p, smem, C, num_tiles);
+    if (lane == 0) producer<kMode, kI8, S>(&map_a, &map_b, &map_b_small, p, smem, C, num_tiles, at);
     __syncwarp();
   } else if (warp == 1) {
-    mma_warp<kMode, kI8, NT>(p, smem, C, num_tiles, tmem_base, lane);
+    if (lane == 0 && at.rank == 0) mma_thread<kMode, kI8, S>(p, smem, C, num_tiles, tmem_base, at);
+    __syncwarp();
+  } else if (warp == 2) {
+    if (kMode == kDw) clear_tails<S>(p, smem, C, num_tiles, at, lane);
   } else if (warp >= 4) {
-    epilogue<kMode, kI8, NT>(p, C, num_tiles, tmem_base, warp, lane);
+    epilogue<kMode, kI8, S>(p, C, num_tiles, tmem_base, at, warp, lane);
   }
   tc_fence_before();
   __syncthreads();
+  if (S::kPair) cluster_sync();  // the leader's MMAs and the copies it counts are done with both CTAs' memory
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, S::kTmemCols);
+    if (S::kPair)
+      tmem_dealloc_pair(tmem_base, S::kTmemCols);
+    else
+      tmem_dealloc(tmem_base, S::kTmemCols);
   }
 }
 
@@ -534,23 +640,32 @@ struct Weights {  // [experts, n, k], strides in elements
   int64_t experts, n, k, ld, expert_stride;
 };
 
-template <int kMode, bool kI8, int NT>
+template <int kMode, bool kI8, class S>
 int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& bs, const Params& p, int64_t tiles_bound,
            int num_sms, cudaStream_t s) {
-  static_assert(smem_bytes<NT>() <= 227 * 1024, "shared memory budget");
+  static_assert(smem_bytes<S>() <= 227 * 1024, "shared memory budget");
   static std::atomic<bool> attr_done[64];
   int dev = 0;
   B2M_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
-  auto kernel = grouped_kernel<kMode, kI8, NT>;
+  auto kernel = grouped_kernel<kMode, kI8, S>;
   if (dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
     B2M_TRY(check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                            static_cast<int>(smem_bytes<NT>())),
+                                            static_cast<int>(smem_bytes<S>())),
                        "grouped: cudaFuncSetAttribute"));
     if (dev < 64) attr_done[dev].store(true, std::memory_order_release);
   }
-  const int grid = static_cast<int>(tiles_bound < num_sms ? tiles_bound : num_sms);
-  kernel<<<grid, kThreads, smem_bytes<NT>(), s>>>(a, b, bs, p);
-  return check_cuda(cudaGetLastError(), "grouped launch");
+  const int64_t most = num_sms / S::kCtas;
+  cudaLaunchAttribute cluster[1];
+  cluster[0].id = cudaLaunchAttributeClusterDimension;
+  cluster[0].val.clusterDim = {static_cast<unsigned>(S::kCtas), 1, 1};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(S::kCtas * (tiles_bound < most ? tiles_bound : most)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem_bytes<S>();
+  cfg.stream = s;
+  cfg.attrs = cluster;
+  cfg.numAttrs = S::kPair ? 1 : 0;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a, b, bs, p), "grouped launch");
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
@@ -607,7 +722,10 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   p.segments = p.experts + (clear_rest ? 1 : 0);
   p.rows = x.rows;
   p.m_dim = static_cast<int32_t>(m_dim);
-  p.m_tiles = static_cast<int32_t>((m_dim + kM - 1) / kM);
+  // Row tiles of 32 while segments are short on average: the ring then holds weights, not room for rows.
+  const bool narrow = (x.rows + w.experts - 1) / w.experts <= Narrow::NT;
+  const int64_t nt = narrow ? Narrow::NT : Wide::NT, tile_m = narrow ? Narrow::kTileM : Wide::kTileM;
+  p.m_tiles = static_cast<int32_t>((m_dim + tile_m - 1) / tile_m);
   p.k_blocks = static_cast<int32_t>((sum + in_row - 1) / in_row);
   p.out = out;
   p.ldo = ldo;
@@ -618,7 +736,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   p.timeout_ns = 2 * timeout_ns();
   p.idesc = (kI8 ? (2u << 4) | (1u << 7) | (1u << 10)                                             // S32, both signed
                  : (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u)) |             // F32
-            (kMode == kDx ? 1u << 15 : 0u) | (static_cast<uint32_t>(kM >> 4) << 24);
+            (kMode == kDx ? 1u << 15 : 0u) | (static_cast<uint32_t>(tile_m >> 4) << 24);
 
   const cuuint64_t w_dims[3] = {static_cast<cuuint64_t>(w.k), static_cast<cuuint64_t>(w.n),
                                 static_cast<cuuint64_t>(w.experts)};
@@ -626,9 +744,6 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   const cuuint32_t w_box[3] = {in_row, kMode == kFwd ? static_cast<cuuint32_t>(kM) : 64u, 1};
   const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows)};
   const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
-  // Row tiles of 32 while segments are short on average: the ring then holds weights, not room for rows.
-  const int64_t mean = (x.rows + w.experts - 1) / w.experts;
-  const int64_t nt = mean <= 32 ? 32 : 256;
   const int64_t row_tiles = (x.rows + nt - 1) / nt + (x.rows < p.segments ? x.rows : p.segments);
   if (row_tiles * p.m_tiles > INT32_MAX) return fail(B2M_ERR_ARG, "%s: more than 2^31 tiles", what);
   int num_sms = 0;
@@ -639,10 +754,10 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   B2M_TRY(encode_map(&ma, type, 3, w.ptr, w_dims, w_strides, w_box, what));
   const cuuint32_t small[2] = {in_row, kSmallBox};
   B2M_TRY(encode_map(&ms, type, 2, x.ptr, x_dims, x_strides, small, what));
-  const cuuint32_t big[2] = {in_row, static_cast<cuuint32_t>(nt)};
+  const cuuint32_t big[2] = {in_row, static_cast<cuuint32_t>(narrow ? Narrow::kBRows : Wide::kBRows)};
   B2M_TRY(encode_map(&mb, type, 2, x.ptr, x_dims, x_strides, big, what));
-  if (nt == 32) return launch<kMode, kI8, 32>(ma, mb, ms, p, row_tiles * p.m_tiles, num_sms, s);
-  return launch<kMode, kI8, 256>(ma, mb, ms, p, row_tiles * p.m_tiles, num_sms, s);
+  if (narrow) return launch<kMode, kI8, Narrow>(ma, mb, ms, p, row_tiles * p.m_tiles, num_sms, s);
+  return launch<kMode, kI8, Wide>(ma, mb, ms, p, row_tiles * p.m_tiles, num_sms, s);
 }
 
 int check_16bit(const char* what, int32_t in_type) {
@@ -700,16 +815,15 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   if (!ends) return fail(B2M_ERR_ARG, "%s: null ends", what);
   B2M_TRY(check_out(what, out, k, ldo, out_type, in_type));
   if (out_stride < (n - 1) * ldo + k) return fail(B2M_ERR_ARG, "%s: experts of the output overlap", what);
-  constexpr int NT = 256;
   Params p{};
   p.ends = ends;
   p.experts = experts;
   p.segments = experts;
   p.rows = rows;
   p.m_dim = static_cast<int32_t>(k);
-  p.m_tiles = static_cast<int32_t>((k + kM - 1) / kM);
+  p.m_tiles = static_cast<int32_t>((k + Wide::kTileM - 1) / Wide::kTileM);
   p.c_dim = static_cast<int32_t>(n);
-  p.c_tiles = static_cast<int32_t>((n + NT - 1) / NT);
+  p.c_tiles = static_cast<int32_t>((n + Wide::NT - 1) / Wide::NT);
   p.out = out;
   p.ldo = ldo;
   p.out_expert = out_stride;
@@ -717,7 +831,7 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   p.status = dev_status;
   p.timeout_ns = 2 * timeout_ns();
   p.idesc = (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) |
-            (static_cast<uint32_t>(kM >> 4) << 24);
+            (static_cast<uint32_t>(Wide::kTileM >> 4) << 24);
   const int64_t tiles = int64_t(p.m_tiles) * p.c_tiles * experts;
   if (tiles > INT32_MAX) return fail(B2M_ERR_ARG, "%s: more than 2^31 tiles", what);
   int num_sms = 0;
@@ -735,7 +849,7 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
     B2M_TRY(encode_map(&ma, type, 2, x, x_dims, x_strides, box, what));
     B2M_TRY(encode_map(&mb, type, 2, dy, dy_dims, dy_strides, box, what));
   }
-  return launch<kDw, false, NT>(ma, mb, mb, p, tiles, num_sms, static_cast<cudaStream_t>(stream));
+  return launch<kDw, false, Wide>(ma, mb, mb, p, tiles, num_sms, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int b2m_int8_mm(const void* a, const float* a_scale, int64_t rows, int64_t lda, const void* w,
