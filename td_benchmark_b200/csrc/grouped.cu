@@ -42,7 +42,7 @@ constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr int kABytes = kM * kRowBytes;
 constexpr int kBand = 8;           // row tiles walked together, so that they share a weight tile in L2
-constexpr int kSmallBox = 32;      // rows of one TMA box of a tile that is not full
+constexpr int kStagePitch = 144;   // bytes between two staged output rows of 128: no bank is hit twice
 
 // A tile is NT output rows by 128 output columns, or, for a pair of CTAs, by 256: each CTA
 // keeps the operand rows and the accumulator of its own 128 columns and half of the row
@@ -54,6 +54,7 @@ struct Shape {
   static constexpr int kCtas = kPair ? 2 : 1;
   static constexpr int kTileM = kM * kCtas;
   static constexpr int kBRows = NT / kCtas;         // rows of the row operand in one CTA
+  static constexpr int kSmallRows = kBRows < 64 ? kBRows : 64;  // the same, where a tile needs no more
   static constexpr int kStep = 16 * kCtas;          // granularity of N in an MMA
   static constexpr int kStageBytes = kABytes + kBRows * kRowBytes;
   static constexpr int kStages = kPair ? 6 : 9;
@@ -66,7 +67,8 @@ template <class S>
 struct Control {
   uint64_t full[S::kStages];    // operands landed; of a pair, the leader's counts both CTAs' copies
   uint64_t empty[S::kStages];   // the stage's MMAs are done
-  uint64_t landed[S::kStages];  // kDw: this CTA's own copies landed (warp 2 passes that on to `full`)
+  uint64_t landed[S::kStages];  // kDw, last stage of a segment: this CTA's copies landed
+  uint64_t cleared[S::kStages];  // of a pair the leader's: the rows behind the segment are cleared
   uint64_t tfull[2];            // accumulator ready
   uint64_t tempty[2];           // accumulator read; of a pair, the leader's counts both CTAs' warps
   uint64_t mma_done;
@@ -76,6 +78,7 @@ struct Control {
   int32_t warp_sum[kThreads / 32];
   int32_t start[kMaxExperts + 2];  // first row of segment e; [E] = end of the last, [E + 1] = rows
   int32_t tile0[kMaxExperts + 2];  // row tiles before segment e
+  alignas(16) uint8_t staging[kEpiWarps / 2][32 * kStagePitch];  // 32 output rows of 64 columns, for two warps
 };
 
 template <class S>
@@ -98,6 +101,7 @@ struct Params {
   int64_t ldo;
   int64_t out_expert;    // kDw: elements between two experts' outputs
   int32_t out_type;
+  bool wide_out;         // 16-bit output rows are 16-byte aligned
   const float* a_scale;  // integers: scale of each row
   const float* w_scale;  // integers: scale of each weight row, [experts, m_dim]
   int32_t* status;
@@ -316,19 +320,18 @@ __device__ __forceinline__ void producer(const CUtensorMap* map_a, const CUtenso
                                          const CUtensorMap* map_b_small, const Params& p, uint8_t* smem,
                                          Control<S>* C, int num_tiles, const Where& at) {
   constexpr int kElems = kI8 ? 128 : 64;  // elements in a 128-byte row
-  // kDw: every CTA counts its own bytes, and warp 2 tells the leader
-  uint64_t* const landed = kMode == kDw ? C->landed : C->full;
-  const bool counts = kMode == kDw || at.rank == 0;
-  constexpr int kSources = kMode == kDw ? 1 : S::kCtas;
   uint32_t kg = 0;
   bool alive = true;
   for (int t = at.first; t < num_tiles && alive; t += at.stride) {
     const Tile r = tile_at<kMode, S>(p, C, t);
     const int half = mma_cols<S>(r.cols) / S::kCtas;  // rows of the row operand in this CTA
-    const int box = kMode == kDw ? 64 : kSmallBox;
-    const int boxes = (half + box - 1) / box;
-    const bool whole = kMode != kDw && half == S::kBRows;
-    const uint32_t bytes = kABytes + boxes * box * kRowBytes;
+    // One box of the row operand for each stage, of two sizes: smaller boxes in their place, as
+    // many as the tile needs, took longer to issue than the rows that they leave out (E=32,
+    // 224 rows each: 419 us in boxes of 32 rows, 385 in these).  kDw: boxes of 64 columns.
+    const bool few = kMode != kDw && half <= S::kSmallRows;
+    const int boxes = (half + 63) / 64;
+    const uint32_t bytes =
+        kABytes + (kMode == kDw ? boxes * 64 : few ? S::kSmallRows : S::kBRows) * kRowBytes;
     const int row = static_cast<int>(r.row0) + static_cast<int>(at.rank) * half;
     const int m0 = r.m0 + static_cast<int>(at.rank) * kM;
     for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
@@ -340,9 +343,16 @@ __device__ __forceinline__ void producer(const CUtensorMap* map_a, const CUtenso
       }
       uint8_t* a = smem + s * S::kStageBytes;
       uint8_t* b = a + kABytes;
-      uint32_t bar = smem_u32(&landed[s]);
-      if (S::kPair && kMode != kDw) bar = mapa_shared(bar, 0);
-      if (counts) mbar_arrive_expect_tx(&landed[s], kSources * bytes);
+      uint32_t bar = smem_u32(&C->full[s]);
+      if (S::kPair) bar = mapa_shared(bar, 0);
+      if (kMode == kDw && r.sum_rows - kb * 64 < 64) {  // warp 2 comes between the copies and the MMA
+        if (at.rank == 0) mbar_arrive(&C->full[s]);
+        mbar_arrive_expect_tx(&C->landed[s], bytes);
+        bar = smem_u32(&C->landed[s]);
+        if (S::kPair) bar = mapa_shared(bar, at.rank);
+      } else if (at.rank == 0) {
+        mbar_arrive_expect_tx(&C->full[s], S::kCtas * bytes);
+      }
       if (kMode == kFwd) {
         load_3d<S::kPair>(a, map_a, bar, kb * kElems, m0, r.e);
       } else if (kMode == kDx) {
@@ -350,53 +360,49 @@ __device__ __forceinline__ void producer(const CUtensorMap* map_a, const CUtenso
         load_3d<S::kPair>(a + kABytes / 2, map_a, bar, m0 + 64, kb * 64, r.e);
       } else {
         const int sum = static_cast<int>(r.sum0) + kb * 64;
-        load_2d<false>(a, map_a, bar, m0, sum);
-        load_2d<false>(a + kABytes / 2, map_a, bar, m0 + 64, sum);
-        for (int i = 0; i < boxes; ++i) load_2d<false>(b + i * 64 * kRowBytes, map_b, bar, row + i * 64, sum);
+        load_2d<S::kPair>(a, map_a, bar, m0, sum);
+        load_2d<S::kPair>(a + kABytes / 2, map_a, bar, m0 + 64, sum);
+        for (int i = 0; i < boxes; ++i) load_2d<S::kPair>(b + i * 64 * kRowBytes, map_b, bar, row + i * 64, sum);
       }
-      if (kMode != kDw) {
-        if (whole)
-          load_2d<S::kPair>(b, map_b, bar, kb * kElems, row);
-        else
-          for (int i = 0; i < boxes; ++i)
-            load_2d<S::kPair>(b + i * kSmallBox * kRowBytes, map_b_small, bar, kb * kElems, row + i * kSmallBox);
-      }
+      if (kMode != kDw) load_2d<S::kPair>(b, few ? map_b_small : map_b, bar, kb * kElems, row);
     }
   }
-  // the copies of the last stages must have landed before the CTA exits
-  if (!counts) return;
+  // The stages still in use are released before the CTA exits: their copies have then landed
+  // (after a timeout elsewhere, when nothing releases them, the wait ends by its limit).
   const uint32_t first = kg > S::kStages ? kg - S::kStages : 0;
   for (uint32_t i = first; i < kg; ++i)
-    mbar_wait(&landed[i % S::kStages], (i / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
+    if (!mbar_wait(&C->empty[i % S::kStages], (i / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN,
+                   nullptr))
+      break;
 }
 
-// Warp 2 of kDw: when this CTA's copies of a stage have landed, clears the rows behind the
-// segment and hands the stage to the (leader's) MMA warp.
+// Warp 2 of kDw: when this CTA's copies of a segment's last, partly filled stage have landed,
+// clears the rows behind the segment, up to the next step of the MMA, and tells the (leader's)
+// MMA warp.
 template <class S>
 __device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, Control<S>* C, int num_tiles,
                                             const Where& at, int lane) {
-  uint32_t kg = 0;
+  uint32_t kg = 0, phases = 0;  // bit s: parity of the next use of landed[s]
   for (int t = at.first; t < num_tiles; t += at.stride) {
     const Tile r = tile_at<kDw, S>(p, C, t);
+    const int left = r.sum_rows & 63;
+    kg += r.k_blocks;
+    if (left == 0) continue;
     const int chunks = 2 + (mma_cols<S>(r.cols) / S::kCtas + 63) / 64;  // 64 columns each, of both operands
-    for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
-      const int s = kg % S::kStages;
-      const int ok = mbar_wait(&C->landed[s], (kg / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
-                               &C->abort);
-      if (!__all_sync(0xffffffffu, ok)) return;
-      const int left = r.sum_rows - kb * 64;
-      if (left < 64) {
-        const int vecs = ((left + 15) / 16 * 16 - left) * (kRowBytes / 16);  // 16-byte pieces of a chunk
-        uint8_t* rows = smem + s * S::kStageBytes + left * kRowBytes;
-        for (int i = lane; i < vecs * chunks; i += 32) {
-          const int chunk = i / vecs;
-          *reinterpret_cast<uint4*>(rows + chunk * 64 * kRowBytes + (i - chunk * vecs) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&C->full[s]), 0));
+    const int s = (kg - 1) % S::kStages;
+    const int ok = mbar_wait(&C->landed[s], (phases >> s) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
+                             &C->abort);
+    if (!__all_sync(0xffffffffu, ok)) return;
+    phases ^= 1u << s;
+    const int vecs = ((left + 15) / 16 * 16 - left) * (kRowBytes / 16);  // 16-byte pieces of a chunk
+    uint8_t* rows = smem + s * S::kStageBytes + left * kRowBytes;
+    for (int i = lane; i < vecs * chunks; i += 32) {
+      const int chunk = i / vecs;
+      *reinterpret_cast<uint4*>(rows + chunk * 64 * kRowBytes + (i - chunk * vecs) * 16) = make_uint4(0, 0, 0, 0);
     }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&C->cleared[s]), 0));
   }
 }
 
@@ -404,7 +410,7 @@ __device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, Cont
 template <int kMode, bool kI8, class S>
 __device__ __forceinline__ void mma_thread(const Params& p, uint8_t* smem, Control<S>* C, int num_tiles,
                                            uint32_t tmem_base, const Where& at) {
-  uint32_t kg = 0, used = 0;
+  uint32_t kg = 0, used = 0, phases = 0;  // phases, bit s: parity of the next use of cleared[s]
   bool alive = true;
   for (int t = at.first; t < num_tiles && alive; t += at.stride) {
     const Tile r = tile_at<kMode, S>(p, C, t);
@@ -419,6 +425,13 @@ __device__ __forceinline__ void mma_thread(const Params& p, uint8_t* smem, Contr
       if (!mbar_wait(&C->full[s], (kg / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort)) {
         alive = false;
         break;
+      }
+      if (kMode == kDw && r.sum_rows - kb * 64 < 64) {
+        if (!mbar_wait(&C->cleared[s], (phases >> s) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort)) {
+          alive = false;
+          break;
+        }
+        phases ^= 1u << s;
       }
       tc_fence_after();
       const uint32_t as = smem_u32(smem + s * S::kStageBytes), bs = as + kABytes;
@@ -453,28 +466,133 @@ __device__ __forceinline__ void mma_thread(const Params& p, uint8_t* smem, Contr
   }
 }
 
-template <typename T>
-__device__ __forceinline__ T round_to(float v);
-template <>
-__device__ __forceinline__ float round_to<float>(float v) {
-  return v;
-}
-template <>
-__device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) {
-  return __float2bfloat16_rn(v);
-}
-template <>
-__device__ __forceinline__ __half round_to<__half>(float v) {
-  return __float2half_rn(v);
+// 16 TMEM lanes x 32 columns.  Thread l gets, for each group g of eight columns, lane l/4
+// (v[4g], v[4g+1]) and lane l/4 + 8 (v[4g+2], v[4g+3]) of columns 8g + 2(l%4) and the next.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 
-// Output rows row0 .. row0 + n - 1 at this lane's column: 32 lanes write 32 neighbours.
-template <typename T>
-__device__ __forceinline__ void store_rows(void* out, int64_t at, int64_t ldo, int n, const float (&v)[32]) {
-  T* o = static_cast<T*>(out) + at;
+// Four 8x8 matrices of 16-bit values, each stored transposed: thread l gives the address of
+// row l%8 of matrix l/8.
+__device__ __forceinline__ void store_matrices_t(uint32_t saddr, const uint32_t (&m)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(saddr), "r"(m[0]),
+               "r"(m[1]), "r"(m[2]), "r"(m[3])
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_16bit(float a, float b, bool bf16) {
+  if (bf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Two epilogue warps that share a staging block.
+struct Duo {
+  int bar;   // named barrier
+  int half;  // which 32 of the 64 output columns this warp holds
+  __device__ __forceinline__ void sync() const { named_bar_sync(bar, 64); }
+  // Whether both warps say yes: the warps leave the kernel's loop together or not at all.
+  __device__ __forceinline__ bool both(bool yes) const {
+    int r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, %2, 64, p;\n\t"
+        "selp.b32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(static_cast<int>(yes)), "r"(bar)
+        : "memory");
+    return r != 0;
+  }
+};
+
+// 64 output columns (TMEM lanes of two warps) of 32 output rows (TMEM columns), rounded to 16
+// bits.  An output row is contiguous along the lanes, so the block is transposed on its way
+// out: pairs of rows in a register, 8x8 matrices through stmatrix into the staging block, and
+// from there whole 128-byte lines, four in a warp's store.  (The weight gradient of E=32,
+// 4096 x 7168 took 1.08 ms with two-byte stores straight from the registers and 0.66 ms with
+// half lines, both bound by the L1's stores.)
+// `o`: the block's first element; n rows and m columns of it exist.
+template <bool kI8>
+__device__ __forceinline__ void emit_16bit(uint16_t* o, int64_t ldo, int n, int m, bool wide, bool bf16, bool zero,
+                                           uint32_t taddr, uint8_t* staging, const Duo& duo, float a_scale,
+                                           const float (&w_scale)[4], int lane) {
+  float v[32];
+  if (!zero) {
+    tmem_ld_16x32(taddr, v);
+    tmem_ld_16x32(taddr + (16u << 16), v + 16);
+    tmem_ld_wait();
+  }
+  const uint32_t to = smem_u32(staging) + (lane & 7) * kStagePitch + duo.half * 64 + (lane >> 3) * 16;
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (j < n) o[j * ldo] = round_to<T>(v[j]);
+  for (int g = 0; g < 4; ++g) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    float s0 = 1.0f, s1 = 1.0f;
+    if (kI8) {
+      s0 = __shfl_sync(0xffffffffu, a_scale, 8 * g + 2 * (lane & 3));
+      s1 = __shfl_sync(0xffffffffu, a_scale, 8 * g + 2 * (lane & 3) + 1);
+    }
+    if (!zero) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // lanes 8i .. 8i + 7
+        float x = v[(i >> 1) * 16 + 4 * g + 2 * (i & 1)], y = v[(i >> 1) * 16 + 4 * g + 2 * (i & 1) + 1];
+        if (kI8) {
+          x = __int2float_rn(__float_as_int(x)) * s0 * w_scale[i];
+          y = __int2float_rn(__float_as_int(y)) * s1 * w_scale[i];
+        }
+        w[i] = pack_16bit(x, y, bf16);
+      }
+    }
+    store_matrices_t(to + 8 * g * kStagePitch, w);
+  }
+  duo.sync();
+  const int at = (lane & 7) * 8;  // this thread's eight columns
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = 16 * duo.half + 4 * i + (lane >> 3);
+    if (j < n && at < m) {
+      const uint4 u = *reinterpret_cast<const uint4*>(staging + j * kStagePitch + at * 2);
+      uint16_t* d = o + j * ldo + at;
+      if (wide && at + 8 <= m) {
+        *reinterpret_cast<uint4*>(d) = u;
+      } else {
+        const uint32_t h[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (at + k < m) d[k] = static_cast<uint16_t>(h[k / 2] >> (16 * (k & 1)));
+      }
+    }
+  }
+  duo.sync();
+}
+
+// The same in fp32: a row's 32 columns are 128 contiguous bytes across the warp.
+template <bool kI8>
+__device__ __forceinline__ void emit_fp32(float* o, int64_t ldo, int n, int m, bool zero, uint32_t taddr,
+                                          float a_scale, float w_scale, int lane) {
+  float v[32];
+  if (!zero) {
+    tmem_ld32(taddr, v);
+    tmem_ld_wait();
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    if (zero) v[j] = 0.0f;
+    if (kI8) {
+      const float s = __shfl_sync(0xffffffffu, a_scale, j);
+      if (!zero) v[j] = __int2float_rn(__float_as_int(v[j])) * s * w_scale;
+    }
+    if (j < n && lane < m) o[j * ldo + lane] = v[j];
+  }
+  __syncwarp();
 }
 
 template <int kMode, bool kI8, class S>
@@ -483,49 +601,42 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, int num
   const int q = warp & 3;  // TMEM lane quarter of this warp
   const int h = (warp - 4) >> 2;
   const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+  const Duo duo{1 + h * 2 + (q >> 1), q & 1};
+  uint8_t* staging = C->staging[duo.bar - 1];
   uint32_t used = 0;
   for (int t = at.first; t < num_tiles; t += at.stride) {
     const Tile r = tile_at<kMode, S>(p, C, t);
     const int buf = used & 1;
-    const int m = r.m0 + static_cast<int>(at.rank) * kM + q * 32 + lane;
-    const bool in = m < p.m_dim;
-    float ws = 0.0f;
-    if (kI8 && in && r.k_blocks) ws = __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + m);
-    if (r.k_blocks) {
+    const int m0 = r.m0 + static_cast<int>(at.rank) * kM + q * 32;
+    const int m = min(32, p.m_dim - m0);  // columns of this warp that exist, and of both
+    const int m_duo = min(64, p.m_dim - m0 + duo.half * 32);
+    const bool zero = r.k_blocks == 0;
+    float w_lane = 0.0f, w_scale[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // of column m0 + lane; of the columns 8i + lane / 4
+    if (kI8 && !zero) {
+      if (lane < m) w_lane = __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + m0 + lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w_scale[i] = __shfl_sync(0xffffffffu, w_lane, 8 * i + (lane >> 2));
+    }
+    if (!zero) {
       const int ok = mbar_wait(&C->tfull[buf], (used >> 1) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_EPILOGUE,
                                &C->abort);
-      if (!__all_sync(0xffffffffu, ok)) return;
+      if (!duo.both(ok)) return;
       tc_fence_after();
     }
-    const int64_t base = (kMode == kDw ? r.e * p.out_expert : 0) + r.row0 * p.ldo + m;
-    for (int c = h * 32; c < r.cols; c += 64) {
-      float v[32];
+    const int64_t base = (kMode == kDw ? r.e * p.out_expert : 0) + r.row0 * p.ldo + m0;
+    for (int c = h * 32; c < r.cols && m_duo > 0; c += 64) {
       const int n = min(32, r.cols - c);
-      if (r.k_blocks) {
-        tmem_ld32(tmem_base + lane_off + static_cast<uint32_t>(buf * S::NT + c), v);
-        tmem_ld_wait();
-        if (kI8) {
-          const float as = lane < n ? __ldg(p.a_scale + r.row0 + c + lane) : 0.0f;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            v[j] = __int2float_rn(__float_as_int(v[j])) * __shfl_sync(0xffffffffu, as, j) * ws;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-      }
-      if (in) {
-        const int64_t o = base + c * p.ldo;
-        if (p.out_type == B2M_BF16)
-          store_rows<__nv_bfloat16>(p.out, o, p.ldo, n, v);
-        else if (p.out_type == B2M_FP16)
-          store_rows<__half>(p.out, o, p.ldo, n, v);
-        else
-          store_rows<float>(p.out, o, p.ldo, n, v);
-      }
-      __syncwarp();
+      const uint32_t taddr = tmem_base + lane_off + static_cast<uint32_t>(buf * S::NT + c);
+      float a_scale = 0.0f;
+      if (kI8 && !zero && lane < n) a_scale = __ldg(p.a_scale + r.row0 + c + lane);
+      const int64_t o = base + c * p.ldo;
+      if (p.out_type == B2M_FP32)
+        emit_fp32<kI8>(static_cast<float*>(p.out) + o, p.ldo, n, m, zero, taddr, a_scale, w_lane, lane);
+      else
+        emit_16bit<kI8>(static_cast<uint16_t*>(p.out) + o - duo.half * 32, p.ldo, n, m_duo, p.wide_out,
+                        p.out_type == B2M_BF16, zero, taddr, staging, duo, a_scale, w_scale, lane);
     }
-    if (r.k_blocks) {
+    if (!zero) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -552,9 +663,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                  static_cast<int>(gridDim.x) / S::kCtas};
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(&C->full[s], kMode == kDw ? S::kCtas : 1);
+      mbar_init(&C->full[s], 1);
       mbar_init(&C->empty[s], 1);
       mbar_init(&C->landed[s], 1);
+      mbar_init(&C->cleared[s], S::kCtas);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&C->tfull[b], 1);
@@ -730,6 +842,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   p.out = out;
   p.ldo = ldo;
   p.out_type = out_type;
+  p.wide_out = aligned16(out) && ldo % 8 == 0;
   p.a_scale = a_scale;
   p.w_scale = w_scale;
   p.status = status;
@@ -752,7 +865,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   CUtensorMap ma, mb, ms;
   B2M_TRY(encode_map(&ma, type, 3, w.ptr, w_dims, w_strides, w_box, what));
-  const cuuint32_t small[2] = {in_row, kSmallBox};
+  const cuuint32_t small[2] = {in_row, static_cast<cuuint32_t>(narrow ? Narrow::kSmallRows : Wide::kSmallRows)};
   B2M_TRY(encode_map(&ms, type, 2, x.ptr, x_dims, x_strides, small, what));
   const cuuint32_t big[2] = {in_row, static_cast<cuuint32_t>(narrow ? Narrow::kBRows : Wide::kBRows)};
   B2M_TRY(encode_map(&mb, type, 2, x.ptr, x_dims, x_strides, big, what));
@@ -828,6 +941,7 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   p.ldo = ldo;
   p.out_expert = out_stride;
   p.out_type = out_type;
+  p.wide_out = aligned16(out) && ldo % 8 == 0 && out_stride % 8 == 0;
   p.status = dev_status;
   p.timeout_ns = 2 * timeout_ns();
   p.idesc = (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) |
