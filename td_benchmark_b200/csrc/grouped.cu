@@ -42,6 +42,8 @@ constexpr int kThreads = 384;
 constexpr int kEpiWarps = 8;
 constexpr int kABytes = kM * kRowBytes;
 constexpr int kBand = 8;           // row tiles walked together, so that they share a weight tile in L2
+constexpr int kSortMost = 256;     // experts up to which segments are sorted by length
+constexpr int kFeed = 4;           // tiles found ahead
 constexpr int kStagePitch = 144;   // bytes between two staged output rows of 128: no bank is hit twice
 
 // A tile is NT output rows by 128 output columns, or, for a pair of CTAs, by 256: each CTA
@@ -54,7 +56,6 @@ struct Shape {
   static constexpr int kCtas = kPair ? 2 : 1;
   static constexpr int kTileM = kM * kCtas;
   static constexpr int kBRows = NT / kCtas;         // rows of the row operand in one CTA
-  static constexpr int kSmallRows = kBRows < 64 ? kBRows : 64;  // the same, where a tile needs no more
   static constexpr int kStep = 16 * kCtas;          // granularity of N in an MMA
   static constexpr int kStageBytes = kABytes + kBRows * kRowBytes;
   static constexpr int kStages = kPair ? 6 : 9;
@@ -62,6 +63,19 @@ struct Shape {
 };
 using Wide = Shape<256, true>;
 using Narrow = Shape<32, false>;
+
+// One output tile: rows [row0, row0 + cols) of the output (kDw: of expert e's output),
+// columns from m0.  k_blocks == 0: all zero, nothing is multiplied.  e < 0: no tile is left.
+struct alignas(16) Tile {
+  int e;
+  int m0;
+  int row0;
+  int cols;
+  int k_blocks;
+  int sum0;      // kDw: first row of the sum
+  int sum_rows;  // kDw: rows of the sum
+  int pad;
+};
 
 template <class S>
 struct Control {
@@ -76,8 +90,12 @@ struct Control {
   int abort;
   int32_t warp_max[kThreads / 32];
   int32_t warp_sum[kThreads / 32];
-  int32_t start[kMaxExperts + 2];  // first row of segment e; [E] = end of the last, [E + 1] = rows
-  int32_t tile0[kMaxExperts + 2];  // row tiles before segment e
+  uint64_t fed[kFeed];             // a tile is there
+  uint64_t taken[kFeed];           // every role has read it
+  Tile feed[kFeed];
+  alignas(16) int32_t start[kMaxExperts + 4];  // first row of segment e; [E] = end of the last, [E + 1] = rows
+  int32_t tile0[kMaxExperts + 2];  // row tiles before the segment at place r of the walk
+  uint16_t seg[kMaxExperts + 2];   // the segment at place r
   alignas(16) uint8_t staging[kEpiWarps / 2][32 * kStagePitch];  // 32 output rows of 64 columns, for two warps
 };
 
@@ -85,6 +103,13 @@ template <class S>
 constexpr size_t smem_bytes() {
   return size_t(S::kStages) * S::kStageBytes + sizeof(Control<S>) + 1024;
 }
+
+// Tensor maps: the operand whose rows or columns are the output's columns, and the row operand
+// with boxes of a quarter, half and all of the rows that a CTA can hold (kDw: rows[2] alone).
+struct Maps {
+  CUtensorMap cols;
+  CUtensorMap rows[3];
+};
 
 struct Params {
   const int32_t* ends;   // nullptr: one segment of all rows
@@ -108,18 +133,6 @@ struct Params {
   uint64_t timeout_ns;
 };
 
-// One output tile: rows [row0, row0 + cols) of the output (kDw: of expert e's output),
-// columns from m0.  k_blocks == 0: all zero, nothing is multiplied.
-struct Tile {
-  int e;
-  int m0;
-  int64_t row0;
-  int cols;
-  int k_blocks;
-  int64_t sum0;  // kDw: first row of the sum
-  int sum_rows;  // kDw: rows of the sum
-};
-
 template <class S>
 __device__ __forceinline__ int find_segment(const Control<S>* C, int segments, int slot) {
   int lo = 0, hi = segments - 1;  // the last segment whose first tile is <= slot
@@ -139,13 +152,15 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Control<S>* C, in
   int tiles, i;  // row tiles of the segment, and this tile's index among the segment's tiles
   if (kMode == kDw) {
     const int per = p.m_tiles * p.c_tiles;
-    r.e = t / per;
-    i = t - r.e * per;
+    const int place = t / per;
+    r.e = C->seg[place];
+    i = t - place * per;
     tiles = p.c_tiles;
   } else {
-    r.e = find_segment(C, p.segments, t / p.m_tiles);
-    i = t - C->tile0[r.e] * p.m_tiles;
-    tiles = C->tile0[r.e + 1] - C->tile0[r.e];
+    const int place = find_segment(C, p.segments, t / p.m_tiles);
+    r.e = C->seg[place];
+    i = t - C->tile0[place] * p.m_tiles;
+    tiles = C->tile0[place + 1] - C->tile0[place];
   }
   const int band = i / (kBand * p.m_tiles);
   const int in_band = i - band * kBand * p.m_tiles;
@@ -160,7 +175,7 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Control<S>* C, in
     r.sum_rows = C->start[r.e + 1] - C->start[r.e];
     r.k_blocks = (r.sum_rows + 63) >> 6;
   } else {
-    r.row0 = static_cast<int64_t>(C->start[r.e]) + c0;
+    r.row0 = C->start[r.e] + c0;
     r.cols = min(S::NT, C->start[r.e + 1] - C->start[r.e] - c0);
     r.k_blocks = r.e < p.experts ? p.k_blocks : 0;
     r.sum0 = 0;
@@ -169,30 +184,44 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Control<S>* C, in
   return r;
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.b32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // Columns of a tile as an MMA takes them: N is a multiple of 16 (of 32 for a pair).
 template <class S>
 __device__ __forceinline__ int mma_cols(int cols) {
   return (cols + S::kStep - 1) / S::kStep * S::kStep;
 }
 
-// Segment starts and row-tile counts from `ends`, by all threads.  An end that is below an
-// earlier one or outside [0, rows] is taken as the nearest one that is in order, and noted
-// in the status word.  Returns the number of tiles.
+// Segment starts, their order and row-tile counts from `ends`, by all threads.  An end that is
+// below an earlier one or outside [0, rows] is taken as the nearest one that is in order, and
+// noted in the status word.  Returns the number of tiles.
 template <int kMode, class S>
 __device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
   constexpr int NT = S::NT;
   constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = static_cast<int>(p.rows);
-  int v[kPer], top = 0;
+  int v[kPer], top = 0, lowest = rows;
   bool bad = false;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = tid * kPer + i;
-    const int raw = e < p.experts ? (p.ends ? __ldg(p.ends + e) : rows) : 0;
-    const int end = min(max(raw, 0), rows);
-    bad |= end != raw || (e < p.experts && end < top);
-    top = max(top, end);
+    v[i] = e < p.experts ? (p.ends ? __ldg(p.ends + e) : rows) : rows;
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    lowest = min(lowest, v[i]);
+    bad |= v[i] < top || v[i] > rows;  // below 0 is below `top`
+    if (tid * kPer + i < p.experts) top = max(top, min(v[i], rows));
     v[i] = top;
   }
   int scan = top;
@@ -203,23 +232,49 @@ __device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
   }
   if (lane == 31) C->warp_max[warp] = scan;
   __syncthreads();
-  int before = __shfl_up_sync(0xffffffffu, scan, 1);
-  if (lane == 0) before = 0;
-  for (int w = 0; w < warp; ++w) before = max(before, C->warp_max[w]);
-  if (tid * kPer < p.experts && p.ends && __ldg(p.ends + tid * kPer) < before) bad = true;
-  if (bad && blockIdx.x == 0) set_status(p.status, B2M_STATUS_BAD_ROUTING);
-  int n[kPer], sum = 0, prev = before;
+  int prev = __shfl_up_sync(0xffffffffu, scan, 1);
+  if (lane == 0) prev = 0;
+  for (int w = 0; w < warp; ++w) prev = max(prev, C->warp_max[w]);
+  if ((bad || lowest < prev) && blockIdx.x == 0) set_status(p.status, B2M_STATUS_BAD_ROUTING);
+  int n[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = tid * kPer + i;
-    const int end = max(v[i], before);
+    const int end = max(v[i], prev);
     if (e < p.experts) C->start[e] = prev;
     if (e == p.experts - 1) C->start[p.experts] = end;
     n[i] = e < p.experts ? (end - prev + NT - 1) / NT : 0;
-    sum += n[i];
     prev = end;
   }
   if (tid == 0) C->start[p.experts + 1] = rows;
+  if (S::kPair && p.experts > 1 && p.experts <= kSortMost) {  // longest segments first
+    __syncthreads();
+    if (tid < p.experts) {
+      const int mine = C->start[tid + 1] - C->start[tid];
+      int place = 0, at = 0;
+      for (int e = 0; e < p.experts; ++e) {
+        const int end = C->start[e + 1];
+        place += end - at > mine || (end - at == mine && e < tid);
+        at = end;
+      }
+      C->seg[place] = static_cast<uint16_t>(tid);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = tid * kPer + i;
+      const int e = r < p.experts ? C->seg[r] : 0;
+      n[i] = r < p.experts ? (C->start[e + 1] - C->start[e] + NT - 1) / NT : 0;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (tid * kPer + i < p.experts) C->seg[tid * kPer + i] = static_cast<uint16_t>(tid * kPer + i);
+  }
+  if (tid == 0) C->seg[p.experts] = static_cast<uint16_t>(p.experts);
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) sum += n[i];
   int acc = sum;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -235,8 +290,8 @@ __device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int e = tid * kPer + i;
-    if (e < p.experts) C->tile0[e] = at;
+    const int r = tid * kPer + i;
+    if (r < p.experts) C->tile0[r] = at;
     at += n[i];
   }
   if (tid == 0) C->tile0[p.experts] = total;
@@ -248,6 +303,72 @@ __device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
   return kMode == kDw ? p.experts * p.m_tiles * p.c_tiles : total * p.m_tiles;
 }
 
+// Place of this CTA in its pair, and of the pair in the grid.
+struct Where {
+  uint32_t rank;
+  int first;   // first tile
+  int stride;  // pairs (or CTAs) in the grid
+};
+
+// Warp 3, one lane: this CTA's tiles, on their way to its other roles.  Finding a tile takes
+// some hundred cycles of divisions and searches, longer than a short sum.  (The CTAs of a pair
+// find the same tiles each for itself: handing them over needs releases at cluster scope, which
+// wait for the epilogue's output stores, 3000 cycles a tile.)
+//
+// The pairs of a wide launch walk the tiles from both ends in turn: long segments first from
+// the front, where the tensor cores are the limit, short and empty ones from the back, where
+// memory is, so that both are busy at any time.  Every second round of tiles is dealt out
+// backwards, so that each pair gets its share of either end.
+template <int kMode, class S>
+__device__ __forceinline__ void feed_tiles(const Params& p, Control<S>* C, int num_tiles, const Where& at) {
+  uint32_t s = 0, phase = 0;
+  for (int i = 0;; ++i) {
+    int t = i * at.stride + (S::kPair && (i & 1) ? at.stride - 1 - at.first : at.first);
+    Tile r{};
+    r.e = -1;
+    if (t < num_tiles) {
+      if (S::kPair) t = t & 1 ? num_tiles - 1 - (t >> 1) : t >> 1;
+      r = tile_at<kMode, S>(p, C, t);
+    }
+    const bool last = i * at.stride >= num_tiles;  // no CTA has a tile in this round
+    if (r.e >= 0 || last) {
+      if (!mbar_wait(&C->taken[s], phase ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_PRODUCER, &C->abort)) return;
+      C->feed[s] = r;
+      mbar_arrive(&C->fed[s]);
+      if (++s == kFeed) s = 0, phase ^= 1;
+    }
+    if (last) return;
+  }
+}
+
+// The receiving end, for a whole warp.
+template <class S>
+struct TileFeed {
+  Control<S>* C;
+  const Params& p;
+  uint32_t s = 0, phase = 0;
+
+  __device__ __forceinline__ TileFeed(const Params& p_, Control<S>* c) : C(c), p(p_) {}
+
+  // False after a timeout, else the next tile (e < 0: none is left).
+  __device__ __forceinline__ bool next(Tile& r) {
+    const int ok = mbar_wait(&C->fed[s], phase, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    const Tile v = C->feed[s];
+    // equal in all lanes, which the compiler then knows
+    r.e = __shfl_sync(0xffffffffu, v.e, 0);
+    r.m0 = __shfl_sync(0xffffffffu, v.m0, 0);
+    r.row0 = __shfl_sync(0xffffffffu, v.row0, 0);
+    r.cols = __shfl_sync(0xffffffffu, v.cols, 0);
+    r.k_blocks = __shfl_sync(0xffffffffu, v.k_blocks, 0);
+    r.sum0 = __shfl_sync(0xffffffffu, v.sum0, 0);
+    r.sum_rows = __shfl_sync(0xffffffffu, v.sum_rows, 0);
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&C->taken[s]);
+    if (++s == kFeed) s = 0, phase ^= 1;
+    return true;
+  }
+};
+
 // Shared-memory descriptor of an operand whose 128-byte swizzled rows run along M or N:
 // 64 elements of M (N) in a row, eight rows (indices of the sum) in a group, groups 1024
 // bytes apart, the next 64 of M (N) `chunk_bytes` further on.
@@ -256,9 +377,10 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t chunk_
   return d | static_cast<uint64_t>(chunk_bytes >> 4) << 16;
 }
 
+// D = A B (first) or D += A B.
 template <bool kI8, bool kPair>
-__device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                    uint32_t accumulate) {
+__device__ __forceinline__ void mma_first(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                          uint32_t accumulate) {
 #define B2M_MMA(group, kind)                                                                      \
   asm volatile(                                                                                   \
       "{\n\t.reg .pred p;\n\t"                                                                    \
@@ -276,95 +398,116 @@ __device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t adesc, uint64_t bd
     B2M_MMA("1", "f16");
 #undef B2M_MMA
 }
+template <bool kI8, bool kPair>
+__device__ __forceinline__ void mma_more(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc) {
+#define B2M_MMA(group, kind)                                                                           \
+  asm volatile("tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, 1;" ::"r"(d_tmem),     \
+               "l"(adesc), "l"(bdesc), "r"(idesc)                                                       \
+               : "memory")
+  if (kI8 && kPair)
+    B2M_MMA("2", "i8");
+  else if (kI8)
+    B2M_MMA("1", "i8");
+  else if (kPair)
+    B2M_MMA("2", "f16");
+  else
+    B2M_MMA("1", "f16");
+#undef B2M_MMA
+}
 
 // Tiled loads whose bytes are counted on the barrier at `bar`, an address in the cluster's
 // shared memory (of a pair: the leader's barrier).  No multicast.
 template <bool kPair>
-__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
   if (kPair)
-    tma_load_2d_pair(dst, map, bar, x, y);
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
   else
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+        " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
         : "memory");
 }
 template <bool kPair>
-__device__ __forceinline__ void load_3d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
                                         int32_t z) {
   if (kPair)
     asm volatile(
         "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
   else
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 
-// Place of this CTA in its pair, and of the pair in the grid.
-struct Where {
-  uint32_t rank;
-  int first;   // first tile
-  int stride;  // tiles between two of this pair (or CTA)
-};
-
-// Warp 0, one lane: this CTA's operands of every stage.
+// Warp 0: this CTA's operands of every stage.  Like the MMA warp, all lanes run the loop and
+// one is elected for each copy: addresses and coordinates are then uniform across the warp.
 template <int kMode, bool kI8, class S>
-__device__ __forceinline__ void producer(const CUtensorMap* map_a, const CUtensorMap* map_b,
-                                         const CUtensorMap* map_b_small, const Params& p, uint8_t* smem,
-                                         Control<S>* C, int num_tiles, const Where& at) {
+__device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint8_t* smem, Control<S>* C,
+                                         const Where& at) {
   constexpr int kElems = kI8 ? 128 : 64;  // elements in a 128-byte row
-  uint32_t kg = 0;
+  const uint32_t smem0 = smem_u32(smem);
+  uint32_t kg = 0, s = 0, phase = 0;
   bool alive = true;
-  for (int t = at.first; t < num_tiles && alive; t += at.stride) {
-    const Tile r = tile_at<kMode, S>(p, C, t);
+  TileFeed<S> feed(p, C);
+  Tile r;
+  while (alive) {
+    if (!feed.next(r) || r.e < 0) break;
     const int half = mma_cols<S>(r.cols) / S::kCtas;  // rows of the row operand in this CTA
-    // One box of the row operand for each stage, of two sizes: smaller boxes in their place, as
-    // many as the tile needs, took longer to issue than the rows that they leave out (E=32,
-    // 224 rows each: 419 us in boxes of 32 rows, 385 in these).  kDw: boxes of 64 columns.
-    const bool few = kMode != kDw && half <= S::kSmallRows;
+    // One box of the row operand for each stage, of the smallest size that holds the tile's rows:
+    // as many 32-row boxes as it needs took longer to issue than the rows that they leave out
+    // (E=32, 224 rows each: 419 us, 385 with single boxes).  kDw: boxes of 64 columns.
+    const int size = half <= S::kBRows / 4 ? 0 : half <= S::kBRows / 2 ? 1 : 2;
     const int boxes = (half + 63) / 64;
-    const uint32_t bytes =
-        kABytes + (kMode == kDw ? boxes * 64 : few ? S::kSmallRows : S::kBRows) * kRowBytes;
-    const int row = static_cast<int>(r.row0) + static_cast<int>(at.rank) * half;
+    const uint32_t bytes = kABytes + (kMode == kDw ? boxes * 64 : S::kBRows >> (2 - size)) * kRowBytes;
+    const CUtensorMap* const map_cols = &maps.cols;
+    const CUtensorMap* const map_rows = &maps.rows[kMode == kDw ? 2 : size];
+    const int row = r.row0 + static_cast<int>(at.rank) * half;
     const int m0 = r.m0 + static_cast<int>(at.rank) * kM;
     for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
-      const int s = kg % S::kStages;
-      if (!mbar_wait(&C->empty[s], ((kg / S::kStages) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_PRODUCER,
-                     &C->abort)) {
+      const int ok = mbar_wait(&C->empty[s], phase ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_PRODUCER, &C->abort);
+      if (!__all_sync(0xffffffffu, ok)) {
         alive = false;
         break;
       }
-      uint8_t* a = smem + s * S::kStageBytes;
-      uint8_t* b = a + kABytes;
-      uint32_t bar = smem_u32(&C->full[s]);
-      if (S::kPair) bar = mapa_shared(bar, 0);
-      if (kMode == kDw && r.sum_rows - kb * 64 < 64) {  // warp 2 comes between the copies and the MMA
-        if (at.rank == 0) mbar_arrive(&C->full[s]);
-        mbar_arrive_expect_tx(&C->landed[s], bytes);
-        bar = smem_u32(&C->landed[s]);
-        if (S::kPair) bar = mapa_shared(bar, at.rank);
-      } else if (at.rank == 0) {
-        mbar_arrive_expect_tx(&C->full[s], S::kCtas * bytes);
+      if (elect_one()) {
+        const uint32_t a = smem0 + s * S::kStageBytes, b = a + kABytes;
+        uint32_t bar = smem_u32(&C->full[s]);
+        if (S::kPair) bar = mapa_shared(bar, 0);
+        if (kMode == kDw && r.sum_rows - kb * 64 < 64) {  // warp 2 comes between the copies and the MMA
+          if (at.rank == 0) mbar_arrive(&C->full[s]);
+          mbar_arrive_expect_tx(&C->landed[s], bytes);
+          bar = smem_u32(&C->landed[s]);
+          if (S::kPair) bar = mapa_shared(bar, at.rank);
+        } else if (at.rank == 0) {
+          mbar_arrive_expect_tx(&C->full[s], S::kCtas * bytes);
+        }
+        if (kMode == kFwd) {
+          load_3d<S::kPair>(a, map_cols, bar, kb * kElems, m0, r.e);
+          load_2d<S::kPair>(b, map_rows, bar, kb * kElems, row);
+        } else if (kMode == kDx) {
+          load_3d<S::kPair>(a, map_cols, bar, m0, kb * 64, r.e);
+          load_3d<S::kPair>(a + kABytes / 2, map_cols, bar, m0 + 64, kb * 64, r.e);
+          load_2d<S::kPair>(b, map_rows, bar, kb * kElems, row);
+        } else {
+          const int sum = r.sum0 + kb * 64;
+          load_2d<S::kPair>(a, map_cols, bar, m0, sum);
+          load_2d<S::kPair>(a + kABytes / 2, map_cols, bar, m0 + 64, sum);
+          load_2d<S::kPair>(b, map_rows, bar, row, sum);
+          if (boxes > 1) load_2d<S::kPair>(b + 64 * kRowBytes, map_rows, bar, row + 64, sum);
+        }
       }
-      if (kMode == kFwd) {
-        load_3d<S::kPair>(a, map_a, bar, kb * kElems, m0, r.e);
-      } else if (kMode == kDx) {
-        load_3d<S::kPair>(a, map_a, bar, m0, kb * 64, r.e);
-        load_3d<S::kPair>(a + kABytes / 2, map_a, bar, m0 + 64, kb * 64, r.e);
-      } else {
-        const int sum = static_cast<int>(r.sum0) + kb * 64;
-        load_2d<S::kPair>(a, map_a, bar, m0, sum);
-        load_2d<S::kPair>(a + kABytes / 2, map_a, bar, m0 + 64, sum);
-        for (int i = 0; i < boxes; ++i) load_2d<S::kPair>(b + i * 64 * kRowBytes, map_b, bar, row + i * 64, sum);
-      }
-      if (kMode != kDw) load_2d<S::kPair>(b, few ? map_b_small : map_b, bar, kb * kElems, row);
+      __syncwarp();
+      if (++s == S::kStages) s = 0, phase ^= 1;
     }
   }
   // The stages still in use are released before the CTA exits: their copies have then landed
@@ -374,17 +517,19 @@ __device__ __forceinline__ void producer(const CUtensorMap* map_a, const CUtenso
     if (!mbar_wait(&C->empty[i % S::kStages], (i / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN,
                    nullptr))
       break;
+  __syncwarp();
 }
 
 // Warp 2 of kDw: when this CTA's copies of a segment's last, partly filled stage have landed,
 // clears the rows behind the segment, up to the next step of the MMA, and tells the (leader's)
 // MMA warp.
 template <class S>
-__device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, Control<S>* C, int num_tiles,
-                                            const Where& at, int lane) {
+__device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, Control<S>* C, int lane) {
   uint32_t kg = 0, phases = 0;  // bit s: parity of the next use of landed[s]
-  for (int t = at.first; t < num_tiles; t += at.stride) {
-    const Tile r = tile_at<kDw, S>(p, C, t);
+  TileFeed<S> feed(p, C);
+  Tile r;
+  while (true) {
+    if (!feed.next(r) || r.e < 0) return;
     const int left = r.sum_rows & 63;
     kg += r.k_blocks;
     if (left == 0) continue;
@@ -406,64 +551,85 @@ __device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, Cont
   }
 }
 
-// Warp 1 (of a pair: the leader's), one lane issuing.
+// Warp 1 (of a pair: the leader's).  Short segments make this loop's own instructions count:
+// the tensor cores need 157 cycles for a block of the sum (four MMAs) with N = 32, 256 with
+// N = 128 and 512 with N = 256.  All lanes run the loop and one is elected to issue, so that
+// descriptors live in uniform registers; only the low word of a descriptor changes, and only
+// a block's first MMA carries a predicate.  Measured alone, with operands in place: 208, 256
+// and 512 cycles; with 64-bit descriptor sums and a predicate each it was 371, 371 and 512,
+// and a loop run by one lane took 510 whatever N.
 template <int kMode, bool kI8, class S>
-__device__ __forceinline__ void mma_thread(const Params& p, uint8_t* smem, Control<S>* C, int num_tiles,
-                                           uint32_t tmem_base, const Where& at) {
-  uint32_t kg = 0, used = 0, phases = 0;  // phases, bit s: parity of the next use of cleared[s]
-  bool alive = true;
-  for (int t = at.first; t < num_tiles && alive; t += at.stride) {
-    const Tile r = tile_at<kMode, S>(p, C, t);
+__device__ __forceinline__ void mma_warp(const Params& p, uint8_t* smem, Control<S>* C, uint32_t tmem_base) {
+  // 32 bytes of the sum in each step: within the row, or 16 rows further on
+  constexpr uint32_t a_step = kMode == kFwd ? 2 : 128, b_step = kMode == kDw ? 128 : 2;
+  const uint32_t as = smem_u32(smem), bs = as + kABytes;
+  const uint64_t adesc = kMode == kFwd ? smem_desc_sw128(as) : smem_desc_mn(as, kABytes / 2);
+  const uint64_t bdesc = kMode == kDw ? smem_desc_mn(bs, 64 * kRowBytes) : smem_desc_sw128(bs);
+  const uint32_t a_lo = static_cast<uint32_t>(adesc), b_lo = static_cast<uint32_t>(bdesc);
+  const uint64_t a_hi = adesc >> 32 << 32, b_hi = bdesc >> 32 << 32;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+  uint32_t s = 0, phase = 0, used = 0, tails = 0;  // tails, bit s: parity of the next use of cleared[s]
+  bool alive = true, any = false;
+  TileFeed<S> feed(p, C);
+  Tile r;
+  while (alive) {
+    if (!feed.next(r) || r.e < 0) break;
     if (r.k_blocks == 0) continue;
-    const int buf = used & 1;
-    if (!mbar_wait(&C->tempty[buf], ((used >> 1) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort))
-      break;
-    const uint32_t d = tmem_base + static_cast<uint32_t>(buf * S::NT);
+    const uint32_t buf = used & 1;
+    int ok = mbar_wait(&C->tempty[buf], ((used >> 1) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
+                       &C->abort);
+    if (!__all_sync(0xffffffffu, ok)) break;
+    const uint32_t d = tmem + buf * S::NT;
     const uint32_t idesc = p.idesc | (static_cast<uint32_t>(mma_cols<S>(r.cols)) >> 3 << 17);
-    for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
-      const int s = kg % S::kStages;
-      if (!mbar_wait(&C->full[s], (kg / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort)) {
+    for (int kb = 0; kb < r.k_blocks; ++kb) {
+      ok = mbar_wait(&C->full[s], phase, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort);
+      const int left = kMode == kDw ? r.sum_rows - kb * 64 : 64;
+      if (kMode == kDw && left < 64) {
+        ok = ok && mbar_wait_cluster(&C->cleared[s], (tails >> s) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
+                                     &C->abort);
+        tails ^= 1u << s;
+      }
+      if (!__all_sync(0xffffffffu, ok)) {
         alive = false;
         break;
       }
-      if (kMode == kDw && r.sum_rows - kb * 64 < 64) {
-        if (!mbar_wait(&C->cleared[s], (phases >> s) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort)) {
-          alive = false;
-          break;
-        }
-        phases ^= 1u << s;
-      }
       tc_fence_after();
-      const uint32_t as = smem_u32(smem + s * S::kStageBytes), bs = as + kABytes;
-      const uint64_t adesc = kMode == kFwd ? smem_desc_sw128(as) : smem_desc_mn(as, kABytes / 2);
-      const uint64_t bdesc = kMode == kDw ? smem_desc_mn(bs, 64 * kRowBytes) : smem_desc_sw128(bs);
-      // 32 bytes of the sum in each step: within the row, or 16 rows further on
-      constexpr uint64_t a_step = kMode == kFwd ? 2 : 128, b_step = kMode == kDw ? 128 : 2;
-      const int steps = kMode == kDw ? min(4, (r.sum_rows - kb * 64 + 15) >> 4) : 4;
+      const uint32_t a_s = a_lo + s * (S::kStageBytes >> 4), b_s = b_lo + s * (S::kStageBytes >> 4);
+      if (elect_one()) {
+        mma_first<kI8, S::kPair>(d, a_hi | a_s, b_hi | b_s, idesc, kb > 0);
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (kMode != kDw || k < steps)
-          mma<kI8, S::kPair>(d, adesc + a_step * k, bdesc + b_step * k, idesc, kb > 0 || k > 0 ? 1u : 0u);
-      if (S::kPair)
-        mma_commit_pair(&C->empty[s], 0x3);
-      else
-        mma_commit(&C->empty[s]);
+        for (int k = 1; k < 4; ++k)
+          if (kMode != kDw || k * 16 < left)
+            mma_more<kI8, S::kPair>(d, a_hi | (a_s + a_step * k), b_hi | (b_s + b_step * k), idesc);
+        if (S::kPair)
+          mma_commit_pair(&C->empty[s], 0x3);
+        else
+          mma_commit(&C->empty[s]);
+        if (kb == r.k_blocks - 1) {
+          if (S::kPair)
+            mma_commit_pair(&C->tfull[buf], 0x3);
+          else
+            mma_commit(&C->tfull[buf]);
+        }
+      }
+      __syncwarp();
+      any = true;
+      if (++s == S::kStages) s = 0, phase ^= 1;
     }
-    if (!alive) break;
-    if (S::kPair)
-      mma_commit_pair(&C->tfull[buf], 0x3);
-    else
-      mma_commit(&C->tfull[buf]);
     ++used;
   }
   // every MMA issued here has completed before TMEM is freed
-  if (kg > 0) {
-    if (S::kPair)
-      mma_commit_pair(&C->mma_done, 0x1);
-    else
-      mma_commit(&C->mma_done);
+  if (any) {
+    if (elect_one()) {
+      if (S::kPair)
+        mma_commit_pair(&C->mma_done, 0x1);
+      else
+        mma_commit(&C->mma_done);
+    }
+    __syncwarp();
     mbar_wait(&C->mma_done, 0, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
   }
+  __syncwarp();
 }
 
 // 16 TMEM lanes x 32 columns.  Thread l gets, for each group g of eight columns, lane l/4
@@ -596,18 +762,20 @@ __device__ __forceinline__ void emit_fp32(float* o, int64_t ldo, int n, int m, b
 }
 
 template <int kMode, bool kI8, class S>
-__device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, int num_tiles, uint32_t tmem_base,
-                                         const Where& at, int warp, int lane) {
+__device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, uint32_t tmem_base, uint32_t rank, int warp,
+                                         int lane) {
   const int q = warp & 3;  // TMEM lane quarter of this warp
   const int h = (warp - 4) >> 2;
   const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
   const Duo duo{1 + h * 2 + (q >> 1), q & 1};
   uint8_t* staging = C->staging[duo.bar - 1];
   uint32_t used = 0;
-  for (int t = at.first; t < num_tiles; t += at.stride) {
-    const Tile r = tile_at<kMode, S>(p, C, t);
+  TileFeed<S> feed(p, C);
+  Tile r;
+  while (true) {
+    if (!duo.both(feed.next(r)) || r.e < 0) return;
     const int buf = used & 1;
-    const int m0 = r.m0 + static_cast<int>(at.rank) * kM + q * 32;
+    const int m0 = r.m0 + static_cast<int>(rank) * kM + q * 32;
     const int m = min(32, p.m_dim - m0);  // columns of this warp that exist, and of both
     const int m_duo = min(64, p.m_dim - m0 + duo.half * 32);
     const bool zero = r.k_blocks == 0;
@@ -623,7 +791,7 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, int num
       if (!duo.both(ok)) return;
       tc_fence_after();
     }
-    const int64_t base = (kMode == kDw ? r.e * p.out_expert : 0) + r.row0 * p.ldo + m0;
+    const int64_t base = (kMode == kDw ? r.e * p.out_expert : 0) + static_cast<int64_t>(r.row0) * p.ldo + m0;
     for (int c = h * 32; c < r.cols && m_duo > 0; c += 64) {
       const int n = min(32, r.cols - c);
       const uint32_t taddr = tmem_base + lane_off + static_cast<uint32_t>(buf * S::NT + c);
@@ -652,12 +820,11 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, int num
 
 template <int kMode, bool kI8, class S>
 __global__ void __launch_bounds__(kThreads, 1)
-    grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ CUtensorMap map_b_small, const __grid_constant__ Params p) {
+    grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Control<S>* C = reinterpret_cast<Control<S>*>(smem + S::kStages * S::kStageBytes);
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0);
   const int lane = threadIdx.x & 31;
   const Where at{S::kPair ? cluster_ctarank() : 0u, static_cast<int>(blockIdx.x) / S::kCtas,
                  static_cast<int>(gridDim.x) / S::kCtas};
@@ -672,13 +839,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&C->tfull[b], 1);
       mbar_init(&C->tempty[b], S::kCtas * kEpiWarps);
     }
+    // readers of a tile: producer, epilogue warps, (kDw) warp 2, and the MMA warp of the leader
+    for (int s = 0; s < kFeed; ++s) {
+      mbar_init(&C->fed[s], 1);
+      mbar_init(&C->taken[s], 1 + kEpiWarps + (kMode == kDw ? 1 : 0) + (at.rank == 0 ? 1 : 0));
+    }
     mbar_init(&C->mma_done, 1);
     C->abort = 0;
     fence_mbar_init();
     if (p.rows > 0) {  // without rows nothing is loaded, and kDw has no maps
-      tma_prefetch_desc(&map_a);
-      tma_prefetch_desc(&map_b);
-      if (kMode != kDw) tma_prefetch_desc(&map_b_small);
+      tma_prefetch_desc(&maps.cols);
+      for (int i = kMode == kDw ? 2 : S::kPair ? 0 : 1; i < 3; ++i) tma_prefetch_desc(&maps.rows[i]);
     }
   }
   if (warp == 1) {
@@ -696,15 +867,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = C->tmem_base;
   if (warp == 0) {
-    if (lane == 0) producer<kMode, kI8, S>(&map_a, &map_b, &map_b_small, p, smem, C, num_tiles, at);
-    __syncwarp();
+    producer<kMode, kI8, S>(maps, p, smem, C, at);
   } else if (warp == 1) {
-    if (lane == 0 && at.rank == 0) mma_thread<kMode, kI8, S>(p, smem, C, num_tiles, tmem_base, at);
-    __syncwarp();
+    if (at.rank == 0) mma_warp<kMode, kI8, S>(p, smem, C, tmem_base);
   } else if (warp == 2) {
-    if (kMode == kDw) clear_tails<S>(p, smem, C, num_tiles, at, lane);
-  } else if (warp >= 4) {
-    epilogue<kMode, kI8, S>(p, C, num_tiles, tmem_base, at, warp, lane);
+    if (kMode == kDw) clear_tails<S>(p, smem, C, lane);
+  } else if (warp == 3) {
+    if (lane == 0) feed_tiles<kMode, S>(p, C, num_tiles, at);
+    __syncwarp();
+  } else {
+    epilogue<kMode, kI8, S>(p, C, tmem_base, at.rank, warp, lane);
   }
   tc_fence_before();
   __syncthreads();
@@ -753,8 +925,7 @@ struct Weights {  // [experts, n, k], strides in elements
 };
 
 template <int kMode, bool kI8, class S>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& bs, const Params& p, int64_t tiles_bound,
-           int num_sms, cudaStream_t s) {
+int launch(const Maps& maps, const Params& p, int64_t tiles_bound, int num_sms, cudaStream_t s) {
   static_assert(smem_bytes<S>() <= 227 * 1024, "shared memory budget");
   static std::atomic<bool> attr_done[64];
   int dev = 0;
@@ -777,7 +948,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& bs, co
   cfg.stream = s;
   cfg.attrs = cluster;
   cfg.numAttrs = S::kPair ? 1 : 0;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, a, b, bs, p), "grouped launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, maps, p), "grouped launch");
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
@@ -863,14 +1034,15 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   B2M_TRY(device_ready(&num_sms));
   if (x.rows == 0) return B2M_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  CUtensorMap ma, mb, ms;
-  B2M_TRY(encode_map(&ma, type, 3, w.ptr, w_dims, w_strides, w_box, what));
-  const cuuint32_t small[2] = {in_row, static_cast<cuuint32_t>(narrow ? Narrow::kSmallRows : Wide::kSmallRows)};
-  B2M_TRY(encode_map(&ms, type, 2, x.ptr, x_dims, x_strides, small, what));
-  const cuuint32_t big[2] = {in_row, static_cast<cuuint32_t>(narrow ? Narrow::kBRows : Wide::kBRows)};
-  B2M_TRY(encode_map(&mb, type, 2, x.ptr, x_dims, x_strides, big, what));
-  if (narrow) return launch<kMode, kI8, Narrow>(ma, mb, ms, p, row_tiles * p.m_tiles, num_sms, s);
-  return launch<kMode, kI8, Wide>(ma, mb, ms, p, row_tiles * p.m_tiles, num_sms, s);
+  Maps maps;
+  B2M_TRY(encode_map(&maps.cols, type, 3, w.ptr, w_dims, w_strides, w_box, what));
+  const cuuint32_t b_rows = narrow ? Narrow::kBRows : Wide::kBRows;
+  for (int i = narrow ? 1 : 0; i < 3; ++i) {  // a narrow tile's MMA takes half of its rows at least
+    const cuuint32_t box[2] = {in_row, b_rows >> (2 - i)};
+    B2M_TRY(encode_map(&maps.rows[i], type, 2, x.ptr, x_dims, x_strides, box, what));
+  }
+  if (narrow) return launch<kMode, kI8, Narrow>(maps, p, row_tiles * p.m_tiles, num_sms, s);
+  return launch<kMode, kI8, Wide>(maps, p, row_tiles * p.m_tiles, num_sms, s);
 }
 
 int check_16bit(const char* what, int32_t in_type) {
@@ -899,8 +1071,7 @@ extern "C" int b2m_grouped_mm(const void* x, int64_t rows, int64_t ldx, const vo
 
 extern "C" int b2m_grouped_mm_dx(const void* dy, int64_t rows, int64_t lddy, const void* w, int32_t experts, int64_t n,
                                  int64_t k, int64_t ldw, int64_t w_stride, const int32_t* ends, int32_t in_type,
-                                 void* out, int64_t ldo, int32_t out_type, int32_t clear_rest, int32_t* dev_status,
-                                 void* stream) {
+                                 void* out, int64_t ldo, int32_t out_type, int32_t clear_rest, int32_t* dev_status, void* stream) {
   using namespace b2m;
   const Matrix mdy{dy, rows, n, lddy};
   const Weights mw{w, experts, n, k, ldw, w_stride};
@@ -915,8 +1086,7 @@ extern "C" int b2m_grouped_mm_dx(const void* dy, int64_t rows, int64_t lddy, con
 
 extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows, int64_t n,
                                  int64_t k, const int32_t* ends, int32_t experts, int32_t in_type, void* out,
-                                 int64_t ldo, int64_t out_stride, int32_t out_type, int32_t* dev_status,
-                                 void* stream) {
+                                 int64_t ldo, int64_t out_stride, int32_t out_type, int32_t* dev_status, void* stream) {
   using namespace b2m;
   const char* what = "grouped_mm_dw";
   const Matrix mdy{dy, rows, n, lddy}, mx{x, rows, k, ldx};
@@ -958,12 +1128,13 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(ldx * 2)};
   const cuuint64_t dy_strides[1] = {static_cast<cuuint64_t>(lddy * 2)};
   const cuuint32_t box[2] = {64, 64};
-  CUtensorMap ma{}, mb{};
+  Maps maps{};
   if (rows > 0) {
-    B2M_TRY(encode_map(&ma, type, 2, x, x_dims, x_strides, box, what));
-    B2M_TRY(encode_map(&mb, type, 2, dy, dy_dims, dy_strides, box, what));
+    B2M_TRY(encode_map(&maps.cols, type, 2, x, x_dims, x_strides, box, what));
+    B2M_TRY(encode_map(&maps.rows[2], type, 2, dy, dy_dims, dy_strides, box, what));
   }
-  return launch<kDw, false, Wide>(ma, mb, mb, p, tiles, num_sms, static_cast<cudaStream_t>(stream));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return launch<kDw, false, Wide>(maps, p, tiles, num_sms, s);
 }
 
 extern "C" int b2m_int8_mm(const void* a, const float* a_scale, int64_t rows, int64_t lda, const void* w,
