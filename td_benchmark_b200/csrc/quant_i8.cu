@@ -3,9 +3,10 @@
 //   scale = max(amax / 127, 1e-12)      IEEE fp32 division
 //   q     = rne(x / scale) within +-127  IEEE fp32 division for each element
 //
-// A group of 32 to 1024 threads owns a row and keeps it in registers (up to four 16-byte
-// vectors in each thread) between the maximum and the codes, so x is read once; wider rows
-// are read a second time, from L2.  Bound by HBM: size + 1 bytes for each element.
+// A group of 32 to 1024 threads owns a row and keeps it in registers as loaded (up to four
+// 16-byte vectors in each thread) between the maximum and the codes, so x is read once; wider
+// rows are read a second time, from L2.  The next row's vectors are in flight while a row is
+// worked on.  Bound by HBM: size + 1 bytes for each element (8192 x 7168 bf16: see below).
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -25,36 +26,71 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+// What a 32-bit word of the row holds: two 16-bit values or one of 32 bits.
 template <typename T>
-__device__ __forceinline__ float to_f32(T v);
+struct Word;
 template <>
-__device__ __forceinline__ float to_f32<float>(float v) {
-  return v;
-}
+struct Word<float> {
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t w) {  // a >= 0, |w|
+    return __float_as_uint(max_nan(__uint_as_float(a), fabsf(__uint_as_float(w))));
+  }
+  static __device__ __forceinline__ float top(uint32_t a) { return __uint_as_float(a); }
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) { f[0] = __uint_as_float(w); }
+};
 template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) {
-  return __bfloat162float(v);
-}
+struct Word<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t w) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(w & 0x7FFF7FFFu));
+    return r;
+  }
+  static __device__ __forceinline__ float top(uint32_t a) {
+    return max_nan(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+    f[0] = __uint_as_float(w << 16);
+    f[1] = __uint_as_float(w & 0xFFFF0000u);
+  }
+};
 template <>
-__device__ __forceinline__ float to_f32<__half>(__half v) {
-  return __half2float(v);
-}
+struct Word<__half> {
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t w) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(w & 0x7FFF7FFFu));
+    return r;
+  }
+  static __device__ __forceinline__ float top(uint32_t a) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    return max_nan(v.x, v.y);
+  }
+  static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    f[0] = v.x;
+    f[1] = v.y;
+  }
+};
 
-// Vector `i` of a row (16 / sizeof(T) elements), zero beyond the row.
+// Vector `i` of a row (16 bytes), zero beyond the row.
 template <typename T, bool kAligned>
-__device__ __forceinline__ void load_vec(const T* __restrict__ row, int64_t cols, int64_t i,
-                                         float (&f)[16 / sizeof(T)]) {
+__device__ __forceinline__ uint4 load_vec(const T* __restrict__ row, int64_t cols, int64_t i) {
   constexpr int N = 16 / sizeof(T);
   const int64_t c = i * N;
-  if (kAligned && c + N <= cols) {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + c));
-    const T* t = reinterpret_cast<const T*>(&raw);
+  if (kAligned && c + N <= cols) return __ldg(reinterpret_cast<const uint4*>(row + c));
+  uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = to_f32<T>(t[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = c + j < cols ? to_f32<T>(row[c + j]) : 0.0f;
+  for (int j = 0; j < N; ++j) {
+    if (c + j >= cols) continue;
+    if (sizeof(T) == 4)
+      w[j & 3] = reinterpret_cast<const uint32_t*>(row)[c + j];
+    else
+      w[j / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[c + j]) << (16 * (j & 1));
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t larger_vec(uint32_t a, const uint4& v) {
+  return Word<T>::larger(Word<T>::larger(Word<T>::larger(Word<T>::larger(a, v.x), v.y), v.z), v.w);
 }
 
 // Codes of one vector.  x * (1 / scale) is within 1.6e-5 of x / scale (two roundings of a
@@ -88,9 +124,15 @@ __device__ __forceinline__ void codes_of(const float (&f)[N], float scale, float
 
 template <typename T, bool kAligned>
 __device__ __forceinline__ void store_codes(int8_t* __restrict__ q, int64_t cols, int64_t i, float scale, float inv,
-                                            bool divide, const float (&f)[16 / sizeof(T)]) {
+                                            bool divide, const uint4& v) {
   constexpr int N = 16 / sizeof(T);
+  constexpr int kIn = 4 / sizeof(T);  // values in a word
   const int64_t c = i * N;
+  float f[N];
+  Word<T>::unpack(v.x, f);
+  Word<T>::unpack(v.y, f + kIn);
+  Word<T>::unpack(v.z, f + 2 * kIn);
+  Word<T>::unpack(v.w, f + 3 * kIn);
   uint32_t w[N / 4];
   codes_of<N>(f, scale, inv, divide, w);
   if (kAligned && c + N <= cols) {
@@ -111,55 +153,68 @@ __global__ void __launch_bounds__(1024)
     quant_i8_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int8_t* __restrict__ q,
                     int64_t ldq, float* __restrict__ scale, int group) {
   constexpr int N = 16 / sizeof(T);
-  __shared__ float part[32];
+  __shared__ float part[2][32];
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
   const int in_row = threadIdx.x & (group - 1);
-  const int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
-  const int64_t vecs = r < rows ? (cols + N - 1) / N : 0;
-  const T* row = x + r * ldx;
-  float f[kInRegisters ? kVecs : 1][N];
-  float amax = 0.0f;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / group);
+  const int vecs = static_cast<int>((cols + N - 1) / N);
+  int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
+  uint4 v[kInRegisters ? kVecs : 1];
   if (kInRegisters) {
 #pragma unroll
     for (int u = 0; u < kVecs; ++u)
-      if (in_row + u * group < vecs) load_vec<T, kAligned>(row, cols, in_row + u * group, f[u]);
-#pragma unroll
-    for (int u = 0; u < kVecs; ++u)
-      if (in_row + u * group < vecs) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) amax = max_nan(amax, fabsf(f[u][j]));
-      }
-  } else {
-    for (int64_t i = in_row; i < vecs; i += group) {
-      load_vec<T, kAligned>(row, cols, i, f[0]);
-#pragma unroll
-      for (int j = 0; j < N; ++j) amax = max_nan(amax, fabsf(f[0][j]));
-    }
+      if (r < rows && in_row + u * group < vecs) v[u] = load_vec<T, kAligned>(x + r * ldx, cols, in_row + u * group);
   }
+  // every thread of the block makes the same number of rounds
+  for (int64_t first = r - threadIdx.x / group, round = 0; first < rows; first += step, r += step, ++round) {
+    const bool mine = r < rows;
+    const T* row = x + r * ldx;
+    uint4 next[kInRegisters ? kVecs : 1];
+    uint32_t most = 0;
+    if (kInRegisters) {
+      const int64_t rn = r + step;
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  if (group > 32) {
-    if (lane == 0) part[warp] = amax;
-    __syncthreads();
-    const int first = (threadIdx.x & ~(group - 1)) >> 5;
-    amax = part[first + (lane & (group / 32 - 1))];
+      for (int u = 0; u < kVecs; ++u)
+        if (rn < rows && in_row + u * group < vecs)
+          next[u] = load_vec<T, kAligned>(x + rn * ldx, cols, in_row + u * group);
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u)
+        if (mine && in_row + u * group < vecs) most = larger_vec<T>(most, v[u]);
+    } else if (mine) {
+      for (int i = in_row; i < vecs; i += group) most = larger_vec<T>(most, load_vec<T, kAligned>(row, cols, i));
+    }
+    float amax = Word<T>::top(most);
 #pragma unroll
     for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  }
-  const float s = max_nan(amax / 127.0f, 1e-12f);
-  if (r < rows && in_row == 0) scale[r] = s;
-  const float inv = 1.0f / s;
-  const bool divide = !(s < INFINITY);  // the row holds a NaN or an infinity
-  int8_t* qr = q + r * ldq;
-  if (kInRegisters) {
+    if (group > 32) {
+      float* p = part[round & 1];  // the other half is still read by warps of the round before
+      if (lane == 0) p[warp] = amax;
+      __syncthreads();
+      const int at = (threadIdx.x & ~(group - 1)) >> 5;
+      amax = p[at + (lane & (group / 32 - 1))];
 #pragma unroll
-    for (int u = 0; u < kVecs; ++u)
-      if (in_row + u * group < vecs) store_codes<T, kAligned>(qr, cols, in_row + u * group, s, inv, divide, f[u]);
-  } else {
-    for (int64_t i = in_row; i < vecs; i += group) {
-      load_vec<T, kAligned>(row, cols, i, f[0]);
-      store_codes<T, kAligned>(qr, cols, i, s, inv, divide, f[0]);
+      for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+    }
+    if (mine) {
+      const float s = max_nan(amax / 127.0f, 1e-12f);
+      if (in_row == 0) scale[r] = s;
+      const float inv = 1.0f / s;
+      const bool divide = !(s < INFINITY);  // the row holds a NaN or an infinity
+      int8_t* qr = q + r * ldq;
+      if (kInRegisters) {
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u)
+          if (in_row + u * group < vecs)
+            store_codes<T, kAligned>(qr, cols, in_row + u * group, s, inv, divide, v[u]);
+      } else {
+        for (int i = in_row; i < vecs; i += group)
+          store_codes<T, kAligned>(qr, cols, i, s, inv, divide, load_vec<T, kAligned>(row, cols, i));
+      }
+    }
+    if (kInRegisters) {
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u) v[u] = next[u];
     }
   }
 }
@@ -178,8 +233,10 @@ int launch_quant(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q
   const bool aligned = aligned16(x) && ldx * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % N == 0 && ldq % N == 0;
   const int block = group > kBlock ? group : kBlock;
   const int64_t per_block = block / group;
-  const int64_t grid = (rows + per_block - 1) / per_block;
-  if (grid > INT32_MAX) return fail(B2M_ERR_ARG, "quant_i8: too many rows (%lld)", (long long)rows);
+  // four resident blocks of 256 threads on each SM (64 registers a thread), each several rows
+  const int64_t resident = int64_t(num_sms) * (1024 / block);
+  const int64_t blocks = (rows + per_block - 1) / per_block;
+  const int64_t grid = blocks < resident ? blocks : resident;
   auto kernel = aligned ? (fits ? quant_i8_kernel<T, true, true> : quant_i8_kernel<T, true, false>)
                         : (fits ? quant_i8_kernel<T, false, true> : quant_i8_kernel<T, false, false>);
   kernel<<<static_cast<int>(grid), block, 0, s>>>(static_cast<const T*>(x), rows, cols, ldx, static_cast<int8_t*>(q),
