@@ -20,7 +20,7 @@
 // the last, rounded once.
 //
 // Rows that a tile loads beyond its segment are other output rows in kFwd and kDx, computed
-// and never stored.  In kDw they would enter the sum: warp 2 clears them (in both operands,
+// and never stored.  In kDw they would enter the sum: warp 12 clears them (in both operands,
 // so an infinity there cannot meet a zero) in the segment's last stage before its MMA.
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -38,7 +38,9 @@ enum Mode { kFwd = 0, kDx = 1, kDw = 2 };
 constexpr int kM = 128;            // output columns of a CTA's part of a tile (TMEM lanes)
 constexpr int kRowBytes = 128;     // one swizzled shared-memory row
 constexpr int kMaxExperts = 1024;
-constexpr int kThreads = 384;
+// Warps: 0 and 2 feed the ring, 1 issues MMAs, 3 finds tiles, 4-11 write outputs, 12 clears tails (kDw).
+constexpr int threads_of(int mode) { return mode == kDw ? 416 : 384; }
+constexpr int kMostWarps = 13;
 constexpr int kEpiWarps = 8;
 constexpr int kABytes = kM * kRowBytes;
 constexpr int kBand = 8;           // row tiles walked together, so that they share a weight tile in L2
@@ -88,8 +90,8 @@ struct Control {
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort;
-  int32_t warp_max[kThreads / 32];
-  int32_t warp_sum[kThreads / 32];
+  int32_t warp_max[kMostWarps];
+  int32_t warp_sum[kMostWarps];
   uint64_t fed[kFeed];             // a tile is there
   uint64_t taken[kFeed];           // every role has read it
   Tile feed[kFeed];
@@ -121,6 +123,9 @@ struct Params {
   int32_t c_dim;         // kDw: output rows of one expert
   int32_t c_tiles;       // kDw
   int32_t k_blocks;      // kFwd, kDx: blocks of the sum
+  uint32_t m_magic;      // for division by m_tiles, by kBand * m_tiles and (kDw) by m_tiles * c_tiles
+  uint32_t band_magic;
+  uint32_t expert_magic;
   uint32_t idesc;        // instruction descriptor without N
   void* out;
   int64_t ldo;
@@ -146,27 +151,37 @@ __device__ __forceinline__ int find_segment(const Control<S>* C, int segments, i
   return lo;
 }
 
+// a / d with magic = ceil(2^32 / d), for a < 2^31: the product is the quotient or one more.
+__device__ __forceinline__ int quotient(int a, int d, uint32_t magic) {
+  if (d == 1) return a;
+  const uint32_t q = __umulhi(static_cast<uint32_t>(a), magic);
+  return static_cast<int>(q * static_cast<uint32_t>(d) > static_cast<uint32_t>(a) ? q - 1 : q);
+}
+
 template <int kMode, class S>
 __device__ __forceinline__ Tile tile_at(const Params& p, const Control<S>* C, int t) {
   Tile r;
   int tiles, i;  // row tiles of the segment, and this tile's index among the segment's tiles
   if (kMode == kDw) {
     const int per = p.m_tiles * p.c_tiles;
-    const int place = t / per;
+    const int place = quotient(t, per, p.expert_magic);
     r.e = C->seg[place];
     i = t - place * per;
     tiles = p.c_tiles;
   } else {
-    const int place = find_segment(C, p.segments, t / p.m_tiles);
+    const int place = find_segment(C, p.segments, quotient(t, p.m_tiles, p.m_magic));
     r.e = C->seg[place];
     i = t - C->tile0[place] * p.m_tiles;
     tiles = C->tile0[place + 1] - C->tile0[place];
   }
-  const int band = i / (kBand * p.m_tiles);
-  const int in_band = i - band * kBand * p.m_tiles;
-  const int wide = min(kBand, tiles - band * kBand);
-  const int m = in_band / wide;
-  const int c0 = (band * kBand + in_band - m * wide) * S::NT;
+  int m = i, c0 = 0;
+  if (tiles > 1) {
+    const int band = tiles > kBand ? quotient(i, kBand * p.m_tiles, p.band_magic) : 0;
+    const int in_band = i - band * kBand * p.m_tiles;
+    const int wide = min(kBand, tiles - band * kBand);
+    m = in_band / wide;
+    c0 = (band * kBand + in_band - m * wide) * S::NT;
+  }
   r.m0 = m * S::kTileM;
   if (kMode == kDw) {
     r.row0 = c0;
@@ -201,12 +216,86 @@ __device__ __forceinline__ int mma_cols(int cols) {
   return (cols + S::kStep - 1) / S::kStep * S::kStep;
 }
 
-// Segment starts, their order and row-tile counts from `ends`, by all threads.  An end that is
-// below an earlier one or outside [0, rows] is taken as the nearest one that is in order, and
-// noted in the status word.  Returns the number of tiles.
+// Waits of a whole warp: true when every lane has seen the phase complete.  The slow path,
+// with its clock and its limit, stays out of line: in a call of a few microseconds each line
+// of code is fetched once, and fetching is part of its time.
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, const Params& p, int32_t code, volatile int* abort) {
+  return mbar_wait(bar, parity, p.timeout_ns, p.status, code, abort);
+}
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, const Params& p, int32_t code, int* abort) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, wait_on(bar, parity, p, code, abort));
+}
+
+// Segment starts and row-tile counts from `ends`.  An end that is below an earlier one or
+// outside [0, rows] is taken as the nearest one that is in order, and noted in the status word.
+//
+// Narrow launches: by one warp, each lane with a run of consecutive segments.  They are the
+// calls of a few tokens, and barriers between all warps would cost them more.
+template <class S>
+__device__ __forceinline__ void plan_narrow(const Params& p, Control<S>* C, int lane) {
+  constexpr int kBatch = 4;
+  const int rows = static_cast<int>(p.rows);
+  const int per = (p.experts + 31) >> 5;
+  const int e0 = lane * per, e1 = min(e0 + per, p.experts);
+  int top = 0, lowest = rows;
+  bool bad = false;
+  for (int b = e0; b < e1; b += kBatch) {
+    int v[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) v[i] = b + i < e1 ? (p.ends ? __ldg(p.ends + b + i) : rows) : rows;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (b + i < e1) {
+        lowest = min(lowest, v[i]);
+        bad |= v[i] < top || v[i] > rows;  // below 0 is below `top`
+        top = max(top, min(v[i], rows));
+        C->start[b + i + 1] = top;
+      }
+  }
+  int before = top;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before = max(before, o);
+  }
+  before = __shfl_up_sync(0xffffffffu, before, 1);
+  if (lane == 0) before = 0;
+  if ((bad || lowest < before) && blockIdx.x == 0) set_status(p.status, B2M_STATUS_BAD_ROUTING);
+  int prev = before, sum = 0;
+  for (int e = e0; e < e1; ++e) {
+    const int end = max(C->start[e + 1], before);
+    C->start[e + 1] = end;
+    C->tile0[e] = sum;
+    C->seg[e] = static_cast<uint16_t>(e);
+    sum += (end - prev + S::NT - 1) / S::NT;
+    prev = end;
+  }
+  int at = sum;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, at, off);
+    if (lane >= off) at += o;
+  }
+  const int total = __shfl_sync(0xffffffffu, at, 31);
+  at -= sum;
+  for (int e = e0; e < e1; ++e) C->tile0[e] += at;
+  const int last = __shfl_sync(0xffffffffu, max(prev, before), 31);
+  if (lane == 0) {
+    C->start[0] = 0;
+    C->start[p.experts + 1] = rows;
+    C->tile0[p.experts] = total;
+    C->seg[p.experts] = static_cast<uint16_t>(p.experts);
+    // the rows behind the last segment, as one more segment
+    C->tile0[p.experts + 1] = total + (rows - last + S::NT - 1) / S::NT;
+  }
+}
+
+// Wide launches: by all threads, longest segments first in the walk.
 template <int kMode, class S>
-__device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
+__device__ __forceinline__ void plan_wide(const Params& p, Control<S>* C) {
   constexpr int NT = S::NT;
+  constexpr int kThreads = threads_of(kMode);
   constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = static_cast<int>(p.rows);
@@ -234,7 +323,9 @@ __device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
   __syncthreads();
   int prev = __shfl_up_sync(0xffffffffu, scan, 1);
   if (lane == 0) prev = 0;
-  for (int w = 0; w < warp; ++w) prev = max(prev, C->warp_max[w]);
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w)
+    if (w < warp) prev = max(prev, C->warp_max[w]);
   if ((bad || lowest < prev) && blockIdx.x == 0) set_status(p.status, B2M_STATUS_BAD_ROUTING);
   int n[kPer];
 #pragma unroll
@@ -247,7 +338,7 @@ __device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
     prev = end;
   }
   if (tid == 0) C->start[p.experts + 1] = rows;
-  if (S::kPair && p.experts > 1 && p.experts <= kSortMost) {  // longest segments first
+  if (p.experts > 1 && p.experts <= kSortMost) {
     __syncthreads();
     if (tid < p.experts) {
       const int mine = C->start[tid + 1] - C->start[tid];
@@ -294,13 +385,11 @@ __device__ __forceinline__ int plan_segments(const Params& p, Control<S>* C) {
     if (r < p.experts) C->tile0[r] = at;
     at += n[i];
   }
-  if (tid == 0) C->tile0[p.experts] = total;
-  if (p.segments > p.experts) {  // the rows behind the last segment, as one more segment
-    total += (rows - C->start[p.experts] + NT - 1) / NT;
-    if (tid == 0) C->tile0[p.experts + 1] = total;
+  if (tid == 0) {
+    C->tile0[p.experts] = total;
+    // the rows behind the last segment, as one more segment
+    C->tile0[p.experts + 1] = total + (rows - C->start[p.experts] + NT - 1) / NT;
   }
-  __syncthreads();
-  return kMode == kDw ? p.experts * p.m_tiles * p.c_tiles : total * p.m_tiles;
 }
 
 // Place of this CTA in its pair, and of the pair in the grid.
@@ -327,12 +416,13 @@ __device__ __forceinline__ void feed_tiles(const Params& p, Control<S>* C, int n
     Tile r{};
     r.e = -1;
     if (t < num_tiles) {
-      if (S::kPair) t = t & 1 ? num_tiles - 1 - (t >> 1) : t >> 1;
       r = tile_at<kMode, S>(p, C, t);
     }
     const bool last = i * at.stride >= num_tiles;  // no CTA has a tile in this round
     if (r.e >= 0 || last) {
-      if (!mbar_wait(&C->taken[s], phase ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_PRODUCER, &C->abort)) return;
+      if (!mbar_try_wait(&C->taken[s], phase ^ 1) &&
+          !wait_on(&C->taken[s], phase ^ 1, p, B2M_STATUS_TIMEOUT_PRODUCER, &C->abort))
+        return;
       C->feed[s] = r;
       mbar_arrive(&C->fed[s]);
       if (++s == kFeed) s = 0, phase ^= 1;
@@ -352,8 +442,7 @@ struct TileFeed {
 
   // False after a timeout, else the next tile (e < 0: none is left).
   __device__ __forceinline__ bool next(Tile& r) {
-    const int ok = mbar_wait(&C->fed[s], phase, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort);
-    if (!__all_sync(0xffffffffu, ok)) return false;
+    if (!wait_warp(&C->fed[s], phase, p, B2M_STATUS_TIMEOUT_MMA, &C->abort)) return false;
     const Tile v = C->feed[s];
     // equal in all lanes, which the compiler then knows
     r.e = __shfl_sync(0xffffffffu, v.e, 0);
@@ -449,14 +538,19 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, ui
         : "memory");
 }
 
-// Warp 0: this CTA's operands of every stage.  Like the MMA warp, all lanes run the loop and
-// one is elected for each copy: addresses and coordinates are then uniform across the warp.
+// Warps 0 and 2, every second stage each: this CTA's operands.  Like the MMA warp, all lanes
+// run the loop and one is elected for the copies, so that addresses and coordinates are
+// uniform across the warp.  One such warp took 330 cycles to issue a stage (380 for kDx, which
+// has three copies in it), about what a short segment's MMAs take.
 template <int kMode, bool kI8, class S>
 __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint8_t* smem, Control<S>* C,
-                                         const Where& at) {
+                                         uint32_t rank, int which) {
   constexpr int kElems = kI8 ? 128 : 64;  // elements in a 128-byte row
   const uint32_t smem0 = smem_u32(smem);
-  uint32_t kg = 0, s = 0, phase = 0;
+  const uint32_t full0 = smem_u32(&C->full[0]), landed0 = smem_u32(&C->landed[0]);
+  const uint32_t full0_leader = S::kPair ? mapa_shared(full0, 0) : full0;
+  const uint32_t landed0_own = S::kPair ? mapa_shared(landed0, rank) : landed0;
+  uint32_t kg = 0;  // stages of the tiles before this one
   bool alive = true;
   TileFeed<S> feed(p, C);
   Tile r;
@@ -471,24 +565,23 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
     const uint32_t bytes = kABytes + (kMode == kDw ? boxes * 64 : S::kBRows >> (2 - size)) * kRowBytes;
     const CUtensorMap* const map_cols = &maps.cols;
     const CUtensorMap* const map_rows = &maps.rows[kMode == kDw ? 2 : size];
-    const int row = r.row0 + static_cast<int>(at.rank) * half;
-    const int m0 = r.m0 + static_cast<int>(at.rank) * kM;
-    for (int kb = 0; kb < r.k_blocks; ++kb, ++kg) {
-      const int ok = mbar_wait(&C->empty[s], phase ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_PRODUCER, &C->abort);
-      if (!__all_sync(0xffffffffu, ok)) {
+    const int row = r.row0 + static_cast<int>(rank) * half;
+    const int m0 = r.m0 + static_cast<int>(rank) * kM;
+    int kb = (kg + which) & 1;
+    uint32_t s = (kg + kb) % S::kStages, phase = ((kg + kb) / S::kStages) & 1;
+    for (; kb < r.k_blocks; kb += 2) {
+      if (!wait_warp(&C->empty[s], phase ^ 1, p, B2M_STATUS_TIMEOUT_PRODUCER, &C->abort)) {
         alive = false;
         break;
       }
+      const uint32_t a = smem0 + s * S::kStageBytes, b = a + kABytes;
+      const bool tail = kMode == kDw && r.sum_rows - kb * 64 < 64;  // warp 12 comes between the copies and the MMA
+      const uint32_t bar = (tail ? landed0_own : full0_leader) + s * 8;
       if (elect_one()) {
-        const uint32_t a = smem0 + s * S::kStageBytes, b = a + kABytes;
-        uint32_t bar = smem_u32(&C->full[s]);
-        if (S::kPair) bar = mapa_shared(bar, 0);
-        if (kMode == kDw && r.sum_rows - kb * 64 < 64) {  // warp 2 comes between the copies and the MMA
-          if (at.rank == 0) mbar_arrive(&C->full[s]);
+        if (tail) {
+          if (rank == 0) mbar_arrive(&C->full[s]);
           mbar_arrive_expect_tx(&C->landed[s], bytes);
-          bar = smem_u32(&C->landed[s]);
-          if (S::kPair) bar = mapa_shared(bar, at.rank);
-        } else if (at.rank == 0) {
+        } else if (rank == 0) {
           mbar_arrive_expect_tx(&C->full[s], S::kCtas * bytes);
         }
         if (kMode == kFwd) {
@@ -507,20 +600,18 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
         }
       }
       __syncwarp();
-      if (++s == S::kStages) s = 0, phase ^= 1;
+      if ((s += 2) >= S::kStages) s -= S::kStages, phase ^= 1;
     }
+    kg += r.k_blocks;
   }
   // The stages still in use are released before the CTA exits: their copies have then landed
   // (after a timeout elsewhere, when nothing releases them, the wait ends by its limit).
   const uint32_t first = kg > S::kStages ? kg - S::kStages : 0;
-  for (uint32_t i = first; i < kg; ++i)
-    if (!mbar_wait(&C->empty[i % S::kStages], (i / S::kStages) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN,
-                   nullptr))
-      break;
-  __syncwarp();
+  for (uint32_t i = first; i < kg && alive; ++i)
+    alive = wait_warp(&C->empty[i % S::kStages], (i / S::kStages) & 1, p, B2M_STATUS_TIMEOUT_DRAIN, &C->abort);
 }
 
-// Warp 2 of kDw: when this CTA's copies of a segment's last, partly filled stage have landed,
+// Warp 12 of kDw: when this CTA's copies of a segment's last, partly filled stage have landed,
 // clears the rows behind the segment, up to the next step of the MMA, and tells the (leader's)
 // MMA warp.
 template <class S>
@@ -535,9 +626,7 @@ __device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, Cont
     if (left == 0) continue;
     const int chunks = 2 + (mma_cols<S>(r.cols) / S::kCtas + 63) / 64;  // 64 columns each, of both operands
     const int s = (kg - 1) % S::kStages;
-    const int ok = mbar_wait(&C->landed[s], (phases >> s) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
-                             &C->abort);
-    if (!__all_sync(0xffffffffu, ok)) return;
+    if (!wait_warp(&C->landed[s], (phases >> s) & 1, p, B2M_STATUS_TIMEOUT_MMA, &C->abort)) return;
     phases ^= 1u << s;
     const int vecs = ((left + 15) / 16 * 16 - left) * (kRowBytes / 16);  // 16-byte pieces of a chunk
     uint8_t* rows = smem + s * S::kStageBytes + left * kRowBytes;
@@ -576,20 +665,18 @@ __device__ __forceinline__ void mma_warp(const Params& p, uint8_t* smem, Control
     if (!feed.next(r) || r.e < 0) break;
     if (r.k_blocks == 0) continue;
     const uint32_t buf = used & 1;
-    int ok = mbar_wait(&C->tempty[buf], ((used >> 1) & 1) ^ 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
-                       &C->abort);
-    if (!__all_sync(0xffffffffu, ok)) break;
+    if (!wait_warp(&C->tempty[buf], ((used >> 1) & 1) ^ 1, p, B2M_STATUS_TIMEOUT_MMA, &C->abort)) break;
     const uint32_t d = tmem + buf * S::NT;
     const uint32_t idesc = p.idesc | (static_cast<uint32_t>(mma_cols<S>(r.cols)) >> 3 << 17);
     for (int kb = 0; kb < r.k_blocks; ++kb) {
-      ok = mbar_wait(&C->full[s], phase, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA, &C->abort);
+      bool ok = wait_warp(&C->full[s], phase, p, B2M_STATUS_TIMEOUT_MMA, &C->abort);
       const int left = kMode == kDw ? r.sum_rows - kb * 64 : 64;
       if (kMode == kDw && left < 64) {
-        ok = ok && mbar_wait_cluster(&C->cleared[s], (tails >> s) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_MMA,
-                                     &C->abort);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_cluster(&C->cleared[s], (tails >> s) & 1, p.timeout_ns, p.status,
+                                                             B2M_STATUS_TIMEOUT_MMA, &C->abort));
         tails ^= 1u << s;
       }
-      if (!__all_sync(0xffffffffu, ok)) {
+      if (!ok) {
         alive = false;
         break;
       }
@@ -627,7 +714,7 @@ __device__ __forceinline__ void mma_warp(const Params& p, uint8_t* smem, Control
         mma_commit(&C->mma_done);
     }
     __syncwarp();
-    mbar_wait(&C->mma_done, 0, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
+    wait_on(&C->mma_done, 0, p, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
   }
   __syncwarp();
 }
@@ -680,6 +767,14 @@ struct Duo {
   }
 };
 
+// The first n of eight 16-bit values, one by one.
+__device__ __noinline__ void store_edge(uint16_t* d, uint4 u, int n) {
+  const uint32_t h[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k < n) d[k] = static_cast<uint16_t>(h[k / 2] >> (16 * (k & 1)));
+}
+
 // 64 output columns (TMEM lanes of two warps) of 32 output rows (TMEM columns), rounded to 16
 // bits.  An output row is contiguous along the lanes, so the block is transposed on its way
 // out: pairs of rows in a register, 8x8 matrices through stmatrix into the staging block, and
@@ -727,14 +822,10 @@ __device__ __forceinline__ void emit_16bit(uint16_t* o, int64_t ldo, int n, int 
     if (j < n && at < m) {
       const uint4 u = *reinterpret_cast<const uint4*>(staging + j * kStagePitch + at * 2);
       uint16_t* d = o + j * ldo + at;
-      if (wide && at + 8 <= m) {
+      if (wide && at + 8 <= m)
         *reinterpret_cast<uint4*>(d) = u;
-      } else {
-        const uint32_t h[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (at + k < m) d[k] = static_cast<uint16_t>(h[k / 2] >> (16 * (k & 1)));
-      }
+      else
+        store_edge(d, u, m - at);
     }
   }
   duo.sync();
@@ -786,8 +877,7 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, uint32_
       for (int i = 0; i < 4; ++i) w_scale[i] = __shfl_sync(0xffffffffu, w_lane, 8 * i + (lane >> 2));
     }
     if (!zero) {
-      const int ok = mbar_wait(&C->tfull[buf], (used >> 1) & 1, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_EPILOGUE,
-                               &C->abort);
+      const bool ok = wait_warp(&C->tfull[buf], (used >> 1) & 1, p, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort);
       if (!duo.both(ok)) return;
       tc_fence_after();
     }
@@ -819,7 +909,7 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, uint32_
 }
 
 template <int kMode, bool kI8, class S>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(threads_of(kMode), 1)
     grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -839,10 +929,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&C->tfull[b], 1);
       mbar_init(&C->tempty[b], S::kCtas * kEpiWarps);
     }
-    // readers of a tile: producer, epilogue warps, (kDw) warp 2, and the MMA warp of the leader
+    // readers of a tile: producers, epilogue warps, (kDw) warp 12, and the MMA warp of the leader
     for (int s = 0; s < kFeed; ++s) {
       mbar_init(&C->fed[s], 1);
-      mbar_init(&C->taken[s], 1 + kEpiWarps + (kMode == kDw ? 1 : 0) + (at.rank == 0 ? 1 : 0));
+      mbar_init(&C->taken[s], 2 + kEpiWarps + (kMode == kDw ? 1 : 0) + (at.rank == 0 ? 1 : 0));
     }
     mbar_init(&C->mma_done, 1);
     C->abort = 0;
@@ -858,7 +948,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     else
       tmem_alloc(&C->tmem_base, S::kTmemCols);
   }
-  const int num_tiles = plan_segments<kMode, S>(p, C);
+  if (S::kPair)
+    plan_wide<kMode, S>(p, C);
+  else if (warp == 2)
+    plan_narrow<S>(p, C, lane);
   tc_fence_before();
   if (S::kPair)
     cluster_sync();  // both CTAs' barriers exist before one CTA signals the other's
@@ -866,15 +959,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = C->tmem_base;
-  if (warp == 0) {
-    producer<kMode, kI8, S>(maps, p, smem, C, at);
+  if (warp == 0 || warp == 2) {
+    producer<kMode, kI8, S>(maps, p, smem, C, at.rank, warp >> 1);
   } else if (warp == 1) {
     if (at.rank == 0) mma_warp<kMode, kI8, S>(p, smem, C, tmem_base);
-  } else if (warp == 2) {
-    if (kMode == kDw) clear_tails<S>(p, smem, C, lane);
   } else if (warp == 3) {
+    const int num_tiles = kMode == kDw ? p.experts * p.m_tiles * p.c_tiles : C->tile0[p.segments] * p.m_tiles;
     if (lane == 0) feed_tiles<kMode, S>(p, C, num_tiles, at);
     __syncwarp();
+  } else if (warp == 12) {
+    clear_tails<S>(p, smem, C, lane);
   } else {
     epilogue<kMode, kI8, S>(p, C, tmem_base, at.rank, warp, lane);
   }
@@ -943,7 +1037,7 @@ int launch(const Maps& maps, const Params& p, int64_t tiles_bound, int num_sms, 
   cluster[0].val.clusterDim = {static_cast<unsigned>(S::kCtas), 1, 1};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(S::kCtas * (tiles_bound < most ? tiles_bound : most)));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads_of(kMode));
   cfg.dynamicSmemBytes = smem_bytes<S>();
   cfg.stream = s;
   cfg.attrs = cluster;
@@ -952,6 +1046,8 @@ int launch(const Maps& maps, const Params& p, int64_t tiles_bound, int num_sms, 
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
+
+uint32_t magic(int64_t d) { return static_cast<uint32_t>(((uint64_t(1) << 32) + d - 1) / d); }
 
 int check_matrix(const char* what, const char* name, const Matrix& m, int elem) {
   if (m.rows < 0 || m.rows > kMaxDim || m.cols < 1 || m.cols > kMaxDim)
@@ -1010,6 +1106,8 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   const int64_t nt = narrow ? Narrow::NT : Wide::NT, tile_m = narrow ? Narrow::kTileM : Wide::kTileM;
   p.m_tiles = static_cast<int32_t>((m_dim + tile_m - 1) / tile_m);
   p.k_blocks = static_cast<int32_t>((sum + in_row - 1) / in_row);
+  p.m_magic = magic(p.m_tiles);
+  p.band_magic = magic(int64_t(kBand) * p.m_tiles);
   p.out = out;
   p.ldo = ldo;
   p.out_type = out_type;
@@ -1107,6 +1205,8 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   p.m_tiles = static_cast<int32_t>((k + Wide::kTileM - 1) / Wide::kTileM);
   p.c_dim = static_cast<int32_t>(n);
   p.c_tiles = static_cast<int32_t>((n + Wide::NT - 1) / Wide::NT);
+  p.band_magic = magic(int64_t(kBand) * p.m_tiles);
+  p.expert_magic = magic(int64_t(p.m_tiles) * p.c_tiles);
   p.out = out;
   p.ldo = ldo;
   p.out_expert = out_stride;
