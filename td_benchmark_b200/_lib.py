@@ -95,8 +95,13 @@ def load(path: Path | None = None) -> ctypes.CDLL:
         return lib
 
 
+_bound: dict[str, object] = {}   # entry points of the loaded library, by name
+
+
 def call(name: str, *args) -> None:
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    fn = _bound.get(name)
+    if fn is None:
+        fn = _bound.setdefault(name, getattr(load(), name))
+    rc = fn(*args)
     if rc != 0:
-        raise B2MError(name, rc, lib.b2m_last_error().decode(errors="replace"))
+        raise B2MError(name, rc, load().b2m_last_error().decode(errors="replace"))

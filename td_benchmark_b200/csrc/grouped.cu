@@ -404,20 +404,21 @@ struct Where {
 // find the same tiles each for itself: handing them over needs releases at cluster scope, which
 // wait for the epilogue's output stores, 3000 cycles a tile.)
 //
-// The pairs of a wide launch walk the tiles from both ends in turn: long segments first from
-// the front, where the tensor cores are the limit, short and empty ones from the back, where
-// memory is, so that both are busy at any time.  Every second round of tiles is dealt out
-// backwards, so that each pair gets its share of either end.
+// A wide launch walks its segments from the longest to the shortest, all pairs side by side on
+// the same one, and deals every second round of tiles out backwards, which evens the shares
+// out.  Long segments are limited by the tensor cores and short ones by memory, but doing both
+// at once lost more than it gave: pairs that share weights or rows drift apart and read them
+// again (16384 rows over 32 experts of 4096 x 7168, lengths by Zipf 1.2: 3.6 GB instead of
+// 2.1 GB, 862 us instead of 800), and stores wait behind the others' loads (weight gradient:
+// 1305 us instead of 935 with pairs of their own for the short segments).
 template <int kMode, class S>
 __device__ __forceinline__ void feed_tiles(const Params& p, Control<S>* C, int num_tiles, const Where& at) {
   uint32_t s = 0, phase = 0;
   for (int i = 0;; ++i) {
-    int t = i * at.stride + (S::kPair && (i & 1) ? at.stride - 1 - at.first : at.first);
+    const int t = i * at.stride + (S::kPair && (i & 1) ? at.stride - 1 - at.first : at.first);
     Tile r{};
     r.e = -1;
-    if (t < num_tiles) {
-      r = tile_at<kMode, S>(p, C, t);
-    }
+    if (t < num_tiles) r = tile_at<kMode, S>(p, C, t);
     const bool last = i * at.stride >= num_tiles;  // no CTA has a tile in this round
     if (r.e >= 0 || last) {
       if (!mbar_try_wait(&C->taken[s], phase ^ 1) &&

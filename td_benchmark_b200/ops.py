@@ -263,19 +263,17 @@ FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 def _launch(device: torch.device, name: str, *args) -> None:
     """The C call on the tensors' device and its current stream."""
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
         return
     with torch.cuda.device(index):
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _ld(t: torch.Tensor, dim: int, least: int) -> int:
-    """Stride of ``dim``; for an axis of one entry (whose stride says nothing) the smallest that the kernels take."""
-    if t.shape[dim] > 1:
-        return t.stride(dim)
-    per = 16 // t.element_size()
-    return (least + per - 1) // per * per
+def _row_stride(stride: int, rows: int, cols: int, size: int) -> int:
+    """Stride of an axis with ``rows`` entries; of one entry (whose stride says nothing) the smallest that the kernels
+    take for rows of ``cols`` elements of ``size`` bytes."""
+    return stride if rows > 1 else (cols * size + 15) // 16 * 16 // size
 
 
 def _ldo(out: torch.Tensor) -> int:
@@ -283,19 +281,20 @@ def _ldo(out: torch.Tensor) -> int:
     return out.stride(-2) if out.shape[-2] > 1 else out.shape[-1]
 
 
-def _operand(t: torch.Tensor, name: str, dim: int, dtype: torch.dtype, device: torch.device) -> None:
-    if t.dim() != dim or t.dtype != dtype or t.device != device or (t.stride(-1) != 1 and t.shape[-1] > 1):
+def _operand(t: torch.Tensor, name: str, dim: int, dtype: torch.dtype, device: torch.device) -> tuple:
+    """Strides of a checked operand."""
+    strides = t.stride()
+    if len(strides) != dim or t.dtype is not dtype or t.device != device or (strides[-1] != 1 and t.shape[-1] > 1):
         raise ValueError(f"{name} must be {dim}-D {dtype} on {device} with unit stride along its last axis")
+    return strides
 
 
 def _vector(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype, device: torch.device) -> None:
-    if t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not dtype or t.device != device or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {dtype} {list(shape)} on {device}")
 
 
-def _status_word(status: torch.Tensor | None, device: torch.device) -> int | None:
-    if status is None:
-        return None
+def _status_word(status: torch.Tensor, device: torch.device) -> int:
     _need(status.dtype == torch.int32 and status.device == device and status.numel() >= 1,
           f"status must be int32 [1] on {device}")
     return status.data_ptr()
@@ -311,11 +310,12 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
 
 def _output(out: torch.Tensor | None, shape: tuple, dtypes: tuple, out_dtype: torch.dtype | None,
             device: torch.device, inputs: tuple) -> torch.Tensor:
+    """``out`` checked, or a new tensor.  inputs: the tensors that it must not overlap, the first one on its device."""
     if out is None:
         dtype = dtypes[0] if out_dtype is None else out_dtype
         if dtype not in dtypes:
             raise ValueError(f"out_dtype must be one of {list(dtypes)}")
-        return torch.empty(shape, dtype=dtype, device=device)
+        return inputs[0].new_empty(shape, dtype=dtype)
     _need(out_dtype is None or out_dtype == out.dtype, "out_dtype differs from out's")
     _need(tuple(out.shape) == shape and out.dtype in dtypes and out.device == device and
           (shape[-1] <= 1 or out.stride(-1) == 1),
@@ -332,23 +332,26 @@ def _rows_times_weights(entry: str, name: str, x: torch.Tensor, w: torch.Tensor,
                         ) -> torch.Tensor:
     """x [T, .] times w [E, N, K] of its segment, summed over axis ``summed`` of w."""
     dtype, device = x.dtype, x.device
-    _cuda(x, name)
-    if dtype is not torch.bfloat16 and dtype is not torch.float16:
-        raise ValueError(f"{name} must be bf16 or fp16")
-    _operand(x, name, 2, dtype, device)
-    _operand(w, "w", 3, dtype, device)
+    if not x.is_cuda or (dtype is not torch.bfloat16 and dtype is not torch.float16):
+        raise ValueError(f"{name} must be a CUDA tensor, bf16 or fp16")
+    ldx, _ = _operand(x, name, 2, dtype, device)
+    w_stride, ldw, _ = _operand(w, "w", 3, dtype, device)
     experts, n, k = w.shape
     rows, width = x.shape
     if width != (k if summed == 2 else n):
         raise ValueError(f"{name} is {list(x.shape)} and w {list(w.shape)}: the summed axes differ")
     _vector(ends, "ends", (experts,), torch.int32, device)
-    clear = out is None
-    out = _output(out, (rows, n if summed == 2 else k), (dtype, torch.float32), out_dtype, device, (x, w, ends))
-    ldw = _ld(w, 1, k)
-    _launch(device, entry, x.data_ptr(), rows, _ld(x, 0, width), w.data_ptr(), experts, n, k, ldw,
-            w.stride(0) if experts > 1 else n * ldw, ends.data_ptr(), TYPE_CODES[dtype], out.data_ptr(), _ldo(out),
-            TYPE_CODES[out.dtype], clear, _status_word(status, device))
-    return out
+    cols = n if summed == 2 else k
+    if out is None and (out_dtype is None or out_dtype is dtype):
+        y, ldo, code = x.new_empty((rows, cols)), cols, TYPE_CODES[dtype]
+    else:
+        y = _output(out, (rows, cols), (dtype, torch.float32), out_dtype, device, (x, w, ends))
+        ldo, code = _ldo(y), TYPE_CODES[y.dtype]
+    ldw = _row_stride(ldw, n, k, 2)
+    _launch(device, entry, x.data_ptr(), rows, _row_stride(ldx, rows, width, 2), w.data_ptr(), experts, n, k, ldw,
+            w_stride if experts > 1 else n * ldw, ends.data_ptr(), TYPE_CODES[dtype], y.data_ptr(), ldo, code,
+            out is None, None if status is None else _status_word(status, device))
+    return y
 
 
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.Tensor | None = None,
@@ -384,11 +387,10 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: to
     dy [T, N], x [T, K] -> [E, N, K] of the input type or fp32; types, strides, ends and status as there.  Rows behind
     ``ends[-1]`` enter no sum, whatever they hold."""
     dtype, device = dy.dtype, dy.device
-    _cuda(dy, "dy")
-    if dtype is not torch.bfloat16 and dtype is not torch.float16:
-        raise ValueError("dy must be bf16 or fp16")
-    _operand(dy, "dy", 2, dtype, device)
-    _operand(x, "x", 2, dtype, device)
+    if not dy.is_cuda or (dtype is not torch.bfloat16 and dtype is not torch.float16):
+        raise ValueError("dy must be a CUDA tensor, bf16 or fp16")
+    lddy, _ = _operand(dy, "dy", 2, dtype, device)
+    ldx, _ = _operand(x, "x", 2, dtype, device)
     rows, n = dy.shape
     k = x.shape[1]
     if x.shape[0] != rows:
@@ -398,9 +400,10 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: to
     _vector(ends, "ends", (experts,), torch.int32, device)
     out = _output(out, (experts, n, k), (dtype, torch.float32), out_dtype, device, (dy, x, ends))
     ldo = _ldo(out)
-    _launch(device, "b2m_grouped_mm_dw", dy.data_ptr(), _ld(dy, 0, n), x.data_ptr(), _ld(x, 0, k), rows, n, k,
-            ends.data_ptr(), experts, TYPE_CODES[dtype], out.data_ptr(), ldo,
-            out.stride(0) if experts > 1 else n * ldo, TYPE_CODES[out.dtype], _status_word(status, device))
+    _launch(device, "b2m_grouped_mm_dw", dy.data_ptr(), _row_stride(lddy, rows, n, 2), x.data_ptr(),
+            _row_stride(ldx, rows, k, 2), rows, n, k, ends.data_ptr(), experts, TYPE_CODES[dtype], out.data_ptr(), ldo,
+            out.stride(0) if experts > 1 else n * ldo, TYPE_CODES[out.dtype],
+            None if status is None else _status_word(status, device))
     return out
 
 
@@ -438,44 +441,44 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
 
     Token codes of activations, or channel codes of weights (one row for each output channel).  A row that holds a
     NaN (an infinity) gets a NaN (infinite) scale, and a product with it becomes NaN."""
-    _cuda(x, "x")
     code, device = TYPE_CODES.get(x.dtype), x.device
-    if code is None or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
-        raise ValueError("x must be 2D bf16, fp16 or fp32 with unit column stride")
+    strides = x.stride()
+    if not x.is_cuda or code is None or len(strides) != 2 or (strides[1] != 1 and x.shape[1] > 1):
+        raise ValueError("x must be a CUDA tensor, 2D bf16, fp16 or fp32 with unit column stride")
     rows, cols = x.shape
     if q is None:
-        q = torch.empty((rows, cols), dtype=torch.int8, device=device)
+        q = x.new_empty((rows, cols), dtype=torch.int8)
         ldq = cols
     else:
-        _operand(q, "q", 2, torch.int8, device)
-        ldq = q.stride(0) if rows > 1 else cols
+        ldq, _ = _operand(q, "q", 2, torch.int8, device)
+        ldq = ldq if rows > 1 else cols
         _need(tuple(q.shape) == (rows, cols) and ldq >= cols, "bad q buffer")
         (lo, hi), (a, b) = _extent(q), _extent(x)
         _need(hi <= a or b <= lo, "q overlaps x")
     if scale is None:
-        scale = torch.empty(rows, dtype=torch.float32, device=device)
+        scale = x.new_empty(rows, dtype=torch.float32)
     else:
         _vector(scale, "scale", (rows,), torch.float32, device)
-    _launch(device, "b2m_quant_i8", x.data_ptr(), code, rows, cols, x.stride(0) if rows > 1 else cols, q.data_ptr(),
-            ldq, scale.data_ptr())
+    _launch(device, "b2m_quant_i8", x.data_ptr(), code, rows, cols, strides[0] if rows > 1 else cols, q.data_ptr(), ldq,
+            scale.data_ptr())
     return q, scale
 
 
-def _int8(a, a_scale, w, w_scale, experts, n, k, w_stride, ends, out, out_dtype, status):
+def _int8(a, a_scale, w, w_scale, experts, n, k, w_stride, ldw, ends, out, out_dtype, status):
     device = a.device
-    _operand(a, "a", 2, torch.int8, device)
-    rows = a.shape[0]
-    if a.shape[1] != k:
+    lda, _ = _operand(a, "a", 2, torch.int8, device)
+    rows, width = a.shape
+    if width != k:
         raise ValueError(f"a is {list(a.shape)} and w {list(w.shape)}: the summed axes differ")
     _vector(a_scale, "a_scale", (rows,), torch.float32, device)
-    clear = out is None
-    out = _output(out, (rows, n), FLOATS, out_dtype, device,
-                  (a, w, a_scale, w_scale) if ends is None else (a, w, a_scale, w_scale, ends))
-    ldw = _ld(w, -2, k)
-    _launch(device, "b2m_int8_mm", a.data_ptr(), a_scale.data_ptr(), rows, _ld(a, 0, k), w.data_ptr(),
-            w_scale.data_ptr(), experts, n, k, ldw, n * ldw if experts == 1 else w_stride, _ptr(ends), out.data_ptr(),
-            _ldo(out), TYPE_CODES[out.dtype], clear, _status_word(status, device))
-    return out
+    y = _output(out, (rows, n), FLOATS, out_dtype, device,
+                (a, w, a_scale, w_scale) if ends is None else (a, w, a_scale, w_scale, ends))
+    ldw = _row_stride(ldw, n, k, 1)
+    _launch(device, "b2m_int8_mm", a.data_ptr(), a_scale.data_ptr(), rows, _row_stride(lda, rows, k, 1), w.data_ptr(),
+            w_scale.data_ptr(), experts, n, k, ldw, w_stride if experts > 1 else n * ldw,
+            None if ends is None else ends.data_ptr(), y.data_ptr(), _ldo(y), TYPE_CODES[y.dtype], out is None,
+            None if status is None else _status_word(status, device))
+    return y
 
 
 def int8_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -486,10 +489,10 @@ def int8_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     fp32 [N] -> [M, N] in bf16 (default), fp16 or fp32.  The integer sums are exact (K <= 131071); rows of a and w
     are a multiple of 16 bytes apart and 16-byte aligned."""
     _cuda(a, "a")
-    _operand(w, "w", 2, torch.int8, a.device)
+    ldw, _ = _operand(w, "w", 2, torch.int8, a.device)
     n, k = w.shape
     _vector(w_scale, "w_scale", (n,), torch.float32, a.device)
-    return _int8(a, a_scale, w, w_scale, 1, n, k, 0, None, out, out_dtype, None)
+    return _int8(a, a_scale, w, w_scale, 1, n, k, 0, ldw, None, out, out_dtype, None)
 
 
 def int8_grouped_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -498,8 +501,8 @@ def int8_grouped_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_s
     """``int8_mm`` over expert segments: a int8 [T, K], w int8 [E, N, K], a_scale fp32 [T], w_scale fp32 [E, N], ends
     int32 [E] -> [T, N]; ends, status and the rows behind ``ends[-1]`` as in ``grouped_mm``."""
     _cuda(a, "a")
-    _operand(w, "w", 3, torch.int8, a.device)
+    w_stride, ldw, _ = _operand(w, "w", 3, torch.int8, a.device)
     experts, n, k = w.shape
     _vector(ends, "ends", (experts,), torch.int32, a.device)
     _vector(w_scale, "w_scale", (experts, n), torch.float32, a.device)
-    return _int8(a, a_scale, w, w_scale, experts, n, k, w.stride(0), ends, out, out_dtype, status)
+    return _int8(a, a_scale, w, w_scale, experts, n, k, w_stride, ldw, ends, out, out_dtype, status)
