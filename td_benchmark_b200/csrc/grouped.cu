@@ -107,11 +107,17 @@ constexpr size_t smem_bytes() {
 }
 
 // Tensor maps: the operand whose rows or columns are the output's columns, and the row operand
-// with boxes of a quarter, half and all of the rows that a CTA can hold (kDw: rows[2] alone).
+// with boxes of one to four quarters of the rows that a CTA can hold (kDw: rows[3] alone).
 struct Maps {
   CUtensorMap cols;
-  CUtensorMap rows[3];
+  CUtensorMap rows[4];
 };
+
+// Whether tiles take boxes of i + 1 quarters: an MMA takes half of a narrow tile's rows at least.
+template <class S>
+__host__ __device__ constexpr bool used_map(int i) {
+  return (i + 1) * (S::kBRows / 4) % (S::kStep / S::kCtas) == 0;
+}
 
 struct Params {
   const int32_t* ends;   // nullptr: one segment of all rows
@@ -151,6 +157,12 @@ __device__ __forceinline__ int find_segment(const Control<S>* C, int segments, i
   return lo;
 }
 
+// Columns of a tile as an MMA takes them: N is a multiple of 16 (of 32 for a pair).
+template <class S>
+__device__ __forceinline__ int mma_cols(int cols) {
+  return (cols + S::kStep - 1) / S::kStep * S::kStep;
+}
+
 // a / d with magic = ceil(2^32 / d), for a < 2^31: the product is the quotient or one more.
 __device__ __forceinline__ int quotient(int a, int d, uint32_t magic) {
   if (d == 1) return a;
@@ -174,24 +186,30 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Control<S>* C, in
     i = t - C->tile0[place] * p.m_tiles;
     tiles = C->tile0[place + 1] - C->tile0[place];
   }
-  int m = i, c0 = 0;
+  int m = i, c = 0;
   if (tiles > 1) {
     const int band = tiles > kBand ? quotient(i, kBand * p.m_tiles, p.band_magic) : 0;
     const int in_band = i - band * kBand * p.m_tiles;
     const int wide = min(kBand, tiles - band * kBand);
     m = in_band / wide;
-    c0 = (band * kBand + in_band - m * wide) * S::NT;
+    c = band * kBand + in_band - m * wide;
   }
   r.m0 = m * S::kTileM;
   if (kMode == kDw) {
-    r.row0 = c0;
-    r.cols = min(S::NT, p.c_dim - c0);
+    r.row0 = c * S::NT;
+    r.cols = min(S::NT, p.c_dim - c * S::NT);
     r.sum0 = C->start[r.e];
     r.sum_rows = C->start[r.e + 1] - C->start[r.e];
     r.k_blocks = (r.sum_rows + 63) >> 6;
   } else {
-    r.row0 = C->start[r.e] + c0;
-    r.cols = min(S::NT, C->start[r.e + 1] - C->start[r.e] - c0);
+    // A segment's tiles have about the same rows: one of few rows costs four fifths of a full
+    // one (258 rows: 256 and 2 take 912 cycles a block of the sum, twice 129 take 800).  Sizes
+    // are whole steps of an MMA; with eight tiles and more they come to NT, and the last of
+    // fewer tiles keeps a row (more than 256 (n - 1) rows in n < 8 tiles of at most rows / n + 31).
+    const int rows = C->start[r.e + 1] - C->start[r.e];
+    const int each = S::kPair && tiles > 1 ? mma_cols<S>((rows + tiles - 1) / tiles) : S::NT;
+    r.row0 = C->start[r.e] + c * each;
+    r.cols = min(each, rows - c * each);
     r.k_blocks = r.e < p.experts ? p.k_blocks : 0;
     r.sum0 = 0;
     r.sum_rows = 0;
@@ -208,12 +226,6 @@ __device__ __forceinline__ bool elect_one() {
       "selp.b32 %0, 1, 0, p;\n\t}"
       : "=r"(r));
   return r != 0;
-}
-
-// Columns of a tile as an MMA takes them: N is a multiple of 16 (of 32 for a pair).
-template <class S>
-__device__ __forceinline__ int mma_cols(int cols) {
-  return (cols + S::kStep - 1) / S::kStep * S::kStep;
 }
 
 // Waits of a whole warp: true when every lane has seen the phase complete.  The slow path,
@@ -561,11 +573,12 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
     // One box of the row operand for each stage, of the smallest size that holds the tile's rows:
     // as many 32-row boxes as it needs took longer to issue than the rows that they leave out
     // (E=32, 224 rows each: 419 us, 385 with single boxes).  kDw: boxes of 64 columns.
-    const int size = half <= S::kBRows / 4 ? 0 : half <= S::kBRows / 2 ? 1 : 2;
+    constexpr int kQuarter = S::kBRows / 4;
+    const int size = (half + kQuarter - 1) / kQuarter;
     const int boxes = (half + 63) / 64;
-    const uint32_t bytes = kABytes + (kMode == kDw ? boxes * 64 : S::kBRows >> (2 - size)) * kRowBytes;
+    const uint32_t bytes = kABytes + (kMode == kDw ? boxes * 64 : size * kQuarter) * kRowBytes;
     const CUtensorMap* const map_cols = &maps.cols;
-    const CUtensorMap* const map_rows = &maps.rows[kMode == kDw ? 2 : size];
+    const CUtensorMap* const map_rows = &maps.rows[kMode == kDw ? 3 : size - 1];
     const int row = r.row0 + static_cast<int>(rank) * half;
     const int m0 = r.m0 + static_cast<int>(rank) * kM;
     int kb = (kg + which) & 1;
@@ -940,7 +953,8 @@ __global__ void __launch_bounds__(threads_of(kMode), 1)
     fence_mbar_init();
     if (p.rows > 0) {  // without rows nothing is loaded, and kDw has no maps
       tma_prefetch_desc(&maps.cols);
-      for (int i = kMode == kDw ? 2 : S::kPair ? 0 : 1; i < 3; ++i) tma_prefetch_desc(&maps.rows[i]);
+      for (int i = 0; i < 4; ++i)
+        if (used_map<S>(i) && (kMode != kDw || i == 3)) tma_prefetch_desc(&maps.rows[i]);
     }
   }
   if (warp == 1) {
@@ -1135,9 +1149,10 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Maps maps;
   B2M_TRY(encode_map(&maps.cols, type, 3, w.ptr, w_dims, w_strides, w_box, what));
-  const cuuint32_t b_rows = narrow ? Narrow::kBRows : Wide::kBRows;
-  for (int i = narrow ? 1 : 0; i < 3; ++i) {  // a narrow tile's MMA takes half of its rows at least
-    const cuuint32_t box[2] = {in_row, b_rows >> (2 - i)};
+  const cuuint32_t quarter = (narrow ? Narrow::kBRows : Wide::kBRows) / 4;
+  for (int i = 0; i < 4; ++i) {
+    if (narrow ? !used_map<Narrow>(i) : !used_map<Wide>(i)) continue;
+    const cuuint32_t box[2] = {in_row, quarter * (i + 1)};
     B2M_TRY(encode_map(&maps.rows[i], type, 2, x.ptr, x_dims, x_strides, box, what));
   }
   if (narrow) return launch<kMode, kI8, Narrow>(maps, p, row_tiles * p.m_tiles, num_sms, s);
@@ -1232,7 +1247,7 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   Maps maps{};
   if (rows > 0) {
     B2M_TRY(encode_map(&maps.cols, type, 2, x, x_dims, x_strides, box, what));
-    B2M_TRY(encode_map(&maps.rows[2], type, 2, dy, dy_dims, dy_strides, box, what));
+    B2M_TRY(encode_map(&maps.rows[3], type, 2, dy, dy_dims, dy_strides, box, what));
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return launch<kDw, false, Wide>(maps, p, tiles, num_sms, s);
