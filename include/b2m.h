@@ -423,7 +423,7 @@ int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, 
  * A NaN in a row makes its scale NaN, an infinity makes it infinite; the codes of such values
  * are 0, so whatever is multiplied with the row becomes NaN.  Any strides and alignment. */
 int b2m_quant_i8(const void* x, int32_t in_type, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
-                 float* scale, void* stream);
+                 float* scale, int32_t* dev_status, void* stream);
 
 /* 8-bit integer product with scales for each token and channel:
  *   out[t, n] = (float)(sum_k a[t, k] w[e, n, k]) * a_scale[t] * w_scale[e, n]

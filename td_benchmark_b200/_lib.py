@@ -57,7 +57,7 @@ SIGNATURES: dict[str, list] = {
     "b2m_grouped_mm": [_p, _i64, _i64, _p, _i32, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _i32, _i32, _p, _p],
     "b2m_grouped_mm_dx": [_p, _i64, _i64, _p, _i32, _i64, _i64, _i64, _i64, _p, _i32, _p, _i64, _i32, _i32, _p, _p],
     "b2m_grouped_mm_dw": [_p, _i64, _p, _i64, _i64, _i64, _i64, _p, _i32, _i32, _p, _i64, _i64, _i32, _p, _p],
-    "b2m_quant_i8": [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p],
+    "b2m_quant_i8": [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _p, _p],
     "b2m_int8_mm": [_p, _p, _i64, _i64, _p, _p, _i32, _i64, _i64, _i64, _i64, _p, _p, _i64, _i32, _i32, _p, _p],
 }
 

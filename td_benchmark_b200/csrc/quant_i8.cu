@@ -4,11 +4,15 @@
 //   q     = rne(x / scale) within +-127  IEEE fp32 division for each element
 //
 // A group of 32 to 1024 threads owns a row and keeps it in registers as loaded (up to four
-// 16-byte vectors in each thread) between the maximum and the codes, so x is read once; wider
-// rows are read a second time, from L2.  The next row's vectors are in flight while a row is
-// worked on.  Bound by HBM: size + 1 bytes for each element (8192 x 7168 bf16: see below).
+// 16-byte vectors in each thread) between the maximum and the codes, so x is read once.
+// Bound by HBM: size + 1 bytes for each element.  Rows that bulk copies can read go through a
+// ring of three stages in shared memory, which keeps three rows of every block in flight; rows
+// of other alignments are loaded by their threads, and rows wider than the group's registers
+// are read a second time, from L2.
 #include <cuda_fp16.h>
 #include <math.h>
+
+#include <atomic>
 
 #include "b2m_common.cuh"
 #include "b2m_host.h"
@@ -147,81 +151,142 @@ __device__ __forceinline__ void store_codes(int8_t* __restrict__ q, int64_t cols
   }
 }
 
-// blockDim = rows of the block x group; group = 32 .. 1024 threads of a row.
+// Largest value of the group's partial maxima, in every thread of it.  `part`: one value for
+// each warp of the block, of two sets used in turn.  False in all threads when `ok` is in one.
+__device__ __forceinline__ bool group_max(float& amax, float* part, int group, bool ok) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  if (lane == 0) part[threadIdx.x >> 5] = amax;
+  ok = __syncthreads_and(ok);
+  if (group > 32) {
+    amax = part[((threadIdx.x & ~(group - 1)) >> 5) + (lane & (group / 32 - 1))];
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+  }
+  return ok;
+}
+
+constexpr int kRing = 3;
+
+// blockDim = rows of a stage x group; group = 32 .. 1024 threads of a row.  Rows are `row_bytes`
+// (a multiple of 16) in stages of `stage_bytes`, 16-byte aligned in x.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+    quant_i8_ring_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int8_t* __restrict__ q,
+                         int64_t ldq, float* __restrict__ scale, int group, int stage_bytes, int32_t* status,
+                         uint64_t timeout_ns) {
+  constexpr int N = 16 / sizeof(T);
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ uint64_t full[kRing];
+  __shared__ float part[2][32];
+  __shared__ int abort;
+  const int in_row = threadIdx.x & (group - 1);
+  const int at = threadIdx.x / group, per = blockDim.x / group;  // row of the stage
+  const int row_bytes = static_cast<int>(cols * sizeof(T)), vecs = row_bytes / 16;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * per;
+  auto fetch = [&](int64_t first, int s) {  // rows first .. first + per - 1
+    const int n = static_cast<int>(rows - first < per ? rows - first : per);
+    mbar_arrive_expect_tx(&full[s], static_cast<uint32_t>(n * row_bytes));
+    for (int i = 0; i < n; ++i)
+      bulk_load(ring + s * stage_bytes + i * row_bytes, x + (first + i) * ldx, static_cast<uint32_t>(row_bytes), &full[s]);
+  };
+  int64_t first = static_cast<int64_t>(blockIdx.x) * per;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kRing; ++s) mbar_init(&full[s], 1);
+    abort = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+    for (int s = 0; s < kRing; ++s)
+      if (first + s * step < rows) fetch(first + s * step, s);
+  }
+  __syncthreads();
+  int s = 0, phase = 0;
+  for (int round = 0; first < rows; first += step, round ^= 1) {
+    bool ok = mbar_wait(&full[s], phase, timeout_ns, status, B2M_STATUS_TIMEOUT_PRODUCER, &abort);
+    const int64_t r = first + at;
+    const uint4* row = reinterpret_cast<const uint4*>(ring + s * stage_bytes + at * row_bytes);
+    uint4 v[kVecs];
+    uint32_t most = 0;
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+      if (r < rows && in_row + u * group < vecs) v[u] = row[in_row + u * group];
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+      if (r < rows && in_row + u * group < vecs) most = larger_vec<T>(most, v[u]);
+    float amax = Word<T>::top(most);
+    ok = group_max(amax, part[round], group, ok);  // and everyone has read the stage
+    if (!ok) break;
+    if (threadIdx.x == 0 && first + kRing * step < rows) {
+      fence_proxy_async_smem();
+      fetch(first + kRing * step, s);
+    }
+    if (r < rows) {
+      const float sc = max_nan(amax / 127.0f, 1e-12f);
+      if (in_row == 0) scale[r] = sc;
+      const float inv = 1.0f / sc;
+      const bool divide = !(sc < INFINITY);  // the row holds a NaN or an infinity
+#pragma unroll
+      for (int u = 0; u < kVecs; ++u)
+        if (in_row + u * group < vecs)
+          store_codes<T, true>(q + r * ldq, cols, in_row + u * group, sc, inv, divide, v[u]);
+    }
+    if (++s == kRing) s = 0, phase ^= 1;
+  }
+  // after a timeout: the copies in flight may still land; wait for them, within the limit
+  if (first < rows && threadIdx.x == 0) {
+    for (int i = 0; i < kRing && first < rows; ++i, first += step) {
+      mbar_wait(&full[s], phase, timeout_ns, status, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
+      if (++s == kRing) s = 0, phase ^= 1;
+    }
+  }
+}
+
+// The same for any alignment and width; each thread loads what it works on.
 template <typename T, bool kAligned, bool kInRegisters>
 __global__ void __launch_bounds__(1024)
     quant_i8_kernel(const T* __restrict__ x, int64_t rows, int64_t cols, int64_t ldx, int8_t* __restrict__ q,
                     int64_t ldq, float* __restrict__ scale, int group) {
   constexpr int N = 16 / sizeof(T);
-  __shared__ float part[2][32];
-  const int lane = threadIdx.x & 31;
-  const int warp = threadIdx.x >> 5;
+  __shared__ float part[32];
   const int in_row = threadIdx.x & (group - 1);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / group);
-  const int vecs = static_cast<int>((cols + N - 1) / N);
-  int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * (blockDim.x / group) + threadIdx.x / group;
+  const int64_t vecs = r < rows ? (cols + N - 1) / N : 0;
+  const T* row = x + r * ldx;
   uint4 v[kInRegisters ? kVecs : 1];
+  uint32_t most = 0;
   if (kInRegisters) {
 #pragma unroll
     for (int u = 0; u < kVecs; ++u)
-      if (r < rows && in_row + u * group < vecs) v[u] = load_vec<T, kAligned>(x + r * ldx, cols, in_row + u * group);
+      if (in_row + u * group < vecs) v[u] = load_vec<T, kAligned>(row, cols, in_row + u * group);
+#pragma unroll
+    for (int u = 0; u < kVecs; ++u)
+      if (in_row + u * group < vecs) most = larger_vec<T>(most, v[u]);
+  } else {
+    for (int64_t i = in_row; i < vecs; i += group) most = larger_vec<T>(most, load_vec<T, kAligned>(row, cols, i));
   }
-  // every thread of the block makes the same number of rounds
-  for (int64_t first = r - threadIdx.x / group, round = 0; first < rows; first += step, r += step, ++round) {
-    const bool mine = r < rows;
-    const T* row = x + r * ldx;
-    uint4 next[kInRegisters ? kVecs : 1];
-    uint32_t most = 0;
-    if (kInRegisters) {
-      const int64_t rn = r + step;
+  float amax = Word<T>::top(most);
+  group_max(amax, part, group, true);
+  if (r >= rows) return;
+  const float sc = max_nan(amax / 127.0f, 1e-12f);
+  if (in_row == 0) scale[r] = sc;
+  const float inv = 1.0f / sc;
+  const bool divide = !(sc < INFINITY);  // the row holds a NaN or an infinity
+  int8_t* qr = q + r * ldq;
+  if (kInRegisters) {
 #pragma unroll
-      for (int u = 0; u < kVecs; ++u)
-        if (rn < rows && in_row + u * group < vecs)
-          next[u] = load_vec<T, kAligned>(x + rn * ldx, cols, in_row + u * group);
-#pragma unroll
-      for (int u = 0; u < kVecs; ++u)
-        if (mine && in_row + u * group < vecs) most = larger_vec<T>(most, v[u]);
-    } else if (mine) {
-      for (int i = in_row; i < vecs; i += group) most = larger_vec<T>(most, load_vec<T, kAligned>(row, cols, i));
-    }
-    float amax = Word<T>::top(most);
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-    if (group > 32) {
-      float* p = part[round & 1];  // the other half is still read by warps of the round before
-      if (lane == 0) p[warp] = amax;
-      __syncthreads();
-      const int at = (threadIdx.x & ~(group - 1)) >> 5;
-      amax = p[at + (lane & (group / 32 - 1))];
-#pragma unroll
-      for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-    }
-    if (mine) {
-      const float s = max_nan(amax / 127.0f, 1e-12f);
-      if (in_row == 0) scale[r] = s;
-      const float inv = 1.0f / s;
-      const bool divide = !(s < INFINITY);  // the row holds a NaN or an infinity
-      int8_t* qr = q + r * ldq;
-      if (kInRegisters) {
-#pragma unroll
-        for (int u = 0; u < kVecs; ++u)
-          if (in_row + u * group < vecs)
-            store_codes<T, kAligned>(qr, cols, in_row + u * group, s, inv, divide, v[u]);
-      } else {
-        for (int i = in_row; i < vecs; i += group)
-          store_codes<T, kAligned>(qr, cols, i, s, inv, divide, load_vec<T, kAligned>(row, cols, i));
-      }
-    }
-    if (kInRegisters) {
-#pragma unroll
-      for (int u = 0; u < kVecs; ++u) v[u] = next[u];
-    }
+    for (int u = 0; u < kVecs; ++u)
+      if (in_row + u * group < vecs)
+        store_codes<T, kAligned>(qr, cols, in_row + u * group, sc, inv, divide, v[u]);
+  } else {
+    for (int64_t i = in_row; i < vecs; i += group)
+      store_codes<T, kAligned>(qr, cols, i, sc, inv, divide, load_vec<T, kAligned>(row, cols, i));
   }
 }
 
 template <typename T>
 int launch_quant(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq, float* scale,
-                 int num_sms, cudaStream_t s) {
+                 int32_t* status, int num_sms, cudaStream_t s) {
   constexpr int N = 16 / sizeof(T);
   const int64_t vecs = (cols + N - 1) / N;
   // Threads of a row: as few as hold it, and more while there are too few rows to fill the
@@ -233,14 +298,33 @@ int launch_quant(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q
   const bool aligned = aligned16(x) && ldx * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(q) % N == 0 && ldq % N == 0;
   const int block = group > kBlock ? group : kBlock;
   const int64_t per_block = block / group;
-  // four resident blocks of 256 threads on each SM (64 registers a thread), each several rows
-  const int64_t resident = int64_t(num_sms) * (1024 / block);
   const int64_t blocks = (rows + per_block - 1) / per_block;
-  const int64_t grid = blocks < resident ? blocks : resident;
+  if (blocks > INT32_MAX) return fail(B2M_ERR_ARG, "quant_i8: too many rows (%lld)", (long long)rows);
+  // Blocks that are resident together: 1024 threads an SM (64 registers each), and their rings.
+  const int64_t stage = per_block * cols * sizeof(T);
+  int64_t per_sm = 1024 / block;
+  if (per_sm * (kRing * stage + 2048) > 225 * 1024) per_sm = 225 * 1024 / (kRing * stage + 2048);
+  // The ring pays from the second row of a block on; with one row each, its set-up only adds to
+  // the row's time.
+  if (aligned && fits && cols % N == 0 && per_sm > 0 && blocks > per_sm * num_sms) {
+    static std::atomic<bool> attr_done[64];
+    int dev = 0;
+    B2M_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
+    if (dev >= 64 || !attr_done[dev].load(std::memory_order_acquire)) {
+      B2M_TRY(check_cuda(cudaFuncSetAttribute(quant_i8_ring_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                              224 * 1024),
+                         "quant_i8: cudaFuncSetAttribute"));
+      if (dev < 64) attr_done[dev].store(true, std::memory_order_release);
+    }
+    quant_i8_ring_kernel<T><<<static_cast<int>(per_sm * num_sms), block, kRing * stage, s>>>(
+        static_cast<const T*>(x), rows, cols, ldx, static_cast<int8_t*>(q), ldq, scale, group, static_cast<int>(stage),
+        status, 2 * timeout_ns());
+    return check_cuda(cudaGetLastError(), "quant_i8 launch");
+  }
   auto kernel = aligned ? (fits ? quant_i8_kernel<T, true, true> : quant_i8_kernel<T, true, false>)
                         : (fits ? quant_i8_kernel<T, false, true> : quant_i8_kernel<T, false, false>);
-  kernel<<<static_cast<int>(grid), block, 0, s>>>(static_cast<const T*>(x), rows, cols, ldx, static_cast<int8_t*>(q),
-                                                  ldq, scale, group);
+  kernel<<<static_cast<int>(blocks), block, 0, s>>>(static_cast<const T*>(x), rows, cols, ldx, static_cast<int8_t*>(q),
+                                                    ldq, scale, group);
   return check_cuda(cudaGetLastError(), "quant_i8 launch");
 }
 
@@ -248,7 +332,7 @@ int launch_quant(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q
 }  // namespace b2m
 
 extern "C" int b2m_quant_i8(const void* x, int32_t in_type, int64_t rows, int64_t cols, int64_t ldx, void* q,
-                            int64_t ldq, float* scale, void* stream) {
+                            int64_t ldq, float* scale, int32_t* dev_status, void* stream) {
   using namespace b2m;
   if (rows < 0 || cols < 1 || cols > (int64_t(1) << 30) || ldx < cols || ldq < cols)
     return fail(B2M_ERR_ARG, "quant_i8: bad shape [%lld, %lld], row strides %lld and %lld", (long long)rows,
@@ -262,7 +346,8 @@ extern "C" int b2m_quant_i8(const void* x, int32_t in_type, int64_t rows, int64_
   B2M_TRY(require_sm100(&num_sms));
   if (rows == 0) return B2M_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (in_type == B2M_BF16) return launch_quant<__nv_bfloat16>(x, rows, cols, ldx, q, ldq, scale, num_sms, s);
-  if (in_type == B2M_FP16) return launch_quant<__half>(x, rows, cols, ldx, q, ldq, scale, num_sms, s);
-  return launch_quant<float>(x, rows, cols, ldx, q, ldq, scale, num_sms, s);
+  if (in_type == B2M_BF16)
+    return launch_quant<__nv_bfloat16>(x, rows, cols, ldx, q, ldq, scale, dev_status, num_sms, s);
+  if (in_type == B2M_FP16) return launch_quant<__half>(x, rows, cols, ldx, q, ldq, scale, dev_status, num_sms, s);
+  return launch_quant<float>(x, rows, cols, ldx, q, ldq, scale, dev_status, num_sms, s);
 }

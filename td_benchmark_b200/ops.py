@@ -434,8 +434,8 @@ class _GroupedMM(torch.autograd.Function):
         return dx, dw, None, None
 
 
-def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tensor | None = None
-               ) -> tuple[torch.Tensor, torch.Tensor]:
+def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+               status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 / fp16 / fp32 [rows, cols] -> (int8 [rows, cols], fp32 [rows]): ``scale = max(amax / 127, 1e-12)``,
     ``q = rne(x / scale)`` within +-127, both divisions IEEE fp32.
 
@@ -460,7 +460,7 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
     else:
         _vector(scale, "scale", (rows,), torch.float32, device)
     _launch(device, "b2m_quant_i8", x.data_ptr(), code, rows, cols, strides[0] if rows > 1 else cols, q.data_ptr(), ldq,
-            scale.data_ptr())
+            scale.data_ptr(), None if status is None else _status_word(status, device))
     return q, scale
 
 

@@ -259,7 +259,8 @@ def _quant_ref(x):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 7168), (3, 7), (33, 129), (257, 64), (5, 1000), (64, 4096), (9, 8191),
-                                       (3, 32768), (2, 70001)])
+                                       (3, 32768), (2, 70001), (5000, 64), (3001, 24), (1500, 2048), (700, 7168),
+                                       (900, 16384)])
 def test_quant_int8_is_exact(rows, cols, dtype):
     x = _randn(rows, cols, seed=rows + cols, dtype=dtype, std=3.0)
     if rows > 2:

@@ -10,7 +10,7 @@ MM = dict(x=P, rows=8, ldx=64, w=P, experts=4, n=32, k=64, ldw=64, w_stride=2048
           out_type=BF16, clear=1, status=None, stream=None)
 DW = dict(dy=P, lddy=32, x=P, ldx=64, rows=8, n=32, k=64, ends=P, experts=4, in_type=BF16, out=P, ldo=64,
           out_stride=2048, out_type=BF16, status=None, stream=None)
-QUANT = dict(x=P, in_type=BF16, rows=4, cols=64, ldx=64, q=P, ldq=64, scale=P, stream=None)
+QUANT = dict(x=P, in_type=BF16, rows=4, cols=64, ldx=64, q=P, ldq=64, scale=P, status=None, stream=None)
 INT8 = dict(a=P, a_scale=P, rows=8, lda=64, w=P, w_scale=P, experts=4, n=32, k=64, ldw=64, w_stride=2048, ends=P, out=P,
             ldo=32, out_type=BF16, clear=1, status=None, stream=None)
 
