@@ -30,12 +30,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// What a 32-bit word of the row holds: two 16-bit values or one of 32 bits.
+// What a 32-bit word of the row holds: two 16-bit values or one of 32 bits.  `larger` keeps the
+// larger magnitudes (its signs mean nothing), `top` is the larger magnitude of a word.
 template <typename T>
 struct Word;
 template <>
 struct Word<float> {
-  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t w) {  // a >= 0, |w|
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t w) {
     return __float_as_uint(max_nan(__uint_as_float(a), fabsf(__uint_as_float(w))));
   }
   static __device__ __forceinline__ float top(uint32_t a) { return __uint_as_float(a); }
@@ -45,11 +46,11 @@ template <>
 struct Word<__nv_bfloat16> {
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t w) {
     uint32_t r;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(w & 0x7FFF7FFFu));
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(w));
     return r;
   }
   static __device__ __forceinline__ float top(uint32_t a) {
-    return max_nan(__uint_as_float(a << 16), __uint_as_float(a & 0xFFFF0000u));
+    return max_nan(fabsf(__uint_as_float(a << 16)), fabsf(__uint_as_float(a & 0xFFFF0000u)));
   }
   static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
     f[0] = __uint_as_float(w << 16);
@@ -60,12 +61,12 @@ template <>
 struct Word<__half> {
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t w) {
     uint32_t r;
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(w & 0x7FFF7FFFu));
+    asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(w));
     return r;
   }
   static __device__ __forceinline__ float top(uint32_t a) {
     const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&a));
-    return max_nan(v.x, v.y);
+    return max_nan(fabsf(v.x), fabsf(v.y));
   }
   static __device__ __forceinline__ void unpack(uint32_t w, float* f) {
     const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -99,26 +100,45 @@ __device__ __forceinline__ uint32_t larger_vec(uint32_t a, const uint4& v) {
 
 // Codes of one vector.  x * (1 / scale) is within 1.6e-5 of x / scale (two roundings of a
 // value of at most 127) and the IEEE quotient within 4e-6, so both round to the same integer
-// unless the product lies within 2e-5 of a tie; a vector that comes within kNearTie of one
-// (one in 1500) is divided.  Adding 1.5 * 2^23 rounds to the nearest even integer and leaves
-// it in the low byte.  A division for each element would cost more than the memory traffic
-// (8192 x 7168 bf16: 78 us of divisions against 27 us of HBM).
+// unless the product lies within 2e-5 of a tie; values that come within kNearTie of one are
+// divided.  (Of 16-bit values one in a thousand does, since x / scale is 127 times a ratio of
+// short integers.)  Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the
+// low byte.  A division for each element would cost more than the memory traffic (8192 x 7168
+// bf16: 81 us with them; 27 us is what HBM needs).
 constexpr float kNearTie = 4e-5f;
 constexpr float kRound = 12582912.0f;
+
+// Two values at once: r = x * inv + kRound, and d = x * inv + (kRound - r), what rounding left.
+__device__ __forceinline__ void round_two(float x0, float x1, float inv, float& r0, float& r1, float& d0, float& d1) {
+  asm("{\n\t.reg .b64 x, i, k, n, r, d;\n\t"
+      "mov.b64 x, {%4, %5};\n\t"
+      "mov.b64 i, {%6, %6};\n\t"
+      "mov.b64 k, {%7, %7};\n\t"
+      "mov.b64 n, {%8, %8};\n\t"
+      "fma.rn.f32x2 r, x, i, k;\n\t"
+      "fma.rn.f32x2 d, r, n, k;\n\t"
+      "fma.rn.f32x2 d, x, i, d;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t"
+      "mov.b64 {%2, %3}, d;\n\t}"
+      : "=f"(r0), "=f"(r1), "=f"(d0), "=f"(d1)
+      : "f"(x0), "f"(x1), "f"(inv), "f"(kRound), "f"(-1.0f));
+}
 
 template <int N>
 __device__ __forceinline__ void codes_of(const float (&f)[N], float scale, float inv, bool divide,
                                          uint32_t (&w)[N / 4]) {
   float r[N], off = 0.0f;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    r[j] = __fmaf_rn(f[j], inv, kRound);
-    off = fmaxf(off, fabsf(__fmaf_rn(f[j], inv, kRound - r[j])));
+  for (int j = 0; j < N; j += 2) {
+    float d0, d1;
+    round_two(f[j], f[j + 1], inv, r[j], r[j + 1], d0, d1);
+    off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
   }
   if (divide || off > 0.5f - kNearTie) {
 #pragma unroll
-    for (int j = 0; j < N; ++j)  // a NaN quotient converts to 0
-      r[j] = __int_as_float(max(-127, min(127, __float2int_rn(f[j] / scale))));
+    for (int j = 0; j < N; ++j)
+      if (divide || fabsf(__fmaf_rn(f[j], inv, kRound - r[j])) > 0.5f - kNearTie)
+        r[j] = __int_as_float(max(-127, min(127, __float2int_rn(f[j] / scale))));  // a NaN quotient converts to 0
   }
 #pragma unroll
   for (int i = 0; i < N / 4; ++i)
