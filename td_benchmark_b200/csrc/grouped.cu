@@ -1061,8 +1061,14 @@ int launch(const Maps& maps, const Params& p, int64_t tiles_bound, int num_sms, 
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
+constexpr int64_t kMaxTiles = int64_t(1) << 30;
 
 uint32_t magic(int64_t d) { return static_cast<uint32_t>(((uint64_t(1) << 32) + d - 1) / d); }
+
+// Limit of a wait inside a CTA's pipeline, where nothing but the CTA's own work is waited for: a
+// sum of `blocks` blocks takes a third of a microsecond for each, and a role may wait for
+// several tiles.
+uint64_t wait_limit(int64_t blocks) { return 2 * timeout_ns() + 8000ull * static_cast<uint64_t>(blocks); }
 
 int check_matrix(const char* what, const char* name, const Matrix& m, int elem) {
   if (m.rows < 0 || m.rows > kMaxDim || m.cols < 1 || m.cols > kMaxDim)
@@ -1116,8 +1122,13 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   p.segments = p.experts + (clear_rest ? 1 : 0);
   p.rows = x.rows;
   p.m_dim = static_cast<int32_t>(m_dim);
-  // Row tiles of 32 while segments are short on average: the ring then holds weights, not room for rows.
-  const bool narrow = (x.rows + w.experts - 1) / w.experts <= Narrow::NT;
+  // Row tiles of 32, one CTA each, while segments are short: weights alone bound these calls,
+  // the ring then holds more of them, and twice as many CTAs share them out (E=32, 4096 x 7168,
+  // forward: 274 us narrow, 288 wide at 8 rows each).  The mean is all that the host knows of
+  // the lengths.  Under Zipf 1.2 the longest segments cost a narrow launch more than it saves from
+  // 16 rows on average (299 narrow, 292 wide; 377 and 311 at 32), and not yet at 12 (278, 292).
+  // One segment alone has the length that the host sees: up to one narrow tile.
+  const bool narrow = x.rows <= (w.experts == 1 ? Narrow::NT : 12 * w.experts);
   const int64_t nt = narrow ? Narrow::NT : Wide::NT, tile_m = narrow ? Narrow::kTileM : Wide::kTileM;
   p.m_tiles = static_cast<int32_t>((m_dim + tile_m - 1) / tile_m);
   p.k_blocks = static_cast<int32_t>((sum + in_row - 1) / in_row);
@@ -1130,7 +1141,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   p.a_scale = a_scale;
   p.w_scale = w_scale;
   p.status = status;
-  p.timeout_ns = 2 * timeout_ns();
+  p.timeout_ns = wait_limit(p.k_blocks);
   p.idesc = (kI8 ? (2u << 4) | (1u << 7) | (1u << 10)                                             // S32, both signed
                  : (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u)) |             // F32
             (kMode == kDx ? 1u << 15 : 0u) | (static_cast<uint32_t>(tile_m >> 4) << 24);
@@ -1142,12 +1153,12 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows)};
   const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
   const int64_t row_tiles = (x.rows + nt - 1) / nt + (x.rows < p.segments ? x.rows : p.segments);
-  if (row_tiles * p.m_tiles > INT32_MAX) return fail(B2M_ERR_ARG, "%s: more than 2^31 tiles", what);
+  if (row_tiles * p.m_tiles > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
   int num_sms = 0;
   B2M_TRY(device_ready(&num_sms));
   if (x.rows == 0) return B2M_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  Maps maps;
+  Maps maps{};
   B2M_TRY(encode_map(&maps.cols, type, 3, w.ptr, w_dims, w_strides, w_box, what));
   const cuuint32_t quarter = (narrow ? Narrow::kBRows : Wide::kBRows) / 4;
   for (int i = 0; i < 4; ++i) {
@@ -1229,11 +1240,11 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   p.out_type = out_type;
   p.wide_out = aligned16(out) && ldo % 8 == 0 && out_stride % 8 == 0;
   p.status = dev_status;
-  p.timeout_ns = 2 * timeout_ns();
+  p.timeout_ns = wait_limit(rows / 64);
   p.idesc = (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) |
             (static_cast<uint32_t>(Wide::kTileM >> 4) << 24);
   const int64_t tiles = int64_t(p.m_tiles) * p.c_tiles * experts;
-  if (tiles > INT32_MAX) return fail(B2M_ERR_ARG, "%s: more than 2^31 tiles", what);
+  if (tiles > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
   int num_sms = 0;
   B2M_TRY(device_ready(&num_sms));
   const CUtensorMapDataType type =

@@ -76,6 +76,10 @@ SHAPES = [
     ([1] * 200 + [0] * 56 + [3] * 10, 2, 264, 192),
     ([2, 0, 0, 1] * 256, 0, 64, 128),
     ([5000, 3, 1200], 5, 640, 704),
+    ([700, 0, 41, 3] + [0] * 96, 0, 136, 200),          # short on average, one segment of many tiles
+    ([40] * 300, 0, 72, 80),                              # long on average, more segments than are sorted
+    ([20, 0] * 512, 7, 16, 64),                           # 1024 experts
+    ([257, 513, 1025, 1793, 2049, 256, 512], 0, 264, 96),  # lengths that tiles share evenly
 ]
 
 
