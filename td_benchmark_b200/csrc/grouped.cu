@@ -46,25 +46,44 @@ constexpr int kABytes = kM * kRowBytes;
 constexpr int kBand = 8;           // row tiles walked together, so that they share a weight tile in L2
 constexpr int kSortMost = 256;     // experts up to which segments are sorted by length
 constexpr int kFeed = 4;           // tiles found ahead
+constexpr int kSplitTiles = 64;    // most tiles of a launch whose CTAs share sums
 constexpr int kStagePitch = 144;   // bytes between two staged output rows of 128: no bank is hit twice
 
 // A tile is NT output rows by 128 output columns, or, for a pair of CTAs, by 256: each CTA
 // keeps the operand rows and the accumulator of its own 128 columns and half of the row
 // operand, and the leader's MMAs (cta_group::2) read both halves.
-template <int kRows, bool kTwoCtas>
+//
+// Where there are too few tiles for the SMs, the CTAs of a cluster share a tile along its sum
+// (kSplit): each multiplies its part of the blocks, and each adds up all parts for its share
+// of the output columns.
+template <int kRows, bool kTwoCtas, bool kSplitSum>
 struct Shape {
   static constexpr int NT = kRows;
   static constexpr bool kPair = kTwoCtas;
+  static constexpr bool kSplit = kSplitSum;
   static constexpr int kCtas = kPair ? 2 : 1;
   static constexpr int kTileM = kM * kCtas;
   static constexpr int kBRows = NT / kCtas;         // rows of the row operand in one CTA
   static constexpr int kStep = 16 * kCtas;          // granularity of N in an MMA
   static constexpr int kStageBytes = kABytes + kBRows * kRowBytes;
-  static constexpr int kStages = kPair ? 6 : 9;
+  static constexpr int kStages = kPair ? 6 : kSplit ? 4 : 9;  // split: two CTAs fit on an SM
+  static constexpr int kReaders = kSplit ? kEpiWarps / 2 : kEpiWarps;  // epilogue warps that take tiles
   static constexpr uint32_t kTmemCols = 2 * NT;
 };
-using Wide = Shape<256, true>;
-using Narrow = Shape<32, false>;
+using Wide = Shape<256, true, false>;
+using Narrow = Shape<32, false, false>;
+using Split = Shape<32, false, true>;
+constexpr int kMostParts = 8;
+
+// What the CTAs of a split tile hand to each other: for every part, the accumulators of the
+// columns that this CTA adds up.  A cluster has one tile at most.
+template <bool kSplit>
+struct Join {};
+template <>
+struct Join<true> {
+  uint64_t full;  // every part's accumulators are here
+  alignas(16) uint32_t part[Split::NT * kM];
+};
 
 // One output tile: rows [row0, row0 + cols) of the output (kDw: of expert e's output),
 // columns from m0.  k_blocks == 0: all zero, nothing is multiplied.  e < 0: no tile is left.
@@ -76,7 +95,7 @@ struct alignas(16) Tile {
   int k_blocks;
   int sum0;      // kDw: first row of the sum
   int sum_rows;  // kDw: rows of the sum
-  int pad;
+  int k0;        // first block of this CTA's part of the sum
 };
 
 template <class S>
@@ -98,7 +117,9 @@ struct Control {
   alignas(16) int32_t start[kMaxExperts + 4];  // first row of segment e; [E] = end of the last, [E + 1] = rows
   int32_t tile0[kMaxExperts + 2];  // row tiles before the segment at place r of the walk
   uint16_t seg[kMaxExperts + 2];   // the segment at place r
-  alignas(16) uint8_t staging[kEpiWarps / 2][32 * kStagePitch];  // 32 output rows of 64 columns, for two warps
+  // 32 output rows of 64 columns, for two warps each
+  alignas(16) uint8_t staging[S::kSplit ? 1 : kEpiWarps / 2][S::kSplit ? 16 : 32 * kStagePitch];
+  Join<S::kSplit> join;
 };
 
 template <class S>
@@ -129,6 +150,7 @@ struct Params {
   int32_t c_dim;         // kDw: output rows of one expert
   int32_t c_tiles;       // kDw
   int32_t k_blocks;      // kFwd, kDx: blocks of the sum
+  int32_t parts;         // CTAs that share a tile's sum
   uint32_t m_magic;      // for division by m_tiles, by kBand * m_tiles and (kDw) by m_tiles * c_tiles
   uint32_t band_magic;
   uint32_t expert_magic;
@@ -408,7 +430,8 @@ __device__ __forceinline__ void plan_wide(const Params& p, Control<S>* C) {
 struct Where {
   uint32_t rank;
   int first;   // first tile
-  int stride;  // pairs (or CTAs) in the grid
+  int stride;  // pairs (or CTAs, or clusters that share tiles) in the grid
+  int part;    // of a tile's sum
 };
 
 // Warp 3, one lane: this CTA's tiles, on their way to its other roles.  Finding a tile takes
@@ -431,6 +454,11 @@ __device__ __forceinline__ void feed_tiles(const Params& p, Control<S>* C, int n
     Tile r{};
     r.e = -1;
     if (t < num_tiles) r = tile_at<kMode, S>(p, C, t);
+    if (S::kSplit) {
+      const int blocks = r.k_blocks;
+      r.k0 = blocks * at.part / p.parts;
+      r.k_blocks = blocks * (at.part + 1) / p.parts - r.k0;
+    }
     const bool last = i * at.stride >= num_tiles;  // no CTA has a tile in this round
     if (r.e >= 0 || last) {
       if (!mbar_try_wait(&C->taken[s], phase ^ 1) &&
@@ -465,6 +493,7 @@ struct TileFeed {
     r.k_blocks = __shfl_sync(0xffffffffu, v.k_blocks, 0);
     r.sum0 = __shfl_sync(0xffffffffu, v.sum0, 0);
     r.sum_rows = __shfl_sync(0xffffffffu, v.sum_rows, 0);
+    r.k0 = S::kSplit ? __shfl_sync(0xffffffffu, v.k0, 0) : 0;
     if ((threadIdx.x & 31) == 0) mbar_arrive(&C->taken[s]);
     if (++s == kFeed) s = 0, phase ^= 1;
     return true;
@@ -599,12 +628,12 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
           mbar_arrive_expect_tx(&C->full[s], S::kCtas * bytes);
         }
         if (kMode == kFwd) {
-          load_3d<S::kPair>(a, map_cols, bar, kb * kElems, m0, r.e);
-          load_2d<S::kPair>(b, map_rows, bar, kb * kElems, row);
+          load_3d<S::kPair>(a, map_cols, bar, (r.k0 + kb) * kElems, m0, r.e);
+          load_2d<S::kPair>(b, map_rows, bar, (r.k0 + kb) * kElems, row);
         } else if (kMode == kDx) {
-          load_3d<S::kPair>(a, map_cols, bar, m0, kb * 64, r.e);
-          load_3d<S::kPair>(a + kABytes / 2, map_cols, bar, m0 + 64, kb * 64, r.e);
-          load_2d<S::kPair>(b, map_rows, bar, kb * kElems, row);
+          load_3d<S::kPair>(a, map_cols, bar, m0, (r.k0 + kb) * 64, r.e);
+          load_3d<S::kPair>(a + kABytes / 2, map_cols, bar, m0 + 64, (r.k0 + kb) * 64, r.e);
+          load_2d<S::kPair>(b, map_rows, bar, (r.k0 + kb) * kElems, row);
         } else {
           const int sum = r.sum0 + kb * 64;
           load_2d<S::kPair>(a, map_cols, bar, m0, sum);
@@ -922,16 +951,81 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, uint32_
   }
 }
 
+// One output element.
+__device__ __forceinline__ void put(void* out, int64_t at, int32_t type, float v) {
+  if (type == B2M_FP32)
+    static_cast<float*>(out)[at] = v;
+  else
+    static_cast<uint16_t*>(out)[at] = static_cast<uint16_t>(pack_16bit(v, 0.0f, type == B2M_BF16));
+}
+
+// Epilogue of a split sum, warps 4-7.  Of the tile's 128 columns (TMEM lanes), CTA d of the
+// cluster adds up columns d * 128 / parts and following: every CTA sends each of them the
+// accumulators of its part, [part][row][column], and the owner adds them in the order of the
+// parts, so the result does not depend on who comes first.
+template <bool kI8, class S>
+__device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, uint32_t tmem_base, const Where& at,
+                                               int warp, int lane) {
+  const int q = warp & 3;
+  const int share = kM / p.parts;  // columns of one CTA: 16, 32 or 64
+  const int bits = 31 - __clz(share);
+  const int column = q * 32 + lane, owner = column >> bits, in_share = column & (share - 1);
+  TileFeed<S> feed(p, C);
+  Tile r;
+  if (!feed.next(r) || r.e < 0) return;
+  const int64_t out = static_cast<int64_t>(r.row0) * p.ldo + r.m0;
+  if (r.k_blocks == 0) {  // rows of no expert
+    if (at.part == 0 && r.m0 + column < p.m_dim)
+      for (int j = 0; j < r.cols; ++j) put(p.out, out + j * p.ldo + column, p.out_type, 0.0f);
+    return;
+  }
+  if (!wait_warp(&C->tfull[0], 0, p, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort)) return;
+  tc_fence_after();
+  float v[32];
+  tmem_ld32(tmem_base + (static_cast<uint32_t>(q * 32) << 16), v);
+  tmem_ld_wait();
+  tc_fence_before();
+  const uint32_t to =
+      mapa_shared(smem_u32(&C->join.part[at.part * S::NT * share + in_share]), static_cast<uint32_t>(owner));
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < r.cols)
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + static_cast<uint32_t>(j * share * 4)), "f"(v[j])
+                   : "memory");
+  __syncwarp();
+  if ((lane & (share - 1)) == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&C->join.full), owner));
+
+  const bool ok = mbar_wait_cluster(&C->join.full, 0, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort);
+  if (!ok) return;
+  for (int i = column; i < r.cols << bits; i += kM) {
+    const int j = i >> bits, c = at.part * share + (i & (share - 1));
+    if (r.m0 + c >= p.m_dim) continue;
+    const uint32_t* part = &C->join.part[i];
+    float sum;
+    if (kI8) {
+      int acc = 0;
+      for (int k = 0; k < p.parts; ++k) acc += static_cast<int>(part[k * S::NT * share]);
+      sum = __int2float_rn(acc) * __ldg(p.a_scale + r.row0 + j) *
+            __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + r.m0 + c);
+    } else {
+      sum = __uint_as_float(part[0]);
+      for (int k = 1; k < p.parts; ++k) sum += __uint_as_float(part[k * S::NT * share]);
+    }
+    put(p.out, out + j * p.ldo + c, p.out_type, sum);
+  }
+}
+
 template <int kMode, bool kI8, class S>
-__global__ void __launch_bounds__(threads_of(kMode), 1)
+__global__ void __launch_bounds__(threads_of(kMode), S::kSplit ? 2 : 1)
     grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Control<S>* C = reinterpret_cast<Control<S>*>(smem + S::kStages * S::kStageBytes);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0);
   const int lane = threadIdx.x & 31;
-  const Where at{S::kPair ? cluster_ctarank() : 0u, static_cast<int>(blockIdx.x) / S::kCtas,
-                 static_cast<int>(gridDim.x) / S::kCtas};
+  const int ctas = S::kSplit ? p.parts : S::kCtas;  // of a cluster
+  const Where at{S::kPair ? cluster_ctarank() : 0u, static_cast<int>(blockIdx.x) / ctas,
+                 static_cast<int>(gridDim.x) / ctas, S::kSplit ? static_cast<int>(cluster_ctarank()) : 0};
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(&C->full[s], 1);
@@ -941,12 +1035,14 @@ __global__ void __launch_bounds__(threads_of(kMode), 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&C->tfull[b], 1);
-      mbar_init(&C->tempty[b], S::kCtas * kEpiWarps);
+      mbar_init(&C->tempty[b], S::kCtas * S::kReaders);
     }
+    if constexpr (S::kSplit)  // from every part, one arrival for each run of a warp's lanes
+      mbar_init(&C->join.full, p.parts * max(1, S::kReaders / p.parts));
     // readers of a tile: producers, epilogue warps, (kDw) warp 12, and the MMA warp of the leader
     for (int s = 0; s < kFeed; ++s) {
       mbar_init(&C->fed[s], 1);
-      mbar_init(&C->taken[s], 2 + kEpiWarps + (kMode == kDw ? 1 : 0) + (at.rank == 0 ? 1 : 0));
+      mbar_init(&C->taken[s], 2 + S::kReaders + (kMode == kDw ? 1 : 0) + (at.rank == 0 ? 1 : 0));
     }
     mbar_init(&C->mma_done, 1);
     C->abort = 0;
@@ -968,8 +1064,8 @@ __global__ void __launch_bounds__(threads_of(kMode), 1)
   else if (warp == 2)
     plan_narrow<S>(p, C, lane);
   tc_fence_before();
-  if (S::kPair)
-    cluster_sync();  // both CTAs' barriers exist before one CTA signals the other's
+  if (S::kPair || S::kSplit)
+    cluster_sync();  // all barriers exist before one CTA signals another's
   else
     __syncthreads();
   tc_fence_after();
@@ -984,12 +1080,15 @@ __global__ void __launch_bounds__(threads_of(kMode), 1)
     __syncwarp();
   } else if (warp == 12) {
     clear_tails<S>(p, smem, C, lane);
+  } else if constexpr (S::kSplit) {
+    if (warp < 4 + S::kReaders) epilogue_split<kI8, S>(p, C, tmem_base, at, warp, lane);
   } else {
     epilogue<kMode, kI8, S>(p, C, tmem_base, at.rank, warp, lane);
   }
   tc_fence_before();
   __syncthreads();
-  if (S::kPair) cluster_sync();  // the leader's MMAs and the copies it counts are done with both CTAs' memory
+  // the leader's MMAs and the copies it counts, or the other parts, are done with this CTA's memory
+  if (S::kPair || S::kSplit) cluster_sync();
   if (warp == 1) {
     tc_fence_after();
     if (S::kPair)
@@ -1046,17 +1145,18 @@ int launch(const Maps& maps, const Params& p, int64_t tiles_bound, int num_sms, 
                        "grouped: cudaFuncSetAttribute"));
     if (dev < 64) attr_done[dev].store(true, std::memory_order_release);
   }
-  const int64_t most = num_sms / S::kCtas;
+  const int ctas = S::kSplit ? p.parts : S::kCtas;
+  const int64_t most = S::kSplit ? tiles_bound : num_sms / ctas;  // a cluster that shares a sum has one tile
   cudaLaunchAttribute cluster[1];
   cluster[0].id = cudaLaunchAttributeClusterDimension;
-  cluster[0].val.clusterDim = {static_cast<unsigned>(S::kCtas), 1, 1};
+  cluster[0].val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(S::kCtas * (tiles_bound < most ? tiles_bound : most)));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas * (tiles_bound < most ? tiles_bound : most)));
   cfg.blockDim = dim3(threads_of(kMode));
   cfg.dynamicSmemBytes = smem_bytes<S>();
   cfg.stream = s;
   cfg.attrs = cluster;
-  cfg.numAttrs = S::kPair ? 1 : 0;
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, maps, p), "grouped launch");
 }
 
@@ -1119,7 +1219,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   Params p{};
   p.ends = ends;
   p.experts = static_cast<int32_t>(w.experts);
-  p.segments = p.experts + (clear_rest ? 1 : 0);
+  p.segments = p.experts + (clear_rest && ends ? 1 : 0);
   p.rows = x.rows;
   p.m_dim = static_cast<int32_t>(m_dim);
   // Row tiles of 32, one CTA each, while segments are short: weights alone bound these calls,
@@ -1152,7 +1252,9 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   const cuuint32_t w_box[3] = {in_row, kMode == kFwd ? static_cast<cuuint32_t>(kM) : 64u, 1};
   const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows)};
   const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
-  const int64_t row_tiles = (x.rows + nt - 1) / nt + (x.rows < p.segments ? x.rows : p.segments);
+  // most row tiles that x.rows rows can take: one not full for each segment that has rows
+  const int64_t with_rows = x.rows < p.segments ? x.rows : p.segments;
+  const int64_t row_tiles = (x.rows + (nt - 1) * with_rows) / nt;
   if (row_tiles * p.m_tiles > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
   int num_sms = 0;
   B2M_TRY(device_ready(&num_sms));
@@ -1166,7 +1268,22 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
     const cuuint32_t box[2] = {in_row, quarter * (i + 1)};
     B2M_TRY(encode_map(&maps.rows[i], type, 2, x.ptr, x_dims, x_strides, box, what));
   }
-  if (narrow) return launch<kMode, kI8, Narrow>(maps, p, row_tiles * p.m_tiles, num_sms, s);
+  // Too few tiles for the SMs: clusters of two to eight CTAs share each one along its sum, as
+  // many as are resident together (two CTAs on an SM; 33 clusters of eight were), so that a
+  // cluster has one tile.  Each CTA needs blocks enough to be worth the exchange, and more of
+  // them where two share an SM.  Integers, one row: 2048 x 7168 (16 tiles) 16.4 us unshared, 9.3
+  // by eights; 8192 x 8192 (64) 19.3, 16.8 by fours, 18.2 by twos; 4096 x 4096 (32, four blocks
+  // each by eights) 11.5, 9.25 by fours, 10.0 by eights.  From 65 tiles on sharing costs more
+  // than it gives (14336 x 4096, 112 tiles: 14.7 unshared, 16.0 by twos).
+  if (narrow) {
+    const int64_t tiles = row_tiles * p.m_tiles;
+    p.parts = 1;
+    while (p.parts < kMostParts && tiles <= kSplitTiles && tiles * p.parts * 2 <= 4 * kSplitTiles &&
+           p.k_blocks >= (tiles * p.parts * 2 <= 2 * kSplitTiles ? 4 : 8) * p.parts * 2)
+      p.parts *= 2;
+    if (p.parts > 1) return launch<kMode, kI8, Split>(maps, p, row_tiles * p.m_tiles, num_sms, s);
+    return launch<kMode, kI8, Narrow>(maps, p, row_tiles * p.m_tiles, num_sms, s);
+  }
   return launch<kMode, kI8, Wide>(maps, p, row_tiles * p.m_tiles, num_sms, s);
 }
 

@@ -80,6 +80,8 @@ SHAPES = [
     ([40] * 300, 0, 72, 80),                              # long on average, more segments than are sorted
     ([20, 0] * 512, 7, 16, 64),                           # 1024 experts
     ([257, 513, 1025, 1793, 2049, 256, 512], 0, 264, 96),  # lengths that tiles share evenly
+    ([1], 0, 136, 4104), ([2, 0, 9], 3, 4104, 264),        # few tiles: clusters share a tile's sum
+    ([33, 0, 0, 2, 5], 4, 520, 1032), ([30], 0, 1032, 2056), ([8], 40, 264, 1000),
 ]
 
 
@@ -321,7 +323,8 @@ def _int8_ref(a, a_scale, w, w_scale, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("m,n,k", [(1, 1, 16), (1, 4096, 512), (2, 129, 64), (17, 255, 1008), (33, 640, 2048),
-                                   (300, 1001, 400), (1000, 384, 7168), (257, 128, 16)])
+                                   (300, 1001, 400), (1000, 384, 7168), (257, 128, 16), (1, 2048, 7168),
+                                   (32, 130, 4096), (20, 1000, 2064), (1, 4096, 4096), (7, 64, 1024)])
 def test_int8_mm_is_exact(m, n, k, dtype):
     a, w = _codes(m, k, seed=1), _codes(n, k, seed=2)
     sa, sw = _scales(m, seed=3), _scales(n, seed=4)
