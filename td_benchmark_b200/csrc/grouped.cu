@@ -13,9 +13,9 @@
 // tile.  Operands read across their rows are "MN-major": 64 of M or N in a 128-byte
 // swizzled row, one such row for each index of the sum.
 //
-// Persistent CTAs, one on each SM, in pairs (M = 256 over both) unless segments are short:
+// Persistent CTAs, in pairs (M = 256 over both), or single ones where segments are short:
 // warp 0 feeds a ring of TMA stages, warp 1 issues tcgen05.mma into one of two TMEM
-// accumulators, warps 4-11 turn the other one into output rows.
+// accumulators, warps 4 and following turn the other one into output rows.
 // Every sum is one fp32 (or exact int32) accumulator in TMEM from the first product to
 // the last, rounded once.
 //
@@ -38,10 +38,7 @@ enum Mode { kFwd = 0, kDx = 1, kDw = 2 };
 constexpr int kM = 128;            // output columns of a CTA's part of a tile (TMEM lanes)
 constexpr int kRowBytes = 128;     // one swizzled shared-memory row
 constexpr int kMaxExperts = 1024;
-// Warps: 0 and 2 feed the ring, 1 issues MMAs, 3 finds tiles, 4-11 write outputs, 12 clears tails (kDw).
-constexpr int threads_of(int mode) { return mode == kDw ? 416 : 384; }
 constexpr int kMostWarps = 13;
-constexpr int kEpiWarps = 8;
 constexpr int kABytes = kM * kRowBytes;
 constexpr int kBand = 8;           // row tiles walked together, so that they share a weight tile in L2
 constexpr int kSortMost = 256;     // experts up to which segments are sorted by length
@@ -56,7 +53,7 @@ constexpr int kStagePitch = 144;   // bytes between two staged output rows of 12
 // Where there are too few tiles for the SMs, the CTAs of a cluster share a tile along its sum
 // (kSplit): each multiplies its part of the blocks, and each adds up all parts for its share
 // of the output columns.
-template <int kRows, bool kTwoCtas, bool kSplitSum>
+template <int kRows, bool kTwoCtas, bool kSplitSum, int kRing, int kOnSm>
 struct Shape {
   static constexpr int NT = kRows;
   static constexpr bool kPair = kTwoCtas;
@@ -66,13 +63,18 @@ struct Shape {
   static constexpr int kBRows = NT / kCtas;         // rows of the row operand in one CTA
   static constexpr int kStep = 16 * kCtas;          // granularity of N in an MMA
   static constexpr int kStageBytes = kABytes + kBRows * kRowBytes;
-  static constexpr int kStages = kPair ? 6 : kSplit ? 4 : 9;  // split: two CTAs fit on an SM
-  static constexpr int kReaders = kSplit ? kEpiWarps / 2 : kEpiWarps;  // epilogue warps that take tiles
+  static constexpr int kStages = kRing;
+  static constexpr int kResident = kOnSm;  // CTAs on an SM
+  static constexpr int kEpiWarps = kPair ? 8 : 4;  // two sets of four, or one: 32 rows at a time each
   static constexpr uint32_t kTmemCols = 2 * NT;
 };
-using Wide = Shape<256, true, false>;
-using Narrow = Shape<32, false, false>;
-using Split = Shape<32, false, true>;
+using Wide = Shape<256, true, false, 6, 1>;
+// Two CTAs on an SM: one streams while the other starts or ends a tile, and a few rounds of
+// tiles share the memory out evenly.
+using Narrow = Shape<32, false, false, 4, 2>;
+// For one round of tiles or less: the whole SM's ring for one CTA.
+using Single = Shape<32, false, false, 9, 1>;
+using Split = Shape<32, false, true, 4, 2>;
 constexpr int kMostParts = 8;
 
 // What the CTAs of a split tile hand to each other: for every part, the accumulators of the
@@ -118,9 +120,16 @@ struct Control {
   int32_t tile0[kMaxExperts + 2];  // row tiles before the segment at place r of the walk
   uint16_t seg[kMaxExperts + 2];   // the segment at place r
   // 32 output rows of 64 columns, for two warps each
-  alignas(16) uint8_t staging[S::kSplit ? 1 : kEpiWarps / 2][S::kSplit ? 16 : 32 * kStagePitch];
+  alignas(16) uint8_t staging[S::kSplit ? 1 : S::kEpiWarps / 2][S::kSplit ? 16 : 32 * kStagePitch];
   Join<S::kSplit> join;
 };
+
+// Warps: 0 and 2 feed the ring, 1 issues MMAs, 3 finds tiles, 4 and following write outputs, the
+// last one of kDw clears tails.
+template <class S>
+constexpr int threads_of(int mode) {
+  return (4 + S::kEpiWarps + (mode == kDw ? 1 : 0)) * 32;
+}
 
 template <class S>
 constexpr size_t smem_bytes() {
@@ -329,7 +338,7 @@ __device__ __forceinline__ void plan_narrow(const Params& p, Control<S>* C, int 
 template <int kMode, class S>
 __device__ __forceinline__ void plan_wide(const Params& p, Control<S>* C) {
   constexpr int NT = S::NT;
-  constexpr int kThreads = threads_of(kMode);
+  constexpr int kThreads = threads_of<S>(kMode);
   constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rows = static_cast<int>(p.rows);
@@ -925,7 +934,7 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, uint32_
       tc_fence_after();
     }
     const int64_t base = (kMode == kDw ? r.e * p.out_expert : 0) + static_cast<int64_t>(r.row0) * p.ldo + m0;
-    for (int c = h * 32; c < r.cols && m_duo > 0; c += 64) {
+    for (int c = h * 32; c < r.cols && m_duo > 0; c += S::kEpiWarps / 4 * 32) {
       const int n = min(32, r.cols - c);
       const uint32_t taddr = tmem_base + lane_off + static_cast<uint32_t>(buf * S::NT + c);
       float a_scale = 0.0f;
@@ -1016,7 +1025,7 @@ __device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, u
 }
 
 template <int kMode, bool kI8, class S>
-__global__ void __launch_bounds__(threads_of(kMode), S::kSplit ? 2 : 1)
+__global__ void __launch_bounds__(threads_of<S>(kMode), S::kResident)
     grouped_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -1035,14 +1044,14 @@ __global__ void __launch_bounds__(threads_of(kMode), S::kSplit ? 2 : 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&C->tfull[b], 1);
-      mbar_init(&C->tempty[b], S::kCtas * S::kReaders);
+      mbar_init(&C->tempty[b], S::kCtas * S::kEpiWarps);
     }
     if constexpr (S::kSplit)  // from every part, one arrival for each run of a warp's lanes
-      mbar_init(&C->join.full, p.parts * max(1, S::kReaders / p.parts));
+      mbar_init(&C->join.full, p.parts * max(1, S::kEpiWarps / p.parts));
     // readers of a tile: producers, epilogue warps, (kDw) warp 12, and the MMA warp of the leader
     for (int s = 0; s < kFeed; ++s) {
       mbar_init(&C->fed[s], 1);
-      mbar_init(&C->taken[s], 2 + S::kReaders + (kMode == kDw ? 1 : 0) + (at.rank == 0 ? 1 : 0));
+      mbar_init(&C->taken[s], 2 + S::kEpiWarps + (kMode == kDw ? 1 : 0) + (at.rank == 0 ? 1 : 0));
     }
     mbar_init(&C->mma_done, 1);
     C->abort = 0;
@@ -1081,7 +1090,7 @@ __global__ void __launch_bounds__(threads_of(kMode), S::kSplit ? 2 : 1)
   } else if (warp == 12) {
     clear_tails<S>(p, smem, C, lane);
   } else if constexpr (S::kSplit) {
-    if (warp < 4 + S::kReaders) epilogue_split<kI8, S>(p, C, tmem_base, at, warp, lane);
+    epilogue_split<kI8, S>(p, C, tmem_base, at, warp, lane);
   } else {
     epilogue<kMode, kI8, S>(p, C, tmem_base, at.rank, warp, lane);
   }
@@ -1134,7 +1143,7 @@ struct Weights {  // [experts, n, k], strides in elements
 
 template <int kMode, bool kI8, class S>
 int launch(const Maps& maps, const Params& p, int64_t tiles_bound, int num_sms, cudaStream_t s) {
-  static_assert(smem_bytes<S>() <= 227 * 1024, "shared memory budget");
+  static_assert(S::kResident * (smem_bytes<S>() + 1024) <= 228 * 1024, "shared memory budget");
   static std::atomic<bool> attr_done[64];
   int dev = 0;
   B2M_TRY(check_cuda(cudaGetDevice(&dev), "cudaGetDevice"));
@@ -1146,13 +1155,14 @@ int launch(const Maps& maps, const Params& p, int64_t tiles_bound, int num_sms, 
     if (dev < 64) attr_done[dev].store(true, std::memory_order_release);
   }
   const int ctas = S::kSplit ? p.parts : S::kCtas;
-  const int64_t most = S::kSplit ? tiles_bound : num_sms / ctas;  // a cluster that shares a sum has one tile
+  // a cluster that shares a sum has one tile
+  const int64_t most = S::kSplit ? tiles_bound : S::kResident * num_sms / ctas;
   cudaLaunchAttribute cluster[1];
   cluster[0].id = cudaLaunchAttributeClusterDimension;
   cluster[0].val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas * (tiles_bound < most ? tiles_bound : most)));
-  cfg.blockDim = dim3(threads_of(kMode));
+  cfg.blockDim = dim3(threads_of<S>(kMode));
   cfg.dynamicSmemBytes = smem_bytes<S>();
   cfg.stream = s;
   cfg.attrs = cluster;
@@ -1223,8 +1233,8 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   p.rows = x.rows;
   p.m_dim = static_cast<int32_t>(m_dim);
   // Row tiles of 32, one CTA each, while segments are short: weights alone bound these calls,
-  // the ring then holds more of them, and twice as many CTAs share them out (E=32, 4096 x 7168,
-  // forward: 274 us narrow, 288 wide at 8 rows each).  The mean is all that the host knows of
+  // and four times as many CTAs share them out (E=32, 4096 x 7168, forward: 280 us narrow, 288
+  // wide at 8 rows each).  The mean is all that the host knows of
   // the lengths.  Under Zipf 1.2 the longest segments cost a narrow launch more than it saves from
   // 16 rows on average (299 narrow, 292 wide; 377 and 311 at 32), and not yet at 12 (278, 292).
   // One segment alone has the length that the host sees: up to one narrow tile.
@@ -1281,8 +1291,11 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
     while (p.parts < kMostParts && tiles <= kSplitTiles && tiles * p.parts * 2 <= 4 * kSplitTiles &&
            p.k_blocks >= (tiles * p.parts * 2 <= 2 * kSplitTiles ? 4 : 8) * p.parts * 2)
       p.parts *= 2;
-    if (p.parts > 1) return launch<kMode, kI8, Split>(maps, p, row_tiles * p.m_tiles, num_sms, s);
-    return launch<kMode, kI8, Narrow>(maps, p, row_tiles * p.m_tiles, num_sms, s);
+    if (p.parts > 1) return launch<kMode, kI8, Split>(maps, p, tiles, num_sms, s);
+    // E=128, eight rows, 1536 x 2048 (96 tiles): 14.2 us single, 15.7 two on an SM; integers,
+    // 28672 x 4096 (224): 24.9 and 23.3; E=8, two rows, 28672 x 4096 (448): 84 and 77.5.
+    if (tiles <= num_sms) return launch<kMode, kI8, Single>(maps, p, tiles, num_sms, s);
+    return launch<kMode, kI8, Narrow>(maps, p, tiles, num_sms, s);
   }
   return launch<kMode, kI8, Wide>(maps, p, row_tiles * p.m_tiles, num_sms, s);
 }
