@@ -174,16 +174,15 @@ __device__ __forceinline__ void store_codes(int8_t* __restrict__ q, int64_t cols
 // Largest value of the group's partial maxima, in every thread of it.  `part`: one value for
 // each warp of the block, of two sets used in turn.  False in all threads when `ok` is in one.
 __device__ __forceinline__ bool group_max(float& amax, float* part, int group, bool ok) {
+  // bits of values that are not negative order as the values do, with NaN above infinity
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  if (lane == 0) part[threadIdx.x >> 5] = amax;
+  uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(amax));
+  if (lane == 0) part[threadIdx.x >> 5] = __uint_as_float(most);
   ok = __syncthreads_and(ok);
-  if (group > 32) {
-    amax = part[((threadIdx.x & ~(group - 1)) >> 5) + (lane & (group / 32 - 1))];
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-  }
+  if (group > 32)
+    most = __reduce_max_sync(
+        0xffffffffu, __float_as_uint(part[((threadIdx.x & ~(group - 1)) >> 5) + (lane & (group / 32 - 1))]));
+  amax = __uint_as_float(most);
   return ok;
 }
 
