@@ -601,12 +601,15 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
   const uint32_t full0 = smem_u32(&C->full[0]), landed0 = smem_u32(&C->landed[0]);
   const uint32_t full0_leader = S::kPair ? mapa_shared(full0, 0) : full0;
   const uint32_t landed0_own = S::kPair ? mapa_shared(landed0, rank) : landed0;
-  uint32_t kg = 0;  // stages of the tiles before this one
+  uint32_t kg = 0;      // stages of the tiles before this one
+  uint32_t issued = 0;  // one more than the last stage that this warp issued
+  uint32_t tails = 0, last_tail = 0;  // bit s: parity of the next use of landed[s]; the last use of stage s was one
   bool alive = true;
   TileFeed<S> feed(p, C);
   Tile r;
   while (alive) {
-    if (!feed.next(r) || r.e < 0) break;
+    alive = feed.next(r);
+    if (!alive || r.e < 0) break;
     const int half = mma_cols<S>(r.cols) / S::kCtas;  // rows of the row operand in this CTA
     // One box of the row operand for each stage, of the smallest size that holds the tile's rows:
     // as many 32-row boxes as it needs took longer to issue than the rows that they leave out
@@ -652,15 +655,31 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
         }
       }
       __syncwarp();
+      issued = kg + kb + 1;
+      if (kMode == kDw) {
+        last_tail = tail ? last_tail | 1u << s : last_tail & ~(1u << s);
+        if (tail) tails ^= 1u << s;
+      }
       if ((s += 2) >= S::kStages) s -= S::kStages, phase ^= 1;
     }
     kg += r.k_blocks;
   }
-  // The stages still in use are released before the CTA exits: their copies have then landed
-  // (after a timeout elsewhere, when nothing releases them, the wait ends by its limit).
-  const uint32_t first = kg > S::kStages ? kg - S::kStages : 0;
-  for (uint32_t i = first; i < kg && alive; ++i)
-    alive = wait_warp(&C->empty[i % S::kStages], (i / S::kStages) & 1, p, B2M_STATUS_TIMEOUT_DRAIN, &C->abort);
+  // Before the CTA exits, the copies of the stages still in use have landed: they are when the
+  // stage is released.  After a timeout nothing may release it; then this warp waits, again
+  // within the limit, for its last copies themselves (of a pair, the leader for both CTAs').
+  const uint32_t first = issued > S::kStages ? issued - S::kStages : 0;
+  for (uint32_t i = first; i < issued && alive; ++i)
+    if (((i ^ which) & 1) == 0)
+      alive = wait_warp(&C->empty[i % S::kStages], (i / S::kStages) & 1, p, B2M_STATUS_TIMEOUT_DRAIN, &C->abort);
+  for (uint32_t i = first; i < issued && !alive; ++i) {
+    const uint32_t s = i % S::kStages;
+    if (((i ^ which) & 1) != 0) continue;
+    if (kMode == kDw && (last_tail >> s & 1))
+      wait_on(&C->landed[s], (tails >> s & 1) ^ 1, p, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
+    else if (rank == 0)
+      wait_on(&C->full[s], (i / S::kStages) & 1, p, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
+  }
+  __syncwarp();
 }
 
 // Warp 12 of kDw: when this CTA's copies of a segment's last, partly filled stage have landed,

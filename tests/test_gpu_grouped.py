@@ -499,3 +499,121 @@ def test_results_do_not_change_from_run_to_run():
     for _ in range(5):
         for a, b in zip(first, run()):
             assert torch.equal(a, b)
+
+
+def test_two_graphs_replayed_at_once():
+    """Captured calls hold no workspace that another graph could share."""
+    sets = []
+    for seed, counts in ((1, [30, 0, 300, 70]), (2, [1, 1, 0, 6])):
+        rows = sum(counts)
+        sets.append((_randn(rows, 512, seed=seed), _randn(4, 640, 512, seed=seed + 10), _ends(counts),
+                     _randn(rows, 640, seed=seed + 20)))
+    run = lambda x, w, ends, dy: (ops.grouped_mm(x, w, ends), ops.grouped_mm_dx(dy, w, ends),  # noqa: E731
+                                  ops.grouped_mm_dw(dy, x, ends), *ops.quant_int8(x))
+    want = [run(*s) for s in sets]
+    graphs, held, streams = [], [], [torch.cuda.Stream(DEV) for _ in sets]
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(run(*s))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for h, w in zip(held, want):
+        assert all(torch.equal(a, b) for a, b in zip(h, w))
+
+
+def test_captured_training_step():
+    """Forward and backward of leaves that no eager graph holds, captured and replayed with other values."""
+    counts = [20, 0, 44]
+    x, w, dy = _randn(64, 96, seed=1).requires_grad_(), _randn(3, 80, 96, seed=2).requires_grad_(), _randn(64, 80, seed=3)
+    ends = _ends(counts)
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.grouped_mm(x, w, ends), (x, w), dy)      # its graph is gone before the capture
+    torch.cuda.current_stream(DEV).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gx, gw = torch.autograd.grad(ops.grouped_mm(x, w, ends), (x, w), dy)
+    with torch.no_grad():
+        x.copy_(_randn(64, 96, seed=11))
+        w.copy_(_randn(3, 80, 96, seed=12))
+    graph.replay()
+    torch.cuda.synchronize()
+    xd, wd = x.detach(), w.detach()
+    _close(gx, _dx(dy, wd, counts), _dx(dy.abs(), wd.abs(), counts), 80)
+    _close(gw, _dw(dy, xd, counts), _dw(dy.abs(), xd.abs(), counts), 44)
+
+
+def test_another_current_device(monkeypatch):
+    """With another device current, the call switches to the tensors' one (here: told that another one is)."""
+    x, w, ends = _randn(6, 64, seed=1), _randn(2, 48, 64, seed=2), _ends([4, 2])
+    want = ops.grouped_mm(x, w, ends)
+    switched = []
+    device = torch.cuda.device
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 7)
+    monkeypatch.setattr(torch.cuda, "device", lambda i: switched.append(i) or device(i))
+    got = ops.grouped_mm(x, w, ends)
+    monkeypatch.undo()
+    assert switched == [0] and torch.equal(got, want)
+
+
+def test_refusals_of_the_wrappers():
+    x, w, ends = _randn(8, 64, seed=1), _randn(2, 32, 64, seed=2), _ends([5, 3])
+    dy = _randn(8, 32, seed=3)
+    bad = [
+        (lambda: ops.grouped_mm(x.float(), w, ends), "bf16 or fp16"),
+        (lambda: ops.grouped_mm(x.half(), w, ends), "w must be"),
+        (lambda: ops.grouped_mm(x, w[:, :, :32], ends), "summed axes"),
+        (lambda: ops.grouped_mm(x[0], w, ends), "x must be"),
+        (lambda: ops.grouped_mm(x.t(), w, ends), "x must be"),
+        (lambda: ops.grouped_mm(x, w, ends.long()), "ends must be"),
+        (lambda: ops.grouped_mm(x, w, ends[:1]), "ends must be"),
+        (lambda: ops.grouped_mm(x, w, ends.cpu()), "ends must be"),
+        (lambda: ops.grouped_mm(x, w, ends, out_dtype=torch.float16), "out_dtype"),
+        (lambda: ops.grouped_mm(x, w, ends, out=torch.empty((8, 31), device=DEV, dtype=x.dtype)), "out must be"),
+        (lambda: ops.grouped_mm(x, w, ends, out=x[:, :32]), "overlaps"),
+        (lambda: ops.grouped_mm(x, w, ends, status=torch.zeros(1, device=DEV)), "status"),
+        (lambda: ops.grouped_mm(x.requires_grad_(), w, ends, out=dy), "gradients"),
+        (lambda: ops.grouped_mm_dx(dy, w.transpose(1, 2), ends), "w must be"),
+        (lambda: ops.grouped_mm_dw(dy, x.detach()[:7], ends), "rows"),
+        (lambda: ops.grouped_mm_dw(dy, x.detach().half(), ends), "x must be"),
+        (lambda: ops.grouped_mm_dw(dy, x.detach(), ends[None]), "ends must be"),
+        (lambda: ops.quant_int8(x.detach().double()), "2D"),
+        (lambda: ops.quant_int8(x.detach().t()), "2D"),
+        (lambda: ops.quant_int8(x.detach(), q=torch.empty((8, 63), dtype=torch.int8, device=DEV)), "bad q"),
+        (lambda: ops.quant_int8(x.detach(), scale=torch.empty(7, device=DEV)), "scale must be"),
+    ]
+    a, s = ops.quant_int8(x.detach())
+    wq, sw = ops.quant_int8(w.view(-1, 64))
+    bad += [
+        (lambda: ops.int8_mm(a, s, wq[:, :32], sw), "summed axes"),
+        (lambda: ops.int8_mm(a, s[:7], wq, sw), "a_scale"),
+        (lambda: ops.int8_mm(a, s, wq, sw[:5]), "w_scale"),
+        (lambda: ops.int8_mm(a, s.double(), wq, sw), "a_scale"),
+        (lambda: ops.int8_mm(a.float(), s, wq, sw), "a must be"),
+        (lambda: ops.int8_mm(a, s, wq, sw, out_dtype=torch.int32), "out_dtype"),
+        (lambda: ops.int8_grouped_mm(a, s, wq.view(2, 32, 64), sw, ends), "w_scale"),
+        (lambda: ops.int8_grouped_mm(a, s, wq, sw.view(2, 32), ends), "w must be"),
+    ]
+    for call, match in bad:
+        with pytest.raises(ValueError, match=match):
+            call()
+    for call in (lambda: ops.grouped_mm(x.detach().expand(8, 64)[:, 1:61], w[:, :, 1:61], ends),   # unaligned rows
+                 lambda: ops.grouped_mm(_randn(1, 64).expand(8, 64), w, ends),                     # rows on one another
+                 lambda: ops.grouped_mm(x.detach(), _randn(1, 32, 64).expand(2, 32, 64), ends),
+                 lambda: ops.int8_mm(a[:, :24].contiguous(), s, wq[:, :24].contiguous(), sw)):
+        with pytest.raises(Exception, match="16 bytes|16-byte"):
+            call()
+
+
+def test_one_double_backward_is_refused():
+    x, w = _randn(4, 64, seed=1).requires_grad_(), _randn(1, 32, 64, seed=2).requires_grad_()
+    y = ops.grouped_mm(x, w, _ends([4]))
+    (gx,) = torch.autograd.grad(y, x, torch.ones_like(y), create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gx.sum(), w)
