@@ -156,6 +156,7 @@ struct Params {
   int64_t rows;
   int32_t m_dim;         // extent of the output's contiguous axis
   int32_t m_tiles;       // tiles along it
+  int32_t tile_bits;     // log2 of a tile's most output rows
   int32_t c_dim;         // kDw: output rows of one expert
   int32_t c_tiles;       // kDw
   int32_t k_blocks;      // kFwd, kDx: blocks of the sum
@@ -227,16 +228,17 @@ __device__ __forceinline__ Tile tile_at(const Params& p, const Control<S>* C, in
   }
   r.m0 = m * S::kTileM;
   if (kMode == kDw) {
-    r.row0 = c * S::NT;
-    r.cols = min(S::NT, p.c_dim - c * S::NT);
+    r.row0 = c << p.tile_bits;
+    r.cols = min(1 << p.tile_bits, p.c_dim - r.row0);
     r.sum0 = C->start[r.e];
     r.sum_rows = C->start[r.e + 1] - C->start[r.e];
     r.k_blocks = (r.sum_rows + 63) >> 6;
   } else {
     // A segment's tiles have about the same rows: one of few rows costs four fifths of a full
     // one (258 rows: 256 and 2 take 912 cycles a block of the sum, twice 129 take 800).  Sizes
-    // are whole steps of an MMA; with eight tiles and more they come to NT, and the last of
-    // fewer tiles keeps a row (more than 256 (n - 1) rows in n < 8 tiles of at most rows / n + 31).
+    // are whole steps of an MMA; with eight tiles and more they come to the most that a tile has,
+    // and the last of fewer tiles keeps a row (256: more than 256 (n - 1) rows in n < 8 tiles of at
+    // most rows / n + 31; 128: of 96 or 128; 64: of 64).
     const int rows = C->start[r.e + 1] - C->start[r.e];
     const int each = S::kPair && tiles > 1 ? mma_cols<S>((rows + tiles - 1) / tiles) : S::NT;
     r.row0 = C->start[r.e] + c * each;
@@ -337,7 +339,7 @@ __device__ __forceinline__ void plan_narrow(const Params& p, Control<S>* C, int 
 // Wide launches: by all threads, longest segments first in the walk.
 template <int kMode, class S>
 __device__ __forceinline__ void plan_wide(const Params& p, Control<S>* C) {
-  constexpr int NT = S::NT;
+  const int nt = 1 << p.tile_bits;
   constexpr int kThreads = threads_of<S>(kMode);
   constexpr int kPer = (kMaxExperts + kThreads - 1) / kThreads;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -377,7 +379,7 @@ __device__ __forceinline__ void plan_wide(const Params& p, Control<S>* C) {
     const int end = max(v[i], prev);
     if (e < p.experts) C->start[e] = prev;
     if (e == p.experts - 1) C->start[p.experts] = end;
-    n[i] = e < p.experts ? (end - prev + NT - 1) / NT : 0;
+    n[i] = e < p.experts ? (end - prev + nt - 1) >> p.tile_bits : 0;
     prev = end;
   }
   if (tid == 0) C->start[p.experts + 1] = rows;
@@ -398,7 +400,7 @@ __device__ __forceinline__ void plan_wide(const Params& p, Control<S>* C) {
     for (int i = 0; i < kPer; ++i) {
       const int r = tid * kPer + i;
       const int e = r < p.experts ? C->seg[r] : 0;
-      n[i] = r < p.experts ? (C->start[e + 1] - C->start[e] + NT - 1) / NT : 0;
+      n[i] = r < p.experts ? (C->start[e + 1] - C->start[e] + nt - 1) >> p.tile_bits : 0;
     }
   } else {
 #pragma unroll
@@ -431,7 +433,7 @@ __device__ __forceinline__ void plan_wide(const Params& p, Control<S>* C) {
   if (tid == 0) {
     C->tile0[p.experts] = total;
     // the rows behind the last segment, as one more segment
-    C->tile0[p.experts + 1] = total + (rows - C->start[p.experts] + NT - 1) / NT;
+    C->tile0[p.experts + 1] = total + ((rows - C->start[p.experts] + nt - 1) >> p.tile_bits);
   }
 }
 
@@ -838,35 +840,30 @@ struct Duo {
   }
 };
 
-// The first n of eight 16-bit values, one by one.
-__device__ __noinline__ void store_edge(uint16_t* d, uint4 u, int n) {
-  const uint32_t h[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < n) d[k] = static_cast<uint16_t>(h[k / 2] >> (16 * (k & 1)));
-}
-
 // 64 output columns (TMEM lanes of two warps) of 32 output rows (TMEM columns), rounded to 16
 // bits.  An output row is contiguous along the lanes, so the block is transposed on its way
 // out: pairs of rows in a register, 8x8 matrices through stmatrix into the staging block, and
 // from there whole 128-byte lines, four in a warp's store.  (The weight gradient of E=32,
 // 4096 x 7168 took 1.08 ms with two-byte stores straight from the registers and 0.66 ms with
-// half lines, both bound by the L1's stores.)
+// half lines, both bound by the L1's stores.)  Lines that do not start on 16 bytes, or end
+// inside 16, go out as pairs of elements, a line in a warp's store, four lines read before the
+// first is written: bf16, 3855 x 4745, a sum of 240, 32 us, 58 line by line and 90 with 16 bytes
+// by single elements in each thread; 20 at 4744.
+// `v` holds the block's accumulators, or will when the loads in flight are done, and then takes
+// the next block's from `next` (0: there is none) while this one is written: the weight gradient
+// above takes 600 us, 635 with the loads at the start of the block.
 // `o`: the block's first element; n rows and m columns of it exist.
 template <bool kI8>
 __device__ __forceinline__ void emit_16bit(uint16_t* o, int64_t ldo, int n, int m, bool wide, bool bf16, bool zero,
-                                           uint32_t taddr, uint8_t* staging, const Duo& duo, float a_scale,
-                                           const float (&w_scale)[4], int lane) {
-  float v[32];
-  if (!zero) {
-    tmem_ld_16x32(taddr, v);
-    tmem_ld_16x32(taddr + (16u << 16), v + 16);
-    tmem_ld_wait();
-  }
+                                           uint32_t next, uint8_t* staging, const Duo& duo, float a_scale,
+                                           const float (&w_scale)[4], int lane, float (&v)[32]) {
+  if (!zero) tmem_ld_wait();
+  uint32_t packed[4][4];
   const uint32_t to = smem_u32(staging) + (lane & 7) * kStagePitch + duo.half * 64 + (lane >> 3) * 16;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    uint32_t w[4] = {0, 0, 0, 0};
+    uint32_t(&w)[4] = packed[g];
+    w[0] = w[1] = w[2] = w[3] = 0;
     float s0 = 1.0f, s1 = 1.0f;
     if (kI8) {
       s0 = __shfl_sync(0xffffffffu, a_scale, 8 * g + 2 * (lane & 3));
@@ -883,20 +880,45 @@ __device__ __forceinline__ void emit_16bit(uint16_t* o, int64_t ldo, int n, int 
         w[i] = pack_16bit(x, y, bf16);
       }
     }
-    store_matrices_t(to + 8 * g * kStagePitch, w);
   }
-  duo.sync();
-  const int at = (lane & 7) * 8;  // this thread's eight columns
+  if (next) {
+    tmem_ld_16x32(next, v);
+    tmem_ld_16x32(next + (16u << 16), v + 16);
+  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = 16 * duo.half + 4 * i + (lane >> 3);
-    if (j < n && at < m) {
-      const uint4 u = *reinterpret_cast<const uint4*>(staging + j * kStagePitch + at * 2);
-      uint16_t* d = o + j * ldo + at;
-      if (wide && at + 8 <= m)
-        *reinterpret_cast<uint4*>(d) = u;
-      else
-        store_edge(d, u, m - at);
+  for (int g = 0; g < 4; ++g) store_matrices_t(to + 8 * g * kStagePitch, packed[g]);
+  duo.sync();
+  constexpr int kAtOnce = 4;  // rows
+  if (wide && (m & 7) == 0) {
+    const int at = (lane & 7) * 8;  // this thread's eight columns
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = 16 * duo.half + 4 * i + (lane >> 3);
+      if (j < n && at < m)
+        *reinterpret_cast<uint4*>(o + j * ldo + at) = *reinterpret_cast<const uint4*>(staging + j * kStagePitch + at * 2);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; i += kAtOnce) {
+      // a row that starts between two words: its first element alone, then pairs from the second on
+      const int j0 = 16 * duo.half + i;
+      uint32_t pair[kAtOnce], first[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(staging + (j0 + k) * kStagePitch);
+        const int at = 2 * lane + (static_cast<int>(reinterpret_cast<uintptr_t>(o + (j0 + k) * ldo) >> 1) & 1);
+        first[k] = from[0];
+        pair[k] = from[at] | static_cast<uint32_t>(from[at + 1]) << 16;
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        uint16_t* d = o + (j0 + k) * ldo;
+        const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(d) >> 1) & 1, at = 2 * lane + odd;
+        const bool exists = j0 + k < n;
+        if (exists && at + 1 < m) *reinterpret_cast<uint32_t*>(d + at) = pair[k];
+        if (exists && at + 1 == m) d[at] = static_cast<uint16_t>(pair[k]);
+        if (exists && odd && lane == 0) d[0] = static_cast<uint16_t>(first[k]);
+      }
     }
   }
   duo.sync();
@@ -947,23 +969,34 @@ __device__ __forceinline__ void epilogue(const Params& p, Control<S>* C, uint32_
 #pragma unroll
       for (int i = 0; i < 4; ++i) w_scale[i] = __shfl_sync(0xffffffffu, w_lane, 8 * i + (lane >> 2));
     }
+    // the scales of a block's rows are on their way while the block before them is written
+    float a_next = 0.0f;
+    if (kI8 && !zero && h * 32 + lane < r.cols) a_next = __ldg(p.a_scale + r.row0 + h * 32 + lane);
     if (!zero) {
       const bool ok = wait_warp(&C->tfull[buf], (used >> 1) & 1, p, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort);
       if (!duo.both(ok)) return;
       tc_fence_after();
     }
     const int64_t base = (kMode == kDw ? r.e * p.out_expert : 0) + static_cast<int64_t>(r.row0) * p.ldo + m0;
-    for (int c = h * 32; c < r.cols && m_duo > 0; c += S::kEpiWarps / 4 * 32) {
+    constexpr int kEvery = S::kEpiWarps / 4 * 32;
+    float v[32];
+    if (!zero && p.out_type != B2M_FP32 && h * 32 < r.cols && m_duo > 0) {
+      const uint32_t taddr = tmem_base + lane_off + static_cast<uint32_t>(buf * S::NT + h * 32);
+      tmem_ld_16x32(taddr, v);
+      tmem_ld_16x32(taddr + (16u << 16), v + 16);
+    }
+    for (int c = h * 32; c < r.cols && m_duo > 0; c += kEvery) {
       const int n = min(32, r.cols - c);
       const uint32_t taddr = tmem_base + lane_off + static_cast<uint32_t>(buf * S::NT + c);
-      float a_scale = 0.0f;
-      if (kI8 && !zero && lane < n) a_scale = __ldg(p.a_scale + r.row0 + c + lane);
+      const float a_scale = a_next;
+      if (kI8 && !zero && c + kEvery + lane < r.cols) a_next = __ldg(p.a_scale + r.row0 + c + kEvery + lane);
       const int64_t o = base + c * p.ldo;
       if (p.out_type == B2M_FP32)
         emit_fp32<kI8>(static_cast<float*>(p.out) + o, p.ldo, n, m, zero, taddr, a_scale, w_lane, lane);
       else
         emit_16bit<kI8>(static_cast<uint16_t*>(p.out) + o - duo.half * 32, p.ldo, n, m_duo, p.wide_out,
-                        p.out_type == B2M_BF16, zero, taddr, staging, duo, a_scale, w_scale, lane);
+                        p.out_type == B2M_BF16, zero, !zero && c + kEvery < r.cols ? taddr + kEvery : 0u, staging, duo,
+                        a_scale, w_scale, lane, v);
     }
     if (!zero) {
       tc_fence_before();
@@ -1194,6 +1227,25 @@ constexpr int64_t kMaxTiles = int64_t(1) << 30;
 
 uint32_t magic(int64_t d) { return static_cast<uint32_t>(((uint64_t(1) << 32) + d - 1) / d); }
 
+// Output rows of a wide tile at most: 256, and half or a quarter of it while the tiles, of which
+// there are tiles_of(rows) or fewer, still are no more than the pairs.  A tile of fewer rows
+// reads the other operand as often and takes more than its share of the time, but pairs
+// without a tile take it all: bf16, 1024 x 1024 x 1024, 12.6 us by 256, 9.2 by 64; 4096 x 256, a sum of
+// 7168, 39 and 25; its weight gradient, a sum of 4096, 26 and 21.  (Tiles of 32 gave no more
+// than 0.1 us.)
+template <class F>
+int64_t rows_of_tile(int num_sms, const F& tiles_of) {
+  int64_t n = Wide::NT;
+  while (n > Wide::NT / 4 && tiles_of(n / 2) <= num_sms / 2) n /= 2;
+  return n;
+}
+
+int32_t bits_of(int64_t n) {
+  int32_t b = 0;
+  while (n >> (b + 1)) ++b;
+  return b;
+}
+
 // Limit of a wait inside a CTA's pipeline, where nothing but the CTA's own work is waited for: a
 // sum of `blocks` blocks takes a third of a microsecond for each, and a role may wait for
 // several tiles.
@@ -1258,7 +1310,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   // 16 rows on average (299 narrow, 292 wide; 377 and 311 at 32), and not yet at 12 (278, 292).
   // One segment alone has the length that the host sees: up to one narrow tile.
   const bool narrow = x.rows <= (w.experts == 1 ? Narrow::NT : 12 * w.experts);
-  const int64_t nt = narrow ? Narrow::NT : Wide::NT, tile_m = narrow ? Narrow::kTileM : Wide::kTileM;
+  const int64_t tile_m = narrow ? Narrow::kTileM : Wide::kTileM;
   p.m_tiles = static_cast<int32_t>((m_dim + tile_m - 1) / tile_m);
   p.k_blocks = static_cast<int32_t>((sum + in_row - 1) / in_row);
   p.m_magic = magic(p.m_tiles);
@@ -1283,10 +1335,14 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
   // most row tiles that x.rows rows can take: one not full for each segment that has rows
   const int64_t with_rows = x.rows < p.segments ? x.rows : p.segments;
-  const int64_t row_tiles = (x.rows + (nt - 1) * with_rows) / nt;
-  if (row_tiles * p.m_tiles > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
+  int64_t nt = narrow ? Narrow::NT : Wide::NT;
+  const auto most_tiles = [&](int64_t n) { return (x.rows + (n - 1) * with_rows) / n; };
+  if (most_tiles(nt) * p.m_tiles > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
   int num_sms = 0;
   B2M_TRY(device_ready(&num_sms));
+  if (!narrow) nt = rows_of_tile(num_sms, [&](int64_t n) { return most_tiles(n) * p.m_tiles; });
+  const int64_t row_tiles = most_tiles(nt);
+  p.tile_bits = bits_of(nt);
   if (x.rows == 0) return B2M_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   Maps maps{};
@@ -1380,9 +1436,7 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   p.m_dim = static_cast<int32_t>(k);
   p.m_tiles = static_cast<int32_t>((k + Wide::kTileM - 1) / Wide::kTileM);
   p.c_dim = static_cast<int32_t>(n);
-  p.c_tiles = static_cast<int32_t>((n + Wide::NT - 1) / Wide::NT);
   p.band_magic = magic(int64_t(kBand) * p.m_tiles);
-  p.expert_magic = magic(int64_t(p.m_tiles) * p.c_tiles);
   p.out = out;
   p.ldo = ldo;
   p.out_expert = out_stride;
@@ -1392,10 +1446,14 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   p.timeout_ns = wait_limit(rows / 64);
   p.idesc = (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) |
             (static_cast<uint32_t>(Wide::kTileM >> 4) << 24);
-  const int64_t tiles = int64_t(p.m_tiles) * p.c_tiles * experts;
-  if (tiles > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
+  const auto tiles_of = [&](int64_t rows) { return (n + rows - 1) / rows * p.m_tiles * experts; };
+  if (tiles_of(Wide::NT) > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
   int num_sms = 0;
   B2M_TRY(device_ready(&num_sms));
+  const int64_t nt = rows_of_tile(num_sms, tiles_of), tiles = tiles_of(nt);
+  p.tile_bits = bits_of(nt);
+  p.c_tiles = static_cast<int32_t>((n + nt - 1) / nt);
+  p.expert_magic = magic(int64_t(p.m_tiles) * p.c_tiles);
   const CUtensorMapDataType type =
       in_type == B2M_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   // Without rows every segment is empty: nothing is loaded, and a map of no rows cannot be made.

@@ -160,6 +160,43 @@ def test_given_output_keeps_rows_of_no_expert_and_columns_beside_it():
     assert (big[:, :, k:] == 7).all() and not (big[:, :, :k] == 7).any()
 
 
+@pytest.mark.parametrize("offset", [0, 1, 2, 3, 5])
+@pytest.mark.parametrize("cols,pitch", [(1, 1), (2, 3), (63, 72), (64, 65), (66, 80), (201, 201), (130, 134), (257, 300), (1713, 1713)])
+def test_outputs_that_start_anywhere(cols, pitch, offset):
+    """Output rows at any element and pitch, and nothing beside them written: 16-bit, fp32 and weight gradients."""
+    counts, k = [37, 0, 300, 1], 72
+    rows, wide = sum(counts), (cols + 7) // 8 * 8
+    x, w, ends = _randn(rows, k), _randn(4, cols, k, seed=1), _ends(counts)
+    dy = _randn(rows, wide, seed=2)[:, :cols]
+    want, mass = _fwd(x, w, counts), _fwd(x.abs(), w.abs(), counts)
+    for dtype in (torch.bfloat16, torch.float32):
+        flat = torch.full((offset + rows * pitch + 8,), -7.0, device=DEV, dtype=dtype)
+        out = flat.as_strided((rows, cols), (pitch, 1), offset)
+        ops.grouped_mm(x, w, ends, out=out)
+        _close(out, want, mass, k)
+        out.fill_(-7.0)
+        assert (flat == -7.0).all()
+    flat = torch.full((offset + 4 * k * pitch + 8,), -7.0, device=DEV, dtype=torch.bfloat16)
+    out = flat.as_strided((4, k, cols), (k * pitch, pitch, 1), offset)
+    ops.grouped_mm_dw(x, dy, ends, out=out)
+    _close(out, _dw(x, dy, counts), _dw(x.abs(), dy.abs(), counts), 300)
+    out.fill_(-7.0)
+    assert (flat == -7.0).all()
+
+
+@pytest.mark.parametrize("counts", [[63], [64], [65], [129], [191], [193], [257], [385], [1000], [129, 0, 65], [40, 300, 2],
+                                    [2100], [5000]])
+@pytest.mark.parametrize("n,k", [(40, 264), (264, 40), (300, 136)])
+def test_few_tiles(counts, n, k):
+    """Calls of few tiles, whose tiles have fewer rows: one tile and one more or one less than full ones."""
+    rows = sum(counts)
+    x, w, ends = _randn(rows, k), _randn(len(counts), n, k, seed=1), _ends(counts)
+    dy = _randn(rows, (n + 7) // 8 * 8, seed=2)[:, :n]
+    _close(ops.grouped_mm(x, w, ends), _fwd(x, w, counts), _fwd(x.abs(), w.abs(), counts), k)
+    _close(ops.grouped_mm_dx(dy, w, ends), _dx(dy, w, counts), _dx(dy.abs(), w.abs(), counts), n)
+    _close(ops.grouped_mm_dw(dy, x, ends), _dw(dy, x, counts), _dw(dy.abs(), x.abs(), counts), max(counts))
+
+
 def test_no_rows():
     w, ends = _randn(3, 64, 32, seed=1), _ends([0, 0, 0])
     x, dy = _randn(0, 32), _randn(0, 64)
@@ -331,6 +368,18 @@ def test_int8_mm_is_exact(m, n, k, dtype):
     y = ops.int8_mm(a, sa, w, sw, out_dtype=dtype)
     torch.cuda.synchronize()
     assert torch.equal(y, _int8_ref(a, sa, w, sw, dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n,pitch,offset", [(600, 201, 203, 1), (70, 1714, 1714, 0), (300, 66, 72, 0), (129, 65, 65, 3), (5, 33, 35, 1)])
+def test_int8_outputs_that_start_anywhere(m, n, pitch, offset, dtype):
+    a, a_scale, w, w_scale = _codes(m, 80, seed=1), _scales(m, seed=2), _codes(n, 80, seed=3), _scales(n, seed=4)
+    flat = torch.full((offset + m * pitch + 8,), -7.0, device=DEV, dtype=dtype)
+    out = flat.as_strided((m, n), (pitch, 1), offset)
+    ops.int8_mm(a, a_scale, w, w_scale, out=out)
+    assert torch.equal(out, _int8_ref(a, a_scale, w, w_scale, dtype))
+    out.fill_(-7.0)
+    assert (flat == -7.0).all()
 
 
 def test_int8_sums_at_the_edge_of_32_bits():
