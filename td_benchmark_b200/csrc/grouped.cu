@@ -1040,6 +1040,11 @@ __device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, u
       for (int j = 0; j < r.cols; ++j) put(p.out, out + j * p.ldo + column, p.out_type, 0.0f);
     return;
   }
+  // A thread adds up one column of every 128 / share rows.
+  const int mine = at.part * share + in_share;
+  float a_lane = 0.0f, w_scale = 0.0f;  // a_lane: of row `lane`
+  if (kI8 && lane < r.cols) a_lane = __ldg(p.a_scale + r.row0 + lane);
+  if (kI8 && r.m0 + mine < p.m_dim) w_scale = __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + r.m0 + mine);
   if (!wait_warp(&C->tfull[0], 0, p, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort)) return;
   tc_fence_after();
   float v[32];
@@ -1058,21 +1063,27 @@ __device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, u
 
   const bool ok = mbar_wait_cluster(&C->join.full, 0, p.timeout_ns, p.status, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort);
   if (!ok) return;
-  for (int i = column; i < r.cols << bits; i += kM) {
-    const int j = i >> bits, c = at.part * share + (i & (share - 1));
-    if (r.m0 + c >= p.m_dim) continue;
-    const uint32_t* part = &C->join.part[i];
-    float sum;
-    if (kI8) {
-      int acc = 0;
-      for (int k = 0; k < p.parts; ++k) acc += static_cast<int>(part[k * S::NT * share]);
-      sum = __int2float_rn(acc) * __ldg(p.a_scale + r.row0 + j) *
-            __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + r.m0 + c);
-    } else {
-      sum = __uint_as_float(part[0]);
-      for (int k = 1; k < p.parts; ++k) sum += __uint_as_float(part[k * S::NT * share]);
+  __syncwarp();
+  // four rows at a time: one by one, a thread's 16 rows of two parts took 3 us
+  constexpr int kAtOnce = 4;
+  for (int i0 = column; i0 - lane < r.cols << bits; i0 += kAtOnce * kM) {
+    uint32_t sum[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) sum[u] = (i0 + u * kM) >> bits < r.cols ? C->join.part[i0 + u * kM] : 0;
+    for (int k = 1; k < p.parts; ++k)
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if ((i0 + u * kM) >> bits >= r.cols) continue;
+        const uint32_t add = C->join.part[k * S::NT * share + i0 + u * kM];
+        sum[u] = kI8 ? sum[u] + add : __float_as_uint(__uint_as_float(sum[u]) + __uint_as_float(add));
+      }
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int j = (i0 + u * kM) >> bits;
+      float y = __uint_as_float(sum[u]);
+      if (kI8) y = __int2float_rn(static_cast<int>(sum[u])) * __shfl_sync(0xffffffffu, a_lane, j & 31) * w_scale;
+      if (j < r.cols && r.m0 + mine < p.m_dim) put(p.out, out + j * p.ldo + mine, p.out_type, y);
     }
-    put(p.out, out + j * p.ldo + c, p.out_type, sum);
   }
 }
 
@@ -1308,8 +1319,14 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   // wide at 8 rows each).  The mean is all that the host knows of
   // the lengths.  Under Zipf 1.2 the longest segments cost a narrow launch more than it saves from
   // 16 rows on average (299 narrow, 292 wide; 377 and 311 at 32), and not yet at 12 (278, 292).
-  // One segment alone has the length that the host sees: up to one narrow tile.
-  const bool narrow = x.rows <= (w.experts == 1 ? Narrow::NT : 12 * w.experts);
+  // One segment alone has the length that the host sees: up to one narrow tile.  And narrow
+  // whenever that makes so few tiles that clusters can share them out: bf16, one segment of 96 rows,
+  // 2048 x 7168 (64 tiles at most), 26.8 us wide, 16.7 narrow.
+  // Most row tiles of n that x.rows rows can take: one not full for each segment that has rows.
+  const int64_t with_rows = x.rows < p.segments ? x.rows : p.segments;
+  const auto most_tiles = [&](int64_t n) { return (x.rows + (n - 1) * with_rows) / n; };
+  const bool narrow = x.rows <= (w.experts == 1 ? Narrow::NT : 12 * w.experts) ||
+                      most_tiles(Narrow::NT) * ((m_dim + Narrow::kTileM - 1) / Narrow::kTileM) <= kSplitTiles;
   const int64_t tile_m = narrow ? Narrow::kTileM : Wide::kTileM;
   p.m_tiles = static_cast<int32_t>((m_dim + tile_m - 1) / tile_m);
   p.k_blocks = static_cast<int32_t>((sum + in_row - 1) / in_row);
@@ -1333,10 +1350,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   const cuuint32_t w_box[3] = {in_row, kMode == kFwd ? static_cast<cuuint32_t>(kM) : 64u, 1};
   const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows)};
   const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
-  // most row tiles that x.rows rows can take: one not full for each segment that has rows
-  const int64_t with_rows = x.rows < p.segments ? x.rows : p.segments;
   int64_t nt = narrow ? Narrow::NT : Wide::NT;
-  const auto most_tiles = [&](int64_t n) { return (x.rows + (n - 1) * with_rows) / n; };
   if (most_tiles(nt) * p.m_tiles > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
   int num_sms = 0;
   B2M_TRY(device_ready(&num_sms));
@@ -1355,16 +1369,17 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   }
   // Too few tiles for the SMs: clusters of two to eight CTAs share each one along its sum, as
   // many as are resident together (two CTAs on an SM; 33 clusters of eight were), so that a
-  // cluster has one tile.  Each CTA needs blocks enough to be worth the exchange, and more of
-  // them where two share an SM.  Integers, one row: 2048 x 7168 (16 tiles) 16.4 us unshared, 9.3
-  // by eights; 8192 x 8192 (64) 19.3, 16.8 by fours, 18.2 by twos; 4096 x 4096 (32, four blocks
-  // each by eights) 11.5, 9.25 by fours, 10.0 by eights.  From 65 tiles on sharing costs more
+  // cluster has one tile.  The exchange costs 1 us, which 16 blocks of a sum are worth (integers, 200 rows,
+  // 512 x 1024, eight blocks: 6.3 us unshared, 6.8 by fours; bf16, 16 blocks: 8.2 and 7.5), and CTAs
+  // that share an SM need more of them.  Integers, one row: 2048 x 7168 (16 tiles) 15.8 us unshared,
+  // 7.5 by eights; 8192 x 8192 (64) 19.3, 16.8 by fours, 18.2 by twos; eight rows, 4096 x 4096 (32, four
+  // blocks each by eights) 11.0, 7.5 by fours, 8.2 by eights.  From 65 tiles on sharing costs more
   // than it gives (14336 x 4096, 112 tiles: 14.7 unshared, 16.0 by twos).
   if (narrow) {
     const int64_t tiles = row_tiles * p.m_tiles;
     p.parts = 1;
-    while (p.parts < kMostParts && tiles <= kSplitTiles && tiles * p.parts * 2 <= 4 * kSplitTiles &&
-           p.k_blocks >= (tiles * p.parts * 2 <= 2 * kSplitTiles ? 4 : 8) * p.parts * 2)
+    while (p.parts < kMostParts && tiles <= kSplitTiles && p.k_blocks >= 16 && tiles * p.parts * 2 <= 4 * kSplitTiles &&
+           p.k_blocks >= (tiles * p.parts * 2 <= 2 * kSplitTiles ? 2 : 8) * p.parts * 2)
       p.parts *= 2;
     if (p.parts > 1) return launch<kMode, kI8, Split>(maps, p, tiles, num_sms, s);
     // E=128, eight rows, 1536 x 2048 (96 tiles): 14.2 us single, 15.7 two on an SM; integers,
