@@ -44,6 +44,7 @@ constexpr int kBand = 8;           // row tiles walked together, so that they sh
 constexpr int kSortMost = 256;     // experts up to which segments are sorted by length
 constexpr int kFeed = 4;           // tiles found ahead
 constexpr int kSplitTiles = 64;    // most tiles of a launch whose CTAs share sums
+constexpr int kLeastSplit = 16;    // blocks of a sum that is shared
 constexpr int kStagePitch = 144;   // bytes between two staged output rows of 128: no bank is hit twice
 
 // A tile is NT output rows by 128 output columns, or, for a pair of CTAs, by 256: each CTA
@@ -75,16 +76,17 @@ using Narrow = Shape<32, false, false, 4, 2>;
 // For one round of tiles or less: the whole SM's ring for one CTA.
 using Single = Shape<32, false, false, 9, 1>;
 using Split = Shape<32, false, true, 4, 2>;
+using Split64 = Shape<64, false, true, 7, 1>;
 constexpr int kMostParts = 8;
 
 // What the CTAs of a split tile hand to each other: for every part, the accumulators of the
 // columns that this CTA adds up.  A cluster has one tile at most.
-template <bool kSplit>
+template <bool kSplit, int kRows>
 struct Join {};
-template <>
-struct Join<true> {
+template <int kRows>
+struct Join<true, kRows> {
   uint64_t full;  // every part's accumulators are here
-  alignas(16) uint32_t part[Split::NT * kM];
+  alignas(16) uint32_t part[kRows * kM];
 };
 
 // One output tile: rows [row0, row0 + cols) of the output (kDw: of expert e's output),
@@ -121,7 +123,7 @@ struct Control {
   uint16_t seg[kMaxExperts + 2];   // the segment at place r
   // 32 output rows of 64 columns, for two warps each
   alignas(16) uint8_t staging[S::kSplit ? 1 : S::kEpiWarps / 2][S::kSplit ? 16 : 32 * kStagePitch];
-  Join<S::kSplit> join;
+  Join<S::kSplit, S::NT> join;
 };
 
 // Warps: 0 and 2 feed the ring, 1 issues MMAs, 3 finds tiles, 4 and following write outputs, the
@@ -1042,22 +1044,29 @@ __device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, u
   }
   // A thread adds up one column of every 128 / share rows.
   const int mine = at.part * share + in_share;
-  float a_lane = 0.0f, w_scale = 0.0f;  // a_lane: of row `lane`
-  if (kI8 && lane < r.cols) a_lane = __ldg(p.a_scale + r.row0 + lane);
+  constexpr int kBlocks = S::NT / 32;  // of 32 rows
+  float a_lane[kBlocks] = {}, w_scale = 0.0f;  // a_lane[h]: of row 32 h + lane
+#pragma unroll
+  for (int h = 0; h < kBlocks; ++h)
+    if (kI8 && 32 * h + lane < r.cols) a_lane[h] = __ldg(p.a_scale + r.row0 + 32 * h + lane);
   if (kI8 && r.m0 + mine < p.m_dim) w_scale = __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + r.m0 + mine);
   if (!wait_warp(&C->tfull[0], 0, p, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort)) return;
   tc_fence_after();
-  float v[32];
-  tmem_ld32(tmem_base + (static_cast<uint32_t>(q * 32) << 16), v);
-  tmem_ld_wait();
-  tc_fence_before();
   const uint32_t to =
       mapa_shared(smem_u32(&C->join.part[at.part * S::NT * share + in_share]), static_cast<uint32_t>(owner));
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (j < r.cols)
-      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + static_cast<uint32_t>(j * share * 4)), "f"(v[j])
-                   : "memory");
+  for (int h = 0; h < kBlocks; ++h) {
+    float v[32];
+    tmem_ld32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + 32 * h, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (32 * h + j < r.cols)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + static_cast<uint32_t>((32 * h + j) * share * 4)),
+                     "f"(v[j])
+                     : "memory");
+  }
+  tc_fence_before();
   __syncwarp();
   if ((lane & (share - 1)) == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&C->join.full), owner));
 
@@ -1081,7 +1090,10 @@ __device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, u
     for (int u = 0; u < kAtOnce; ++u) {
       const int j = (i0 + u * kM) >> bits;
       float y = __uint_as_float(sum[u]);
-      if (kI8) y = __int2float_rn(static_cast<int>(sum[u])) * __shfl_sync(0xffffffffu, a_lane, j & 31) * w_scale;
+      if (kI8) {
+        const float a_scale = __shfl_sync(0xffffffffu, a_lane[kBlocks > 1 && j >= 32 ? kBlocks - 1 : 0], j & 31);
+        y = __int2float_rn(static_cast<int>(sum[u])) * a_scale * w_scale;
+      }
       if (j < r.cols && r.m0 + mine < p.m_dim) put(p.out, out + j * p.ldo + mine, p.out_type, y);
     }
   }
@@ -1314,24 +1326,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   p.segments = p.experts + (clear_rest && ends ? 1 : 0);
   p.rows = x.rows;
   p.m_dim = static_cast<int32_t>(m_dim);
-  // Row tiles of 32, one CTA each, while segments are short: weights alone bound these calls,
-  // and four times as many CTAs share them out (E=32, 4096 x 7168, forward: 280 us narrow, 288
-  // wide at 8 rows each).  The mean is all that the host knows of
-  // the lengths.  Under Zipf 1.2 the longest segments cost a narrow launch more than it saves from
-  // 16 rows on average (299 narrow, 292 wide; 377 and 311 at 32), and not yet at 12 (278, 292).
-  // One segment alone has the length that the host sees: up to one narrow tile.  And narrow
-  // whenever that makes so few tiles that clusters can share them out: bf16, one segment of 96 rows,
-  // 2048 x 7168 (64 tiles at most), 26.8 us wide, 16.7 narrow.
-  // Most row tiles of n that x.rows rows can take: one not full for each segment that has rows.
-  const int64_t with_rows = x.rows < p.segments ? x.rows : p.segments;
-  const auto most_tiles = [&](int64_t n) { return (x.rows + (n - 1) * with_rows) / n; };
-  const bool narrow = x.rows <= (w.experts == 1 ? Narrow::NT : 12 * w.experts) ||
-                      most_tiles(Narrow::NT) * ((m_dim + Narrow::kTileM - 1) / Narrow::kTileM) <= kSplitTiles;
-  const int64_t tile_m = narrow ? Narrow::kTileM : Wide::kTileM;
-  p.m_tiles = static_cast<int32_t>((m_dim + tile_m - 1) / tile_m);
   p.k_blocks = static_cast<int32_t>((sum + in_row - 1) / in_row);
-  p.m_magic = magic(p.m_tiles);
-  p.band_magic = magic(int64_t(kBand) * p.m_tiles);
   p.out = out;
   p.ldo = ldo;
   p.out_type = out_type;
@@ -1340,54 +1335,92 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   p.w_scale = w_scale;
   p.status = status;
   p.timeout_ns = wait_limit(p.k_blocks);
-  p.idesc = (kI8 ? (2u << 4) | (1u << 7) | (1u << 10)                                             // S32, both signed
-                 : (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u)) |             // F32
-            (kMode == kDx ? 1u << 15 : 0u) | (static_cast<uint32_t>(tile_m >> 4) << 24);
 
-  const cuuint64_t w_dims[3] = {static_cast<cuuint64_t>(w.k), static_cast<cuuint64_t>(w.n),
-                                static_cast<cuuint64_t>(w.experts)};
-  const cuuint64_t w_strides[2] = {static_cast<cuuint64_t>(w.ld * elem), static_cast<cuuint64_t>(w.expert_stride * elem)};
-  const cuuint32_t w_box[3] = {in_row, kMode == kFwd ? static_cast<cuuint32_t>(kM) : 64u, 1};
-  const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows)};
-  const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
-  int64_t nt = narrow ? Narrow::NT : Wide::NT;
-  if (most_tiles(nt) * p.m_tiles > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
+  // Most row tiles of n that x.rows rows in so many segments can take: one not full for each that has rows.
+  const auto row_tiles = [&](int64_t n, int64_t segments) {
+    return (x.rows + (n - 1) * (x.rows < segments ? x.rows : segments)) / n;
+  };
+  const auto m_tiles = [&](int64_t m) { return (m_dim + m - 1) / m; };
+  // Row tiles of 32, one CTA each, while segments are short: weights alone bound these calls,
+  // and four times as many CTAs share them out (E=32, 4096 x 7168, forward: 280 us narrow, 288
+  // wide at 8 rows each).  The mean is all that the host knows of the lengths.  Under Zipf 1.2 the
+  // longest segments cost a narrow launch more than it saves from 16 rows on average (299
+  // narrow, 292 wide; 377 and 311 at 32), and not yet at 12 (278, 292).  One segment alone has the
+  // length that the host sees: up to one narrow tile.
+  //
+  // Few tiles for the SMs: clusters of two to eight CTAs share each one along its sum.  So a
+  // launch is narrow whenever that makes no more than 64 tiles (bf16, one segment of 96 rows, 2048 x
+  // 7168: 26.8 us wide, 16.7 narrow), and takes tiles of 64 rows when those are so few and their
+  // sums long: 256 rows 26.8 wide, 21.2; 64 rows, 4096 x 4096, 18.8 and 15.7; integers, 64 rows, 7168 x
+  // 2048 (16 blocks), 9.9 and 11.3.
+  const int64_t narrow_tiles = row_tiles(Split::NT, w.experts) * m_tiles(Split::kTileM);
+  const int64_t middle_tiles = row_tiles(Split64::NT, w.experts) * m_tiles(Split64::kTileM);
+  const bool narrow = x.rows <= (w.experts == 1 ? Narrow::NT : 12 * w.experts) || narrow_tiles <= kSplitTiles;
+  const bool middle = !narrow && middle_tiles <= kSplitTiles && p.k_blocks >= 2 * kLeastSplit;
+  const int64_t most = narrow   ? row_tiles(Narrow::NT, p.segments) * m_tiles(Narrow::kTileM)
+                       : middle ? row_tiles(Split64::NT, p.segments) * m_tiles(Split64::kTileM)
+                                : row_tiles(Wide::NT, p.segments) * m_tiles(Wide::kTileM);
+  if (most > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
   int num_sms = 0;
   B2M_TRY(device_ready(&num_sms));
-  if (!narrow) nt = rows_of_tile(num_sms, [&](int64_t n) { return most_tiles(n) * p.m_tiles; });
-  const int64_t row_tiles = most_tiles(nt);
-  p.tile_bits = bits_of(nt);
   if (x.rows == 0) return B2M_OK;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  Maps maps{};
-  B2M_TRY(encode_map(&maps.cols, type, 3, w.ptr, w_dims, w_strides, w_box, what));
-  const cuuint32_t quarter = (narrow ? Narrow::kBRows : Wide::kBRows) / 4;
-  for (int i = 0; i < 4; ++i) {
-    if (narrow ? !used_map<Narrow>(i) : !used_map<Wide>(i)) continue;
-    const cuuint32_t box[2] = {in_row, quarter * (i + 1)};
-    B2M_TRY(encode_map(&maps.rows[i], type, 2, x.ptr, x_dims, x_strides, box, what));
-  }
-  // Too few tiles for the SMs: clusters of two to eight CTAs share each one along its sum, as
-  // many as are resident together (two CTAs on an SM; 33 clusters of eight were), so that a
-  // cluster has one tile.  The exchange costs 1 us, which 16 blocks of a sum are worth (integers, 200 rows,
-  // 512 x 1024, eight blocks: 6.3 us unshared, 6.8 by fours; bf16, 16 blocks: 8.2 and 7.5), and CTAs
-  // that share an SM need more of them.  Integers, one row: 2048 x 7168 (16 tiles) 15.8 us unshared,
-  // 7.5 by eights; 8192 x 8192 (64) 19.3, 16.8 by fours, 18.2 by twos; eight rows, 4096 x 4096 (32, four
-  // blocks each by eights) 11.0, 7.5 by fours, 8.2 by eights.  From 65 tiles on sharing costs more
-  // than it gives (14336 x 4096, 112 tiles: 14.7 unshared, 16.0 by twos).
+
+  // `shape` is the launch's, `n` the rows of its tiles.
+  const auto run = [&](auto shape, int64_t n, int parts) -> int {
+    using S = decltype(shape);
+    p.parts = parts;
+    p.tile_bits = bits_of(n);
+    p.m_tiles = static_cast<int32_t>(m_tiles(S::kTileM));
+    p.m_magic = magic(p.m_tiles);
+    p.band_magic = magic(int64_t(kBand) * p.m_tiles);
+    p.idesc = (kI8 ? (2u << 4) | (1u << 7) | (1u << 10)                                  // S32, both signed
+                   : (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u)) |  // F32
+              (kMode == kDx ? 1u << 15 : 0u) | (static_cast<uint32_t>(S::kTileM >> 4) << 24);
+    const cuuint64_t w_dims[3] = {static_cast<cuuint64_t>(w.k), static_cast<cuuint64_t>(w.n),
+                                  static_cast<cuuint64_t>(w.experts)};
+    const cuuint64_t w_strides[2] = {static_cast<cuuint64_t>(w.ld * elem),
+                                     static_cast<cuuint64_t>(w.expert_stride * elem)};
+    const cuuint32_t w_box[3] = {in_row, kMode == kFwd ? static_cast<cuuint32_t>(kM) : 64u, 1};
+    const cuuint64_t x_dims[2] = {static_cast<cuuint64_t>(x.cols), static_cast<cuuint64_t>(x.rows)};
+    const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
+    Maps maps{};
+    B2M_TRY(encode_map(&maps.cols, type, 3, w.ptr, w_dims, w_strides, w_box, what));
+    for (int i = 0; i < 4; ++i) {
+      if (!used_map<S>(i)) continue;
+      const cuuint32_t box[2] = {in_row, static_cast<cuuint32_t>(S::kBRows / 4 * (i + 1))};
+      B2M_TRY(encode_map(&maps.rows[i], type, 2, x.ptr, x_dims, x_strides, box, what));
+    }
+    return launch<kMode, kI8, S>(maps, p, row_tiles(n, p.segments) * p.m_tiles, num_sms,
+                                 static_cast<cudaStream_t>(stream));
+  };
+  // As many CTAs for a tile as are resident together (33 clusters of eight were, of two CTAs on an
+  // SM), so that a cluster has one tile.  The exchange costs 1 us, which 16 blocks of a sum are
+  // worth (integers, 200 rows, 512 x 1024, eight blocks: 6.3 us unshared, 6.8 by fours; bf16, 16
+  // blocks: 8.2 and 7.5), and CTAs that share an SM need more of them.  Integers, one row: 2048 x
+  // 7168 (16 tiles) 15.8 us unshared, 7.5 by eights; 8192 x 8192 (64) 19.3, 16.8 by fours, 18.2 by
+  // twos; eight rows, 4096 x 4096 (32, four blocks each by eights) 11.0, 7.5 by fours, 8.2 by
+  // eights.  From 65 tiles on sharing costs more than it gives (14336 x 4096, 112 tiles: 14.7
+  // unshared, 16.0 by twos).
+  const auto parts_of = [&](int64_t tiles, int on_sm) {
+    int parts = 1;
+    while (parts < kMostParts && tiles <= kSplitTiles && p.k_blocks >= kLeastSplit &&
+           tiles * parts * 2 <= 2 * on_sm * kSplitTiles &&
+           p.k_blocks >= (tiles * parts * 2 <= 2 * kSplitTiles ? 2 : 8) * parts * 2)
+      parts *= 2;
+    return parts;
+  };
+  if (middle) return run(Split64{}, Split64::NT, parts_of(middle_tiles, Split64::kResident));
   if (narrow) {
-    const int64_t tiles = row_tiles * p.m_tiles;
-    p.parts = 1;
-    while (p.parts < kMostParts && tiles <= kSplitTiles && p.k_blocks >= 16 && tiles * p.parts * 2 <= 4 * kSplitTiles &&
-           p.k_blocks >= (tiles * p.parts * 2 <= 2 * kSplitTiles ? 2 : 8) * p.parts * 2)
-      p.parts *= 2;
-    if (p.parts > 1) return launch<kMode, kI8, Split>(maps, p, tiles, num_sms, s);
+    const int parts = parts_of(narrow_tiles, Split::kResident);
+    if (parts > 1) return run(Split{}, Split::NT, parts);
     // E=128, eight rows, 1536 x 2048 (96 tiles): 14.2 us single, 15.7 two on an SM; integers,
     // 28672 x 4096 (224): 24.9 and 23.3; E=8, two rows, 28672 x 4096 (448): 84 and 77.5.
-    if (tiles <= num_sms) return launch<kMode, kI8, Single>(maps, p, tiles, num_sms, s);
-    return launch<kMode, kI8, Narrow>(maps, p, tiles, num_sms, s);
+    if (most <= num_sms) return run(Single{}, Single::NT, 1);
+    return run(Narrow{}, Narrow::NT, 1);
   }
-  return launch<kMode, kI8, Wide>(maps, p, row_tiles * p.m_tiles, num_sms, s);
+  const int64_t n =
+      rows_of_tile(num_sms, [&](int64_t rows) { return row_tiles(rows, p.segments) * m_tiles(Wide::kTileM); });
+  return run(Wide{}, n, 1);
 }
 
 int check_16bit(const char* what, int32_t in_type) {
