@@ -20,7 +20,7 @@
 // the last, rounded once.
 //
 // Rows that a tile loads beyond its segment are other output rows in kFwd and kDx, computed
-// and never stored.  In kDw they would enter the sum: warp 12 clears them (in both operands,
+// and never stored.  In kDw they would enter the sum: the last warp clears them (in both operands,
 // so an infinity there cannot meet a zero) in the segment's last stage before its MMA.
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
@@ -471,6 +471,10 @@ __device__ __forceinline__ void feed_tiles(const Params& p, Control<S>* C, int n
       const int blocks = r.k_blocks;
       r.k0 = blocks * at.part / p.parts;
       r.k_blocks = blocks * (at.part + 1) / p.parts - r.k0;
+      if (kMode == kDw) {
+        r.sum0 += r.k0 * 64;
+        r.sum_rows = min(r.sum_rows - r.k0 * 64, r.k_blocks * 64);
+      }
     }
     const bool last = i * at.stride >= num_tiles;  // no CTA has a tile in this round
     if (r.e >= 0 || last) {
@@ -634,7 +638,7 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
         break;
       }
       const uint32_t a = smem0 + s * S::kStageBytes, b = a + kABytes;
-      const bool tail = kMode == kDw && r.sum_rows - kb * 64 < 64;  // warp 12 comes between the copies and the MMA
+      const bool tail = kMode == kDw && r.sum_rows - kb * 64 < 64;  // the last warp comes between the copies and the MMA
       const uint32_t bar = (tail ? landed0_own : full0_leader) + s * 8;
       if (elect_one()) {
         if (tail) {
@@ -686,7 +690,7 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
   __syncwarp();
 }
 
-// Warp 12 of kDw: when this CTA's copies of a segment's last, partly filled stage have landed,
+// The last warp of kDw: when this CTA's copies of a segment's last, partly filled stage have landed,
 // clears the rows behind the segment, up to the next step of the MMA, and tells the (leader's)
 // MMA warp.
 template <class S>
@@ -711,7 +715,12 @@ __device__ __forceinline__ void clear_tails(const Params& p, uint8_t* smem, Cont
     }
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&C->cleared[s]), 0));
+    if (lane == 0) {
+      if (S::kPair)
+        mbar_arrive_cluster(mapa_shared(smem_u32(&C->cleared[s]), 0));
+      else
+        mbar_arrive(&C->cleared[s]);
+    }
   }
 }
 
@@ -1026,7 +1035,7 @@ __device__ __forceinline__ void put(void* out, int64_t at, int32_t type, float v
 // cluster adds up columns d * 128 / parts and following: every CTA sends each of them the
 // accumulators of its part, [part][row][column], and the owner adds them in the order of the
 // parts, so the result does not depend on who comes first.
-template <bool kI8, class S>
+template <int kMode, bool kI8, class S>
 __device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, uint32_t tmem_base, const Where& at,
                                                int warp, int lane) {
   const int q = warp & 3;
@@ -1036,8 +1045,8 @@ __device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, u
   TileFeed<S> feed(p, C);
   Tile r;
   if (!feed.next(r) || r.e < 0) return;
-  const int64_t out = static_cast<int64_t>(r.row0) * p.ldo + r.m0;
-  if (r.k_blocks == 0) {  // rows of no expert
+  const int64_t out = (kMode == kDw ? r.e * p.out_expert : 0) + static_cast<int64_t>(r.row0) * p.ldo + r.m0;
+  if (kMode != kDw && r.e >= p.experts) {  // rows of no expert
     if (at.part == 0 && r.m0 + column < p.m_dim)
       for (int j = 0; j < r.cols; ++j) put(p.out, out + j * p.ldo + column, p.out_type, 0.0f);
     return;
@@ -1050,15 +1059,18 @@ __device__ __forceinline__ void epilogue_split(const Params& p, Control<S>* C, u
   for (int h = 0; h < kBlocks; ++h)
     if (kI8 && 32 * h + lane < r.cols) a_lane[h] = __ldg(p.a_scale + r.row0 + 32 * h + lane);
   if (kI8 && r.m0 + mine < p.m_dim) w_scale = __ldg(p.w_scale + static_cast<int64_t>(r.e) * p.m_dim + r.m0 + mine);
-  if (!wait_warp(&C->tfull[0], 0, p, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort)) return;
+  const bool some = kMode != kDw || r.k_blocks > 0;  // a short segment leaves parts without a block
+  if (some && !wait_warp(&C->tfull[0], 0, p, B2M_STATUS_TIMEOUT_EPILOGUE, &C->abort)) return;
   tc_fence_after();
   const uint32_t to =
       mapa_shared(smem_u32(&C->join.part[at.part * S::NT * share + in_share]), static_cast<uint32_t>(owner));
 #pragma unroll
   for (int h = 0; h < kBlocks; ++h) {
-    float v[32];
-    tmem_ld32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + 32 * h, v);
-    tmem_ld_wait();
+    float v[32] = {};
+    if (some) {
+      tmem_ld32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) + 32 * h, v);
+      tmem_ld_wait();
+    }
 #pragma unroll
     for (int j = 0; j < 32; ++j)
       if (32 * h + j < r.cols)
@@ -1123,7 +1135,7 @@ __global__ void __launch_bounds__(threads_of<S>(kMode), S::kResident)
     }
     if constexpr (S::kSplit)  // from every part, one arrival for each run of a warp's lanes
       mbar_init(&C->join.full, p.parts * max(1, S::kEpiWarps / p.parts));
-    // readers of a tile: producers, epilogue warps, (kDw) warp 12, and the MMA warp of the leader
+    // readers of a tile: producers, epilogue warps, (kDw) the last warp, and the MMA warp of the leader
     for (int s = 0; s < kFeed; ++s) {
       mbar_init(&C->fed[s], 1);
       mbar_init(&C->taken[s], 2 + S::kEpiWarps + (kMode == kDw ? 1 : 0) + (at.rank == 0 ? 1 : 0));
@@ -1162,10 +1174,10 @@ __global__ void __launch_bounds__(threads_of<S>(kMode), S::kResident)
     const int num_tiles = kMode == kDw ? p.experts * p.m_tiles * p.c_tiles : C->tile0[p.segments] * p.m_tiles;
     if (lane == 0) feed_tiles<kMode, S>(p, C, num_tiles, at);
     __syncwarp();
-  } else if (warp == 12) {
+  } else if (kMode == kDw && warp == 4 + S::kEpiWarps) {
     clear_tails<S>(p, smem, C, lane);
   } else if constexpr (S::kSplit) {
-    epilogue_split<kI8, S>(p, C, tmem_base, at, warp, lane);
+    epilogue_split<kMode, kI8, S>(p, C, tmem_base, at, warp, lane);
   } else {
     epilogue<kMode, kI8, S>(p, C, tmem_base, at.rank, warp, lane);
   }
@@ -1267,6 +1279,23 @@ int32_t bits_of(int64_t n) {
   int32_t b = 0;
   while (n >> (b + 1)) ++b;
   return b;
+}
+
+// CTAs that share a tile of a sum of `blocks` blocks: as many as are resident together (33 clusters
+// of eight were, of two CTAs on an SM), so that a cluster has one tile.  The exchange costs 1 us,
+// which 16 blocks of a sum are worth (integers, 200 rows, 512 x 1024, eight blocks: 6.3 us
+// unshared, 6.8 by fours; bf16, 16 blocks: 8.2 and 7.5), and CTAs that share an SM need more of
+// them.  Integers, one row: 2048 x 7168 (16 tiles) 15.8 us unshared, 7.5 by eights; 8192 x 8192
+// (64) 19.3, 16.8 by fours, 18.2 by twos; eight rows, 4096 x 4096 (32, four blocks each by
+// eights) 11.0, 7.5 by fours, 8.2 by eights.  From 65 tiles on sharing costs more than it gives
+// (14336 x 4096, 112 tiles: 14.7 unshared, 16.0 by twos).
+int parts_of(int64_t tiles, int64_t blocks, int on_sm) {
+  int parts = 1;
+  while (parts < kMostParts && tiles <= kSplitTiles && blocks >= kLeastSplit &&
+         tiles * parts * 2 <= 2 * on_sm * kSplitTiles &&
+         blocks >= (tiles * parts * 2 <= 2 * kSplitTiles ? 2 : 8) * parts * 2)
+    parts *= 2;
+  return parts;
 }
 
 // Limit of a wait inside a CTA's pipeline, where nothing but the CTA's own work is waited for: a
@@ -1393,25 +1422,9 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
     return launch<kMode, kI8, S>(maps, p, row_tiles(n, p.segments) * p.m_tiles, num_sms,
                                  static_cast<cudaStream_t>(stream));
   };
-  // As many CTAs for a tile as are resident together (33 clusters of eight were, of two CTAs on an
-  // SM), so that a cluster has one tile.  The exchange costs 1 us, which 16 blocks of a sum are
-  // worth (integers, 200 rows, 512 x 1024, eight blocks: 6.3 us unshared, 6.8 by fours; bf16, 16
-  // blocks: 8.2 and 7.5), and CTAs that share an SM need more of them.  Integers, one row: 2048 x
-  // 7168 (16 tiles) 15.8 us unshared, 7.5 by eights; 8192 x 8192 (64) 19.3, 16.8 by fours, 18.2 by
-  // twos; eight rows, 4096 x 4096 (32, four blocks each by eights) 11.0, 7.5 by fours, 8.2 by
-  // eights.  From 65 tiles on sharing costs more than it gives (14336 x 4096, 112 tiles: 14.7
-  // unshared, 16.0 by twos).
-  const auto parts_of = [&](int64_t tiles, int on_sm) {
-    int parts = 1;
-    while (parts < kMostParts && tiles <= kSplitTiles && p.k_blocks >= kLeastSplit &&
-           tiles * parts * 2 <= 2 * on_sm * kSplitTiles &&
-           p.k_blocks >= (tiles * parts * 2 <= 2 * kSplitTiles ? 2 : 8) * parts * 2)
-      parts *= 2;
-    return parts;
-  };
-  if (middle) return run(Split64{}, Split64::NT, parts_of(middle_tiles, Split64::kResident));
+  if (middle) return run(Split64{}, Split64::NT, parts_of(middle_tiles, p.k_blocks, Split64::kResident));
   if (narrow) {
-    const int parts = parts_of(narrow_tiles, Split::kResident);
+    const int parts = parts_of(narrow_tiles, p.k_blocks, Split::kResident);
     if (parts > 1) return run(Split{}, Split::NT, parts);
     // E=128, eight rows, 1536 x 2048 (96 tiles): 14.2 us single, 15.7 two on an SM; integers,
     // 28672 x 4096 (224): 24.9 and 23.3; E=8, two rows, 28672 x 4096 (448): 84 and 77.5.
@@ -1482,9 +1495,7 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   p.segments = experts;
   p.rows = rows;
   p.m_dim = static_cast<int32_t>(k);
-  p.m_tiles = static_cast<int32_t>((k + Wide::kTileM - 1) / Wide::kTileM);
   p.c_dim = static_cast<int32_t>(n);
-  p.band_magic = magic(int64_t(kBand) * p.m_tiles);
   p.out = out;
   p.ldo = ldo;
   p.out_expert = out_stride;
@@ -1492,16 +1503,10 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   p.wide_out = aligned16(out) && ldo % 8 == 0 && out_stride % 8 == 0;
   p.status = dev_status;
   p.timeout_ns = wait_limit(rows / 64);
-  p.idesc = (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) |
-            (static_cast<uint32_t>(Wide::kTileM >> 4) << 24);
-  const auto tiles_of = [&](int64_t rows) { return (n + rows - 1) / rows * p.m_tiles * experts; };
-  if (tiles_of(Wide::NT) > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
+  const auto tiles_of = [&](int64_t c, int64_t m) { return (n + c - 1) / c * ((k + m - 1) / m) * experts; };
+  if (tiles_of(Wide::NT, Wide::kTileM) > kMaxTiles) return fail(B2M_ERR_ARG, "%s: more than 2^30 tiles", what);
   int num_sms = 0;
   B2M_TRY(device_ready(&num_sms));
-  const int64_t nt = rows_of_tile(num_sms, tiles_of), tiles = tiles_of(nt);
-  p.tile_bits = bits_of(nt);
-  p.c_tiles = static_cast<int32_t>((n + nt - 1) / nt);
-  p.expert_magic = magic(int64_t(p.m_tiles) * p.c_tiles);
   const CUtensorMapDataType type =
       in_type == B2M_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   // Without rows every segment is empty: nothing is loaded, and a map of no rows cannot be made.
@@ -1515,8 +1520,25 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
     B2M_TRY(encode_map(&maps.cols, type, 2, x, x_dims, x_strides, box, what));
     B2M_TRY(encode_map(&maps.rows[3], type, 2, dy, dy_dims, dy_strides, box, what));
   }
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return launch<kDw, false, Wide>(maps, p, tiles, num_sms, s);
+  const auto run = [&](auto shape, int64_t c, int parts) -> int {
+    using S = decltype(shape);
+    p.parts = parts;
+    p.tile_bits = bits_of(c);
+    p.m_tiles = static_cast<int32_t>((k + S::kTileM - 1) / S::kTileM);
+    p.c_tiles = static_cast<int32_t>((n + c - 1) / c);
+    p.band_magic = magic(int64_t(kBand) * p.m_tiles);
+    p.expert_magic = magic(int64_t(p.m_tiles) * p.c_tiles);
+    p.idesc = (1u << 4) | (in_type == B2M_BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 15) | (1u << 16) |
+              (static_cast<uint32_t>(S::kTileM >> 4) << 24);
+    return launch<kDw, false, S>(maps, p, tiles_of(c, S::kTileM), num_sms, static_cast<cudaStream_t>(stream));
+  };
+  // Long sums of few tiles are shared like those of the other directions, by the segments' mean
+  // length.  bf16, 272 x 128 (five tiles): 8192 rows 32 us wide, 11 by eights; 1024 rows 9.6, 7.4;
+  // 512 x 1024 (64 tiles): 32.5, 25.6 by twos; 2048 rows 13.1, 12.9; 1024 rows 9.6, 10.6.
+  const int64_t mean = rows / 64 / experts;  // blocks
+  const int parts = parts_of(tiles_of(Split64::NT, Split64::kTileM), mean, Split64::kResident);
+  if (parts > 2 || (parts == 2 && mean >= 2 * kLeastSplit)) return run(Split64{}, Split64::NT, parts);
+  return run(Wide{}, rows_of_tile(num_sms, [&](int64_t c) { return tiles_of(c, Wide::kTileM); }), 1);
 }
 
 extern "C" int b2m_int8_mm(const void* a, const float* a_scale, int64_t rows, int64_t lda, const void* w,

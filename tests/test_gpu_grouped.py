@@ -185,7 +185,7 @@ def test_outputs_that_start_anywhere(cols, pitch, offset):
 
 
 @pytest.mark.parametrize("counts", [[63], [64], [65], [129], [191], [193], [257], [385], [1000], [129, 0, 65], [40, 300, 2],
-                                    [2100], [5000]])
+                                    [2100], [5000], [3000, 0, 1, 70, 2500], [0, 6000, 0], [1, 8191]])
 @pytest.mark.parametrize("n,k", [(40, 264), (264, 40), (300, 136)])
 def test_few_tiles(counts, n, k):
     """Calls of few tiles, whose tiles have fewer rows: one tile and one more or one less than full ones."""
