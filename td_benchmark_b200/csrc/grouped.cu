@@ -1146,7 +1146,8 @@ __global__ void __launch_bounds__(threads_of<S>(kMode), S::kResident)
     if (p.rows > 0) {  // without rows nothing is loaded, and kDw has no maps
       tma_prefetch_desc(&maps.cols);
       for (int i = 0; i < 4; ++i)
-        if (used_map<S>(i) && (kMode != kDw || i == 3)) tma_prefetch_desc(&maps.rows[i]);
+        if (used_map<S>(i) && (kMode == kDw ? i == 3 : S::kBRows / 4 * i * S::kCtas < 1 << p.tile_bits))
+          tma_prefetch_desc(&maps.rows[i]);
     }
   }
   if (warp == 1) {
@@ -1414,7 +1415,7 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
     const cuuint64_t x_strides[1] = {static_cast<cuuint64_t>(x.ld * elem)};
     Maps maps{};
     B2M_TRY(encode_map(&maps.cols, type, 3, w.ptr, w_dims, w_strides, w_box, what));
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4 && S::kBRows / 4 * i < n / S::kCtas; ++i) {  // a tile of n rows takes no larger box
       if (!used_map<S>(i)) continue;
       const cuuint32_t box[2] = {in_row, static_cast<cuuint32_t>(S::kBRows / 4 * (i + 1))};
       B2M_TRY(encode_map(&maps.rows[i], type, 2, x.ptr, x_dims, x_strides, box, what));
