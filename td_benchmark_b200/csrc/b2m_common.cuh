@@ -131,7 +131,6 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-
 // Four-row gather (tensor map box is one row high): rows r0..r3 at column x land
 // in four consecutive 128-byte smem rows starting at dst.  Rows past the tensor's
 // extent are zero filled.

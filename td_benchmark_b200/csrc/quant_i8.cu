@@ -101,10 +101,11 @@ __device__ __forceinline__ uint32_t larger_vec(uint32_t a, const uint4& v) {
 // Codes of one vector.  x * (1 / scale) is within 1.6e-5 of x / scale (two roundings of a
 // value of at most 127) and the IEEE quotient within 4e-6, so both round to the same integer
 // unless the product lies within 2e-5 of a tie; values that come within kNearTie of one are
-// divided.  (Of 16-bit values one in a thousand does, since x / scale is 127 times a ratio of
-// short integers.)  Adding 1.5 * 2^23 rounds to the nearest even integer and leaves it in the
-// low byte.  A division for each element would cost more than the memory traffic (8192 x 7168
-// bf16: 81 us with them; 27 us is what HBM needs).
+// decided by the remainder.  (Of 16-bit values one in a thousand does, since x / scale is 127
+// times a ratio of short integers; dividing those took 1.5 us more at 8192 x 7168.)  Adding
+// 1.5 * 2^23 rounds to the nearest even integer and leaves it in the low byte.  A division for each element
+// would cost more than the memory traffic (8192 x 7168 bf16: 81 us with them; 27 us is what HBM
+// needs).
 constexpr float kNearTie = 4e-5f;
 constexpr float kRound = 12582912.0f;
 
@@ -124,6 +125,19 @@ __device__ __forceinline__ void round_two(float x0, float x1, float inv, float& 
       : "f"(x0), "f"(x1), "f"(inv), "f"(kRound), "f"(-1.0f));
 }
 
+// The code (plus kRound) of an x whose product with 1 / scale lies `d` from the integer m, close
+// to the tie t = m +- 1/2.  e = x - t scale is exact: t has eight bits, so both terms are multiples
+// of 2^-25 of scale's power of two, and they differ by less than 2^11 of those.  The IEEE quotient is t
+// itself when x / scale is within half a step of it.  (Only at t = 1/2, a power of two, is the
+// step below it shorter; both answers are 0 there.)
+__device__ __forceinline__ float code_near_tie(float x, float scale, float m, float d) {
+  const float t = m + copysignf(0.5f, d);
+  const float e = __fmaf_rn(-t, scale, x);
+  const float half_step = __uint_as_float(__float_as_uint(t) & 0x7f800000u) * 5.9604644775390625e-8f;  // 2^-24
+  if (fabsf(e) <= scale * half_step) return t + kRound;  // the even one
+  return (e > 0.0f ? t + 0.5f : t - 0.5f) + kRound;
+}
+
 template <int N>
 __device__ __forceinline__ void codes_of(const float (&f)[N], float scale, float inv, bool divide,
                                          uint32_t (&w)[N / 4]) {
@@ -134,11 +148,16 @@ __device__ __forceinline__ void codes_of(const float (&f)[N], float scale, float
     round_two(f[j], f[j + 1], inv, r[j], r[j + 1], d0, d1);
     off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
   }
-  if (divide || off > 0.5f - kNearTie) {
+  if (divide) {
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      if (divide || fabsf(__fmaf_rn(f[j], inv, kRound - r[j])) > 0.5f - kNearTie)
-        r[j] = __int_as_float(max(-127, min(127, __float2int_rn(f[j] / scale))));  // a NaN quotient converts to 0
+      r[j] = __int_as_float(max(-127, min(127, __float2int_rn(f[j] / scale))));  // a NaN quotient converts to 0
+  } else if (off > 0.5f - kNearTie) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float d = __fmaf_rn(f[j], inv, kRound - r[j]);
+      if (fabsf(d) > 0.5f - kNearTie) r[j] = code_near_tie(f[j], scale, r[j] - kRound, d);
+    }
   }
 #pragma unroll
   for (int i = 0; i < N / 4; ++i)

@@ -459,6 +459,9 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
         scale = x.new_empty(rows, dtype=torch.float32)
     else:
         _vector(scale, "scale", (rows,), torch.float32, device)
+        lo, hi = _extent(scale)
+        for a, b in (_extent(x), _extent(q)):
+            _need(hi <= a or b <= lo, "scale overlaps x or q")
     _launch(device, "b2m_quant_i8", x.data_ptr(), code, rows, cols, strides[0] if rows > 1 else cols, q.data_ptr(), ldq,
             scale.data_ptr(), None if status is None else _status_word(status, device))
     return q, scale

@@ -319,6 +319,23 @@ def test_quant_int8_is_exact(rows, cols, dtype):
     assert torch.equal(q.cpu(), qr)
 
 
+@pytest.mark.parametrize("steps", [0, 1, 3, 300])
+def test_quant_int8_next_to_ties(steps):
+    """Rows whose quotients lie on a tie or up to `steps` steps of x beside it, at scales of every size."""
+    g = torch.Generator().manual_seed(steps)
+    rows, cols = 600, 512
+    top = torch.exp(torch.empty(rows, dtype=torch.float64).uniform_(-20, 60, generator=g)).float()
+    scale = torch.maximum(top.double() / 127, torch.tensor(1e-12, dtype=torch.float64)).float()
+    m = torch.randint(-127, 127, (rows, cols), generator=g)
+    x = ((m + 0.5) * scale.double()[:, None]).float()
+    x = (x.view(torch.int32) + torch.randint(-steps, steps + 1, (rows, cols), generator=g, dtype=torch.int32)).view(torch.float32)
+    x[:, 7] = top
+    q, s = ops.quant_int8(x.to(DEV))
+    qr, sr = _quant_ref(x)
+    assert torch.equal(s.cpu(), sr)
+    assert torch.equal(q.cpu(), qr)
+
+
 def test_quant_int8_strides_and_unaligned_rows():
     big = _randn(20, 700, seed=1)
     for at, cols in [(0, 256), (8, 513), (3, 100), (1, 699)]:
@@ -658,6 +675,14 @@ def test_refusals_of_the_wrappers():
                  lambda: ops.int8_mm(a[:, :24].contiguous(), s, wq[:, :24].contiguous(), sw)):
         with pytest.raises(Exception, match="16 bytes|16-byte"):
             call()
+
+
+def test_quant_refuses_scales_on_its_operands():
+    x = torch.zeros(8, 64, device=DEV)
+    q = torch.zeros(8, 64, device=DEV, dtype=torch.int8)
+    for scale in (x.view(-1)[:8], q.view(-1)[:32].view(torch.float32)):
+        with pytest.raises(ValueError, match="scale overlaps"):
+            ops.quant_int8(x, q=q, scale=scale)
 
 
 def test_one_double_backward_is_refused():
