@@ -66,10 +66,12 @@ struct Shape {
   static constexpr int kStageBytes = kABytes + kBRows * kRowBytes;
   static constexpr int kStages = kRing;
   static constexpr int kResident = kOnSm;  // CTAs on an SM
-  static constexpr int kEpiWarps = kPair ? 8 : 4;  // two sets of four, or one: 32 rows at a time each
+  static constexpr int kEpiWarps = NT > 64 ? 8 : 4;  // two sets of four, or one: 32 rows at a time each
   static constexpr uint32_t kTmemCols = 2 * NT;
 };
 using Wide = Shape<256, true, false, 6, 1>;
+// For weight gradients of up to 128 columns, which leave one CTA of a pair without any.
+using Slim = Shape<256, false, false, 4, 1>;
 // Two CTAs on an SM: one streams while the other starts or ends a tile, and a few rounds of
 // tiles share the memory out evenly.
 using Narrow = Shape<32, false, false, 4, 2>;
@@ -660,6 +662,8 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
           load_2d<S::kPair>(a + kABytes / 2, map_cols, bar, m0 + 64, sum);
           load_2d<S::kPair>(b, map_rows, bar, row, sum);
           if (boxes > 1) load_2d<S::kPair>(b + 64 * kRowBytes, map_rows, bar, row + 64, sum);
+          if (S::kBRows > 128)
+            for (int i = 2; i < boxes; ++i) load_2d<S::kPair>(b + i * 64 * kRowBytes, map_rows, bar, row + i * 64, sum);
         }
       }
       __syncwarp();
@@ -1269,10 +1273,10 @@ uint32_t magic(int64_t d) { return static_cast<uint32_t>(((uint64_t(1) << 32) + 
 // without a tile take it all: bf16, 1024 x 1024 x 1024, 12.6 us by 256, 9.2 by 64; 4096 x 256, a sum of
 // 7168, 39 and 25; its weight gradient, a sum of 4096, 26 and 21.  (Tiles of 32 gave no more
 // than 0.1 us.)
-template <class F>
+template <class S, class F>
 int64_t rows_of_tile(int num_sms, const F& tiles_of) {
-  int64_t n = Wide::NT;
-  while (n > Wide::NT / 4 && tiles_of(n / 2) <= num_sms / 2) n /= 2;
+  int64_t n = S::NT;
+  while (n > S::NT / 4 && tiles_of(n / 2) <= num_sms / S::kCtas) n /= 2;
   return n;
 }
 
@@ -1432,9 +1436,8 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
     if (most <= num_sms) return run(Single{}, Single::NT, 1);
     return run(Narrow{}, Narrow::NT, 1);
   }
-  const int64_t n =
-      rows_of_tile(num_sms, [&](int64_t rows) { return row_tiles(rows, p.segments) * m_tiles(Wide::kTileM); });
-  return run(Wide{}, n, 1);
+  const auto tiles = [&](int64_t n) { return row_tiles(n, p.segments) * m_tiles(Wide::kTileM); };
+  return run(Wide{}, rows_of_tile<Wide>(num_sms, tiles), 1);
 }
 
 int check_16bit(const char* what, int32_t in_type) {
@@ -1539,7 +1542,12 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   const int64_t mean = rows / 64 / experts;  // blocks
   const int parts = parts_of(tiles_of(Split64::NT, Split64::kTileM), mean, Split64::kResident);
   if (parts > 2 || (parts == 2 && mean >= 2 * kLeastSplit)) return run(Split64{}, Split64::NT, parts);
-  return run(Wide{}, rows_of_tile(num_sms, [&](int64_t c) { return tiles_of(c, Wide::kTileM); }), 1);
+  const auto tiles = [&](int64_t c) { return tiles_of(c, Wide::kTileM); };
+  // Gradients of up to 128 columns: 64 experts of 4096 x 64, 100 rows each, 43 us by pairs, 24; 32 of 4096 x
+  // 128, 1024 rows, 59 and 53.  (The other directions at such widths: 32768 rows, k = 4096, 57 by
+  // pairs, 52; but eight segments of 512 rows 17.7 and 19.4, sixteen of 230, k = 12352, 46 and 59.)
+  if (k <= Slim::kTileM) return run(Slim{}, rows_of_tile<Slim>(num_sms, tiles), 1);
+  return run(Wide{}, rows_of_tile<Wide>(num_sms, tiles), 1);
 }
 
 extern "C" int b2m_int8_mm(const void* a, const float* a_scale, int64_t rows, int64_t lda, const void* w,

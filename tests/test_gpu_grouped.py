@@ -197,6 +197,16 @@ def test_few_tiles(counts, n, k):
     _close(ops.grouped_mm_dw(dy, x, ends), _dw(dy, x, counts), _dw(dy.abs(), x.abs(), counts), max(counts))
 
 
+@pytest.mark.parametrize("counts", [[200] * 9, [1, 0, 63, 64, 65, 130], [0] * 40 + [3] * 200, [3000]])
+@pytest.mark.parametrize("n,k", [(264, 128), (1000, 64), (2056, 16), (72, 120), (513, 1)])
+def test_weight_gradients_of_few_columns(counts, n, k):
+    rows = sum(counts)
+    dy = _randn(rows, (n + 7) // 8 * 8, seed=1)[:, :n]
+    x = _randn(rows, (k + 7) // 8 * 8, seed=2)[:, :k]
+    got = ops.grouped_mm_dw(dy, x, _ends(counts))
+    _close(got, _dw(dy, x, counts), _dw(dy.abs(), x.abs(), counts), max(counts))
+
+
 def test_no_rows():
     w, ends = _randn(3, 64, 32, seed=1), _ends([0, 0, 0])
     x, dy = _randn(0, 32), _randn(0, 64)
