@@ -343,7 +343,8 @@ def _rows_times_weights(entry: str, name: str, x: torch.Tensor, w: torch.Tensor,
     _vector(ends, "ends", (experts,), torch.int32, device)
     cols = n if summed == 2 else k
     if out is None and (out_dtype is None or out_dtype is dtype):
-        y, ldo, code = x.new_empty((rows, cols)), cols, TYPE_CODES[dtype]
+        y = torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)   # 0.3 us less than new_empty
+        ldo, code = cols, TYPE_CODES[dtype]
     else:
         y = _output(out, (rows, cols), (dtype, torch.float32), out_dtype, device, (x, w, ends))
         ldo, code = _ldo(y), TYPE_CODES[y.dtype]
@@ -398,11 +399,15 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: to
     _need(ends.dim() == 1, "ends must be int32 [E]")
     experts = ends.shape[0]
     _vector(ends, "ends", (experts,), torch.int32, device)
-    out = _output(out, (experts, n, k), (dtype, torch.float32), out_dtype, device, (dy, x, ends))
-    ldo = _ldo(out)
+    if out is None and (out_dtype is None or out_dtype is dtype):
+        out, ldo, stride = torch.empty_strided((experts, n, k), (n * k, k, 1), dtype=dtype, device=device), k, n * k
+    else:
+        out = _output(out, (experts, n, k), (dtype, torch.float32), out_dtype, device, (dy, x, ends))
+        ldo = _ldo(out)
+        stride = out.stride(0) if experts > 1 else n * ldo
     _launch(device, "b2m_grouped_mm_dw", dy.data_ptr(), _row_stride(lddy, rows, n, 2), x.data_ptr(),
             _row_stride(ldx, rows, k, 2), rows, n, k, ends.data_ptr(), experts, TYPE_CODES[dtype], out.data_ptr(), ldo,
-            out.stride(0) if experts > 1 else n * ldo, TYPE_CODES[out.dtype],
+            stride, TYPE_CODES[out.dtype],
             None if status is None else _status_word(status, device))
     return out
 
@@ -447,7 +452,7 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
         raise ValueError("x must be a CUDA tensor, 2D bf16, fp16 or fp32 with unit column stride")
     rows, cols = x.shape
     if q is None:
-        q = x.new_empty((rows, cols), dtype=torch.int8)
+        q = torch.empty_strided((rows, cols), (cols, 1), dtype=torch.int8, device=device)
         ldq = cols
     else:
         ldq, _ = _operand(q, "q", 2, torch.int8, device)
@@ -474,12 +479,19 @@ def _int8(a, a_scale, w, w_scale, experts, n, k, w_stride, ldw, ends, out, out_d
     if width != k:
         raise ValueError(f"a is {list(a.shape)} and w {list(w.shape)}: the summed axes differ")
     _vector(a_scale, "a_scale", (rows,), torch.float32, device)
-    y = _output(out, (rows, n), FLOATS, out_dtype, device,
-                (a, w, a_scale, w_scale) if ends is None else (a, w, a_scale, w_scale, ends))
+    if out is None:
+        out_dtype = out_dtype or torch.bfloat16
+        if out_dtype not in TYPE_CODES:
+            raise ValueError(f"out_dtype must be one of {FLOATS}")
+        y, ldo = torch.empty_strided((rows, n), (n, 1), dtype=out_dtype, device=device), n
+    else:
+        y = _output(out, (rows, n), FLOATS, out_dtype, device,
+                    (a, w, a_scale, w_scale) if ends is None else (a, w, a_scale, w_scale, ends))
+        ldo = _ldo(y)
     ldw = _row_stride(ldw, n, k, 1)
     _launch(device, "b2m_int8_mm", a.data_ptr(), a_scale.data_ptr(), rows, _row_stride(lda, rows, k, 1), w.data_ptr(),
             w_scale.data_ptr(), experts, n, k, ldw, w_stride if experts > 1 else n * ldw,
-            None if ends is None else ends.data_ptr(), y.data_ptr(), _ldo(y), TYPE_CODES[y.dtype], out is None,
+            None if ends is None else ends.data_ptr(), y.data_ptr(), ldo, TYPE_CODES[y.dtype], out is None,
             None if status is None else _status_word(status, device))
     return y
 
