@@ -950,12 +950,20 @@ __device__ __forceinline__ void emit_fp32(float* o, int64_t ldo, int n, int m, b
   }
 #pragma unroll
   for (int j = 0; j < 32; ++j) {
+    const float s = kI8 ? __shfl_sync(0xffffffffu, a_scale, j) : 0.0f;
+    if (kI8) v[j] = __int2float_rn(__float_as_int(v[j])) * s * w_scale;
     if (zero) v[j] = 0.0f;
-    if (kI8) {
-      const float s = __shfl_sync(0xffffffffu, a_scale, j);
-      if (!zero) v[j] = __int2float_rn(__float_as_int(v[j])) * s * w_scale;
+  }
+  if (lane < m) {
+    float* d = o + lane;
+    if (n == 32) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j, d += ldo) *d = v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j, d += ldo)
+        if (j < n) *d = v[j];
     }
-    if (j < n && lane < m) o[j * ldo + lane] = v[j];
   }
   __syncwarp();
 }
