@@ -207,6 +207,22 @@ def test_weight_gradients_of_few_columns(counts, n, k):
     _close(got, _dw(dy, x, counts), _dw(dy.abs(), x.abs(), counts), max(counts))
 
 
+@pytest.mark.parametrize("experts", [31, 32, 33, 255, 256, 257, 400])
+def test_many_segments_of_any_length(experts):
+    """Walks in order of length: segments of no row, of few, and of several tiles, in any order."""
+    g = torch.Generator().manual_seed(experts)
+    counts = torch.randint(0, 60, (experts,), generator=g).tolist()
+    for e, c in zip(torch.randperm(experts, generator=g)[:8].tolist(), (0, 0, 31, 32, 257, 511, 700, 1300)):
+        counts[e] = c
+    n, k = 136, 72
+    rows = sum(counts) + 5
+    x, w, ends = _randn(rows, k), _randn(experts, n, k, seed=1), _ends(counts)
+    dy = _randn(rows, n, seed=2)
+    _close(ops.grouped_mm(x, w, ends), _fwd(x, w, counts), _fwd(x.abs(), w.abs(), counts), k)
+    _close(ops.grouped_mm_dx(dy, w, ends), _dx(dy, w, counts), _dx(dy.abs(), w.abs(), counts), n)
+    _close(ops.grouped_mm_dw(x, dy, ends), _dw(x, dy, counts), _dw(x.abs(), dy.abs(), counts), max(counts))
+
+
 def test_no_rows():
     w, ends = _randn(3, 64, 32, seed=1), _ends([0, 0, 0])
     x, dy = _randn(0, 32), _randn(0, 64)
