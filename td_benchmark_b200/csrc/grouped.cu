@@ -508,7 +508,7 @@ __device__ __forceinline__ void feed_tiles(const Params& p, Control<S>* C, int n
         r.sum_rows = min(r.sum_rows - r.k0 * 64, r.k_blocks * 64);
       }
     }
-    const bool last = i * at.stride >= num_tiles;  // no CTA has a tile in this round
+    const bool last = i * at.stride >= num_tiles;  // every CTA has had its last tile
     if (r.e >= 0 || last) {
       if (!mbar_try_wait(&C->taken[s], phase ^ 1) &&
           !wait_on(&C->taken[s], phase ^ 1, p, B2M_STATUS_TIMEOUT_PRODUCER, &C->abort))
