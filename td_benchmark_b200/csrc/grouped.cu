@@ -29,6 +29,7 @@
 
 #include "b2m_common.cuh"
 #include "b2m_host.h"
+#include "pair_ring.cuh"
 
 namespace b2m {
 namespace {
@@ -91,6 +92,14 @@ struct Join<true, kRows> {
   alignas(16) uint32_t part[kRows * kM];
 };
 
+// Of a pair: what the CTAs need to know of each other's copies when a wait has run out.
+template <bool kPair, int kStages>
+struct Ends {};
+template <int kStages>
+struct Ends<true, kStages> {
+  PairRing<kStages> ring;
+};
+
 // One output tile: rows [row0, row0 + cols) of the output (kDw: of expert e's output),
 // columns from m0.  k_blocks == 0: all zero, nothing is multiplied.  e < 0: no tile is left.
 struct alignas(16) Tile {
@@ -126,6 +135,7 @@ struct Control {
   // 32 output rows of 64 columns, for two warps each
   alignas(16) uint8_t staging[S::kSplit ? 1 : S::kEpiWarps / 2][S::kSplit ? 16 : 32 * kStagePitch];
   Join<S::kSplit, S::NT> join;
+  Ends<S::kPair, S::kStages> ends;
 };
 
 // Warps: 0 and 2 feed the ring, 1 issues MMAs, 3 finds tiles, 4 and following write outputs, the
@@ -673,6 +683,7 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
       const bool tail = kMode == kDw && r.sum_rows - kb * 64 < 64;  // the last warp comes between the copies and the MMA
       const uint32_t bar = (tail ? landed0_own : full0_leader) + s * 8;
       if (elect_one()) {
+        if constexpr (S::kPair) C->ends.ring.bytes[s] = tail ? 0 : bytes;
         if (tail) {
           if (rank == 0) mbar_arrive(&C->full[s]);
           mbar_arrive_expect_tx(&C->landed[s], bytes);
@@ -708,7 +719,8 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
   }
   // Before the CTA exits, the copies of the stages still in use have landed: they are when the
   // stage is released.  After a timeout nothing may release it; then this warp waits, again
-  // within the limit, for its last copies themselves (of a pair, the leader for both CTAs').
+  // within the limit, for its last copies themselves.  Those that a pair's leader counts are
+  // settled when both CTAs have stopped (leave_pair).
   const uint32_t first = issued > S::kStages ? issued - S::kStages : 0;
   for (uint32_t i = first; i < issued && alive; ++i)
     if (((i ^ which) & 1) == 0)
@@ -718,9 +730,11 @@ __device__ __forceinline__ void producer(const Maps& maps, const Params& p, uint
     if (((i ^ which) & 1) != 0) continue;
     if (kMode == kDw && (last_tail >> s & 1))
       wait_on(&C->landed[s], (tails >> s & 1) ^ 1, p, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
-    else if (rank == 0)
+    else if (!S::kPair)
       wait_on(&C->full[s], (i / S::kStages) & 1, p, B2M_STATUS_TIMEOUT_DRAIN, nullptr);
   }
+  if constexpr (S::kPair)
+    if ((threadIdx.x & 31) == 0) C->ends.ring.issued[which] = issued;
   __syncwarp();
 }
 
@@ -1194,6 +1208,7 @@ __global__ void __launch_bounds__(threads_of<S>(kMode), S::kResident)
     }
     mbar_init(&C->mma_done, 1);
     C->abort = 0;
+    if constexpr (S::kPair) C->ends.ring.peer_abort = 0;
     fence_mbar_init();
     if (p.rows > 0) {  // without rows nothing is loaded, and kDw has no maps
       tma_prefetch_desc(&maps.cols);
@@ -1236,8 +1251,10 @@ __global__ void __launch_bounds__(threads_of<S>(kMode), S::kResident)
   }
   tc_fence_before();
   __syncthreads();
-  // the leader's MMAs and the copies it counts, or the other parts, are done with this CTA's memory
-  if (S::kPair || S::kSplit) cluster_sync();
+  if constexpr (S::kPair)
+    leave_pair(C->full, &C->ends.ring, C->abort, at.rank, p.timeout_ns, p.status);
+  else if (S::kSplit)
+    cluster_sync();  // the other parts are done with this CTA's memory
   if (warp == 1) {
     tc_fence_after();
     if (S::kPair)
