@@ -51,6 +51,7 @@
 
 #include "b2m_common.cuh"
 #include "b2m_host.h"
+#include "pair_ring.cuh"
 
 namespace b2m {
 namespace {
@@ -701,6 +702,7 @@ struct PairControl {
   uint64_t sempty[SRING];
   uint32_t tmem_base;
   int abort;
+  PairRing<PSTAGES> ring;
   alignas(16) float as[SRING][BM];
   alignas(16) float bs[SRING][4];
   float amax[2][2][BM];
@@ -788,13 +790,17 @@ __device__ __forceinline__ void pair_producer(const CUtensorMap* map_a, const CU
       __syncwarp();
     }
   }
-  // Drain: the leader's full barriers count both CTAs' bytes; the scale ring is local.
+  // Drain: the scale ring is local.  The leader's full barriers count both CTAs' bytes: on the normal
+  // path it waits for them here, after a timeout when both CTAs have stopped (leave_pair).
   if (lane == 0) {
+    C->ring.issued[0] = C->ring.issued[1] = kbg;
+    for (int s = 0; s < PSTAGES; ++s) C->ring.bytes[s] = PSTAGE_BYTES;
     if (cr == 0) {
       const uint32_t first = kbg > PSTAGES ? kbg - PSTAGES : 0;
       for (uint32_t i = first; i < kbg; ++i)
-        mbar_wait(&C->full[i % PSTAGES], (i / PSTAGES) & 1, p.pipe_timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN,
-                  nullptr);
+        if (!mbar_wait(&C->full[i % PSTAGES], (i / PSTAGES) & 1, p.pipe_timeout_ns, p.status, B2M_STATUS_TIMEOUT_DRAIN,
+                       abort))
+          break;
     }
     const uint32_t rfirst = kbg > SRING ? kbg - SRING : 0;
     for (uint32_t i = rfirst; i < kbg; ++i)
@@ -961,6 +967,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
     }
     mbar_init(&C->mma_done, 1);
     C->abort = 0;
+    C->ring.peer_abort = 0;
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
@@ -988,7 +995,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NUM_THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // the leader's MMAs and the peer's epilogue are done with both CTAs' memory
+  leave_pair(C->full, &C->ring, C->abort, cr, p.pipe_timeout_ns, p.status);
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, TMEM_COLS);

@@ -1,6 +1,6 @@
 """How a CTA pair's operand ring ends after a wait's limit: every copy has landed before the memory is given up.
 
-The plan of ``csrc/pair_ring.cuh`` is compiled for the host and run against a model of the ring: two CTAs with two
+The plan of ``csrc/pair_ring.cuh`` is compiled for the host and run against a model of the ring: two CTAs with one or two
 producers each and the leader's MMA warp, which take their steps in any order and stop anywhere, and copies that land
 whenever they like.  No GPU takes part; on one, a wait of these kernels runs out only when something else is broken.
 """
@@ -57,8 +57,8 @@ class Barrier:
 
 
 class Pair:
-    def __init__(self, rng, stages):
-        self.rng, self.stages = rng, stages
+    def __init__(self, rng, stages, producers=2):
+        self.rng, self.stages, self.producers = rng, stages, producers
         self.full = [Barrier() for _ in range(stages)]
         self.empty = [[0] * stages for _ in range(2)]      # stages released, as each CTA knows
         self.released = []                                 # (CTA, stage) on their way
@@ -81,7 +81,9 @@ class Pair:
             self.full[s].change(1, 0 if self.tail[i] else 2 * self.size[i])
         self.bytes[c][s] = 0 if self.tail[i] else self.size[i]
         self.flight.append((c, s, self.bytes[c][s], i))
-        self.issued[c, w], self.next[c, w] = i + 1, i + 2
+        self.next[c, w] = i + self.producers
+        for of in (w, 1) if self.producers == 1 else (w,):      # one producer: its count stands for both kinds of stage
+            self.issued[c, of] = i + 1
         return True
 
     def multiply(self):
@@ -102,7 +104,7 @@ class Pair:
         self.landed[c].add(i)
 
     def run_until_all_stopped(self):
-        actors = [("p", c, w) for c in range(2) for w in range(2)] + [("m",)]
+        actors = [("p", c, w) for c in range(2) for w in range(self.producers)] + [("m",)]
         stop = self.rng.choice([0.01, 0.05, 0.2])
         while actors:
             if self.released and self.rng.random() < 0.5:
@@ -137,11 +139,12 @@ def _settle(ring, plan):
     return True
 
 
+@pytest.mark.parametrize("producers", [1, 2])
 @pytest.mark.parametrize("stages", [2, 4, 6])
-def test_every_copy_lands_wherever_the_ctas_stop(end_of_stage, stages):
+def test_every_copy_lands_wherever_the_ctas_stop(end_of_stage, stages, producers):
     ahead = {"leader": 0, "peer": 0, "even": 0}
     for seed in range(4000):
-        ring = Pair(random.Random(seed), stages)
+        ring = Pair(random.Random(seed), stages, producers)
         ring.run_until_all_stopped()
         for w in range(2):
             lead, peer = ring.issued[LEADER, w], ring.issued[PEER, w]
