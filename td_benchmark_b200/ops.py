@@ -497,17 +497,19 @@ def _int8(a, a_scale, w, w_scale, experts, n, k, w_stride, ldw, ends, out, out_d
 
 
 def int8_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
-            out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+            out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+            status: torch.Tensor | None = None) -> torch.Tensor:
     """8-bit integer product with scales for each token and channel: ``y = (a @ w.T) * a_scale[:, None] * w_scale``.
 
     a int8 [M, K], w int8 [N, K] (``quant_int8`` of the activations and of the weights), a_scale fp32 [M], w_scale
     fp32 [N] -> [M, N] in bf16 (default), fp16 or fp32.  The integer sums are exact (K <= 131071); rows of a and w
-    are a multiple of 16 bytes apart and 16-byte aligned."""
+    are a multiple of 16 bytes apart and 16-byte aligned.  ``status`` (``new_status``) records a wait that ran out of
+    its limit and left the output unfinished."""
     _cuda(a, "a")
     ldw, _ = _operand(w, "w", 2, torch.int8, a.device)
     n, k = w.shape
     _vector(w_scale, "w_scale", (n,), torch.float32, a.device)
-    return _int8(a, a_scale, w, w_scale, 1, n, k, 0, ldw, None, out, out_dtype, None)
+    return _int8(a, a_scale, w, w_scale, 1, n, k, 0, ldw, None, out, out_dtype, status)
 
 
 def int8_grouped_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,

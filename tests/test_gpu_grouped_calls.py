@@ -1,0 +1,48 @@
+"""What the calls of the expert-segment and integer products pass on, refuse and leave alone."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from tests.conftest import cuda_ok  # noqa: E402
+
+if not cuda_ok():
+    pytest.skip("needs an sm_100 GPU", allow_module_level=True)
+
+from td_benchmark_b200 import ops  # noqa: E402
+
+DEV = torch.device("cuda", 0)
+
+
+def _randn(*shape, seed=0, dtype=torch.bfloat16):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(DEV)
+
+
+def _ends(counts):
+    return torch.tensor(counts, dtype=torch.int64).cumsum(0).to(torch.int32).to(DEV)
+
+
+@pytest.fixture()
+def launches(monkeypatch):
+    """(entry, status pointer) of every launch; the status is the last argument before the stream."""
+    seen, launch = [], ops._launch
+    monkeypatch.setattr(ops, "_launch",
+                        lambda device, name, *args: seen.append((name, args[-1])) or launch(device, name, *args))
+    return seen
+
+
+# ---------------------------------------------------------------- status words
+def test_status_reaches_every_entry(launches):
+    x, w, ends, dy = _randn(6, 64), _randn(2, 32, 64, seed=1), _ends([4, 2]), _randn(6, 32, seed=2)
+    status = ops.new_status(DEV)
+    q, s = ops.quant_int8(x, status=status)
+    wq, sw = ops.quant_int8(w.view(-1, 64), status=status)
+    ops.grouped_mm(x, w, ends, status=status)
+    ops.grouped_mm_dx(dy, w, ends, status=status)
+    ops.grouped_mm_dw(dy, x, ends, status=status)
+    ops.int8_mm(q, s, wq, sw, status=status)
+    ops.int8_grouped_mm(q, s, wq.view(2, 32, 64), sw.view(2, 32), ends, status=status)
+    assert len(launches) == 7 and all(at == status.data_ptr() for _, at in launches), launches
+    ops.check_status(status)
+    with pytest.raises(ValueError, match="status"):
+        ops.int8_mm(q, s, wq, sw, status=torch.zeros(1, device=DEV))

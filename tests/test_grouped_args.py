@@ -91,3 +91,14 @@ def test_wrappers_refuse_host_tensors_and_wrong_shapes():
                  lambda: ops.int8_grouped_mm(a, s, a.view(2, 2, 64), s, ends)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
+
+
+@pytest.mark.parametrize("name", ["grouped_mm", "grouped_mm_dx", "grouped_mm_dw", "quant_int8", "int8_mm",
+                                  "int8_grouped_mm"])
+def test_every_wrapper_takes_a_status_word(name):
+    """A wait that runs out is reported there and nowhere else."""
+    import inspect
+
+    from td_benchmark_b200 import ops
+
+    assert inspect.signature(getattr(ops, name)).parameters["status"].default is None
