@@ -363,7 +363,8 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.
     segments allowed, E <= 1024) -> [T, N] of the input type or fp32.  No segment is padded and nothing is read back
     to the host.  Rows behind ``ends[-1]`` are zero in an output allocated here and left alone in ``out``.  Rows of x
     and w are a multiple of 16 bytes apart and 16-byte aligned.  ``status`` (``new_status``) records ends that are
-    out of order, which are otherwise taken as the nearest ones in order.
+    out of order, which are otherwise taken as the nearest ones in order, and waits that ran out of their limit and left
+    the output unfinished; a backward pass records both in the same word.
 
     Differentiable in x and w without ``out`` and ``out_dtype``; a weight gradient covers every expert (zero where a
     segment is empty).  As with any autograd function, a backward pass is captured into a CUDA graph only when no
@@ -427,6 +428,7 @@ class _GroupedMM(torch.autograd.Function):
     def forward(ctx, x, w, ends, status):
         y = grouped_mm(x.detach(), w.detach(), ends, status=status)
         ctx.save_for_backward(x, w, ends)
+        ctx.status = status          # not among the saved tensors: the kernels may write to it
         return y
 
     @staticmethod
@@ -434,8 +436,8 @@ class _GroupedMM(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, ends = ctx.saved_tensors
         dy = _kernel_rows(dy)
-        dx = grouped_mm_dx(dy, w, ends) if ctx.needs_input_grad[0] else None
-        dw = grouped_mm_dw(dy, x, ends) if ctx.needs_input_grad[1] else None
+        dx = grouped_mm_dx(dy, w, ends, status=ctx.status) if ctx.needs_input_grad[0] else None
+        dw = grouped_mm_dw(dy, x, ends, status=ctx.status) if ctx.needs_input_grad[1] else None
         return dx, dw, None, None
 
 

@@ -46,3 +46,20 @@ def test_status_reaches_every_entry(launches):
     ops.check_status(status)
     with pytest.raises(ValueError, match="status"):
         ops.int8_mm(q, s, wq, sw, status=torch.zeros(1, device=DEV))
+
+
+def test_status_of_the_forward_reaches_the_backward(launches):
+    x, w = _randn(6, 64).requires_grad_(), _randn(2, 32, 64, seed=1).requires_grad_()
+    status = ops.new_status(DEV)
+    y = ops.grouped_mm(x, w, _ends([4, 2]), status=status)
+    y.backward(torch.ones_like(y))
+    assert [name for name, _ in launches] == ["b2m_grouped_mm", "b2m_grouped_mm_dx", "b2m_grouped_mm_dw"]
+    assert all(at == status.data_ptr() for _, at in launches)
+    ops.check_status(status)
+    # ends that are out of order by the time of the backward pass: what it finds is recorded
+    ends = _ends([4, 2])
+    y = ops.grouped_mm(x, w, ends, status=status)
+    ends.data.copy_(torch.tensor([7, 6]))
+    y.backward(torch.ones_like(y))
+    with pytest.raises(RuntimeError, match="BAD_ROUTING"):
+        ops.check_status(status)
