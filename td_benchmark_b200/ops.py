@@ -260,6 +260,13 @@ TYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 FLOATS = (torch.bfloat16, torch.float16, torch.float32)
 
 
+def _no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse tensors whose gradient the call would drop: it returns, or writes, values that no graph leads to."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what} is not differentiable: call it with detached tensors or under torch.no_grad()")
+
+
 def _launch(device: torch.device, name: str, *args) -> None:
     """The C call on the tensors' device and its current stream."""
     index = device.index
@@ -372,13 +379,16 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         _need(out is None and out_dtype in (None, x.dtype), "gradients need out=None and the input's type as out_dtype")
         return _GroupedMM.apply(x, w, ends, status)
+    _no_gradient("grouped_mm into out", out)
     return _rows_times_weights("b2m_grouped_mm", "x", x, w, ends, 2, out, out_dtype, status)
 
 
 def grouped_mm_dx(dy: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.Tensor | None = None,
                   out_dtype: torch.dtype | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """Gradient of ``grouped_mm``'s rows: ``dx[t] = dy[t] @ w[e]``.  dy [T, N], w [E, N, K] -> [T, K]; types, strides,
-    ends, status and the rows behind ``ends[-1]`` as there."""
+    ends, status and the rows behind ``ends[-1]`` as there.  Not differentiable itself: tensors that require gradients
+    are refused."""
+    _no_gradient("grouped_mm_dx", dy, w, out)
     return _rows_times_weights("b2m_grouped_mm_dx", "dy", dy, w, ends, 1, out, out_dtype, status)
 
 
@@ -387,7 +397,9 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: to
     """Gradient of ``grouped_mm``'s weights: ``dw[e] = dy[seg e].T @ x[seg e]``, zero for an empty segment.
 
     dy [T, N], x [T, K] -> [E, N, K] of the input type or fp32; types, strides, ends and status as there.  Rows behind
-    ``ends[-1]`` enter no sum, whatever they hold."""
+    ``ends[-1]`` enter no sum, whatever they hold.  Not differentiable itself: tensors that require gradients are
+    refused."""
+    _no_gradient("grouped_mm_dw", dy, x, out)
     dtype, device = dy.dtype, dy.device
     if not dy.is_cuda or (dtype is not torch.bfloat16 and dtype is not torch.float16):
         raise ValueError("dy must be a CUDA tensor, bf16 or fp16")
@@ -447,7 +459,9 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
     ``q = rne(x / scale)`` within +-127, both divisions IEEE fp32.
 
     Token codes of activations, or channel codes of weights (one row for each output channel).  A row that holds a
-    NaN (an infinity) gets a NaN (infinite) scale, and a product with it becomes NaN."""
+    NaN (an infinity) gets a NaN (infinite) scale, and a product with it becomes NaN.  Not differentiable: an x that
+    requires gradients is refused."""
+    _no_gradient("quant_int8", x, scale)
     code, device = TYPE_CODES.get(x.dtype), x.device
     strides = x.stride()
     if not x.is_cuda or code is None or len(strides) != 2 or (strides[1] != 1 and x.shape[1] > 1):
@@ -475,6 +489,7 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
 
 
 def _int8(a, a_scale, w, w_scale, experts, n, k, w_stride, ldw, ends, out, out_dtype, status):
+    _no_gradient("int8_mm" if ends is None else "int8_grouped_mm", a_scale, w_scale, out)
     device = a.device
     lda, _ = _operand(a, "a", 2, torch.int8, device)
     rows, width = a.shape
@@ -506,7 +521,7 @@ def int8_mm(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: to
     a int8 [M, K], w int8 [N, K] (``quant_int8`` of the activations and of the weights), a_scale fp32 [M], w_scale
     fp32 [N] -> [M, N] in bf16 (default), fp16 or fp32.  The integer sums are exact (K <= 131071); rows of a and w
     are a multiple of 16 bytes apart and 16-byte aligned.  ``status`` (``new_status``) records a wait that ran out of
-    its limit and left the output unfinished."""
+    its limit and left the output unfinished.  Not differentiable: scales that require gradients are refused."""
     _cuda(a, "a")
     ldw, _ = _operand(w, "w", 2, torch.int8, a.device)
     n, k = w.shape

@@ -63,3 +63,43 @@ def test_status_of_the_forward_reaches_the_backward(launches):
     y.backward(torch.ones_like(y))
     with pytest.raises(RuntimeError, match="BAD_ROUTING"):
         ops.check_status(status)
+
+
+# ---------------------------------------------------------------- derivatives that a call would drop
+def _all_calls():
+    """name -> (call of its float inputs and out, those inputs, an output)."""
+    x, w, ends, dy = _randn(6, 64), _randn(2, 32, 64, seed=1), _ends([4, 2]), _randn(6, 32, seed=2)
+    q, s = ops.quant_int8(x)
+    wq, sw = ops.quant_int8(w.view(-1, 64))
+    w3, sw3 = wq.view(2, 32, 64), sw.view(2, 32)
+    new = lambda *shape: torch.empty(shape, device=DEV, dtype=torch.bfloat16)  # noqa: E731
+    return {
+        "grouped_mm_dx": (lambda a, b, o=None: ops.grouped_mm_dx(a, b, ends, out=o), (dy, w), new(6, 64)),
+        "grouped_mm_dw": (lambda a, b, o=None: ops.grouped_mm_dw(a, b, ends, out=o), (dy, x), new(2, 32, 64)),
+        "quant_int8": (lambda a, o=None: ops.quant_int8(a, scale=o)[1], (x,), torch.empty(6, device=DEV)),
+        "int8_mm": (lambda a, b, o=None: ops.int8_mm(q, a, wq, b, out=o), (s, sw), new(6, 64)),
+        "int8_grouped_mm": (lambda a, b, o=None: ops.int8_grouped_mm(q, a, w3, b, ends, out=o), (s, sw3), new(6, 32)),
+        "grouped_mm": (lambda a, b, o=None: ops.grouped_mm(a, b, ends, out=o), (x, w), new(6, 32)),
+    }
+
+
+@pytest.mark.parametrize("name", ["grouped_mm_dx", "grouped_mm_dw", "quant_int8", "int8_mm", "int8_grouped_mm",
+                                  "grouped_mm"])
+def test_gradients_are_not_dropped(name):
+    call, inputs, out = _all_calls()[name]
+    want = call(*inputs)
+    for i in range(len(inputs)):
+        held = [t.detach().clone().requires_grad_(i == j) for j, t in enumerate(inputs)]
+        if name == "grouped_mm":
+            assert call(*held).requires_grad
+        else:
+            with pytest.raises(ValueError, match=f"{name} is not differentiable"):
+                call(*held)
+            assert torch.equal(call(*(t.detach() for t in held)), want)
+        with torch.no_grad():
+            got = call(*held)
+        assert torch.equal(got, want) and not got.requires_grad
+    with pytest.raises(ValueError, match="not differentiable"):
+        call(*inputs, out.requires_grad_())
+    with torch.no_grad():
+        assert torch.equal(call(*inputs, out), want)
