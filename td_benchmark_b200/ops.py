@@ -7,6 +7,7 @@ pre-allocates everything once); when omitted they are allocated here.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -265,6 +266,14 @@ def _no_gradient(what: str, *tensors: torch.Tensor | None) -> None:
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what} is not differentiable: call it with detached tensors or under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        _no_tangent(what, *tensors)
+
+
+def _no_tangent(what: str, *tensors: torch.Tensor | None) -> None:
+    """The same for forward-mode derivatives, whose tensors do not say that they require gradients."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no forward-mode derivative")
 
 
 def _launch(device: torch.device, name: str, *args) -> None:
@@ -373,9 +382,11 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.
     out of order, which are otherwise taken as the nearest ones in order, and waits that ran out of their limit and left
     the output unfinished; a backward pass records both in the same word.
 
-    Differentiable in x and w without ``out`` and ``out_dtype``; a weight gradient covers every expert (zero where a
+    Differentiable (in reverse mode, once) in x and w without ``out`` and ``out_dtype``; a weight gradient covers every expert (zero where a
     segment is empty).  As with any autograd function, a backward pass is captured into a CUDA graph only when no
     graph of the same leaves that was recorded outside the capture is still alive."""
+    if forward_ad._current_level >= 0:
+        _no_tangent("grouped_mm", x, w)
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         _need(out is None and out_dtype in (None, x.dtype), "gradients need out=None and the input's type as out_dtype")
         return _GroupedMM.apply(x, w, ends, status)

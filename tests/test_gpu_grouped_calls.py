@@ -9,6 +9,8 @@ from tests.conftest import cuda_ok  # noqa: E402
 if not cuda_ok():
     pytest.skip("needs an sm_100 GPU", allow_module_level=True)
 
+import torch.autograd.forward_ad as forward_ad  # noqa: E402
+
 from td_benchmark_b200 import ops  # noqa: E402
 
 DEV = torch.device("cuda", 0)
@@ -83,8 +85,10 @@ def _all_calls():
     }
 
 
-@pytest.mark.parametrize("name", ["grouped_mm_dx", "grouped_mm_dw", "quant_int8", "int8_mm", "int8_grouped_mm",
-                                  "grouped_mm"])
+NAMES = ["grouped_mm_dx", "grouped_mm_dw", "quant_int8", "int8_mm", "int8_grouped_mm", "grouped_mm"]
+
+
+@pytest.mark.parametrize("name", NAMES)
 def test_gradients_are_not_dropped(name):
     call, inputs, out = _all_calls()[name]
     want = call(*inputs)
@@ -103,3 +107,29 @@ def test_gradients_are_not_dropped(name):
         call(*inputs, out.requires_grad_())
     with torch.no_grad():
         assert torch.equal(call(*inputs, out), want)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_are_not_dropped(name):
+    call, inputs, out = _all_calls()[name]
+    want = call(*inputs)
+    with forward_ad.dual_level():
+        for i, t in enumerate(inputs):
+            dual = [forward_ad.make_dual(u, torch.ones_like(u)) if i == j else u for j, u in enumerate(inputs)]
+            with pytest.raises(ValueError, match=f"{name} has no forward-mode derivative"):
+                call(*dual)
+        with pytest.raises(ValueError, match="no forward-mode derivative"):
+            call(*inputs, forward_ad.make_dual(out, torch.ones_like(out)))
+        assert torch.equal(call(*inputs), want)              # nothing carries a tangent
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_function_transforms_are_refused(name):
+    """Batched and differentiated tensors of torch.func have no memory of their own: every call says so."""
+    call, inputs, _ = _all_calls()[name]
+    first, rest = inputs[0], inputs[1:]
+    total = lambda t: call(t, *rest).float().sum()  # noqa: E731
+    for run in (lambda: torch.func.vmap(lambda t: call(t, *rest))(first[None]), lambda: torch.func.grad(total)(first),
+                lambda: torch.func.jvp(total, (first,), (first,))):
+        with pytest.raises((RuntimeError, ValueError)):
+            run()
