@@ -276,8 +276,15 @@ def _no_tangent(what: str, *tensors: torch.Tensor | None) -> None:
         raise ValueError(f"{what} has no forward-mode derivative")
 
 
+def _recording() -> bool:
+    """Whether torch.fx records the operations of real tensors (of tensors without memory, data_ptr raises)."""
+    return torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None
+
+
 def _launch(device: torch.device, name: str, *args) -> None:
     """The C call on the tensors' device and its current stream."""
+    if torch._C._is_tracing() or (torch._C._len_torch_dispatch_stack() and _recording()):
+        raise RuntimeError(f"{name}: a trace would keep the output's allocation and lose the kernel")
     index = device.index
     if index == torch._C._cuda_getDevice():
         _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))

@@ -133,3 +133,32 @@ def test_function_transforms_are_refused(name):
                 lambda: torch.func.jvp(total, (first,), (first,))):
         with pytest.raises((RuntimeError, ValueError)):
             run()
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.filterwarnings("ignore::DeprecationWarning", "ignore::torch.jit.TracerWarning")
+def test_traces_are_refused(name):
+    """A recorded graph would hold an allocation that nothing writes to."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    call, inputs, _ = _all_calls()[name]
+    one = lambda t: call(t, *inputs[1:])  # noqa: E731
+    for record in (lambda: torch.jit.trace(one, inputs[0], check_trace=False), lambda: make_fx(one)(inputs[0]),
+                   lambda: make_fx(one, tracing_mode="fake")(inputs[0])):
+        with pytest.raises(RuntimeError, match="trace|data pointer"):
+            record()
+
+
+def test_compiled_callers_and_dispatch_modes_work():
+    """torch.compile leaves the calls out of its graphs, and modes that only watch do not matter."""
+    from torch.utils.flop_counter import FlopCounterMode
+
+    call, inputs, _ = _all_calls()["grouped_mm"]
+    want = call(*inputs)
+    compiled = torch.compile(lambda a, b: call(a * 1, b) * 1, backend="aot_eager")
+    assert torch.equal(compiled(*inputs), want)
+    with FlopCounterMode(display=False):
+        assert torch.equal(call(*inputs), want)
+    x = inputs[0].clone().requires_grad_()
+    dy = torch.ones_like(want)
+    assert torch.equal(torch.autograd.grad(compiled(x, inputs[1]), x, dy)[0], torch.autograd.grad(call(x, inputs[1]), x, dy)[0])
