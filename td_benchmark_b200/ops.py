@@ -331,6 +331,21 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors share no byte: one lies behind the other, or they are parts of rows (or of other runs) that
+    repeat at the same distance, as the halves of one buffer's columns are."""
+    (lo, hi), (start, stop) = _extent(a), _extent(b)
+    if hi <= start or stop <= lo:
+        return True
+    axes = [[(n, s * t.element_size()) for n, s in zip(t.shape, t.stride()) if n > 1 and s > 0] for t in (a, b)]
+    for pitch in {s for of in axes for _, s in of}:
+        first, second = (t.element_size() + sum((n - 1) * s for n, s in of if s % pitch) for t, of in zip((a, b), axes))
+        at = (start - lo) % pitch                    # b's run behind a's, within a pitch
+        if first <= at and at + second <= pitch:
+            return True
+    return False
+
+
 def _output(out: torch.Tensor | None, shape: tuple, dtypes: tuple, out_dtype: torch.dtype | None,
             device: torch.device, inputs: tuple) -> torch.Tensor:
     """``out`` checked, or a new tensor.  inputs: the tensors that it must not overlap, the first one on its device."""
@@ -343,10 +358,8 @@ def _output(out: torch.Tensor | None, shape: tuple, dtypes: tuple, out_dtype: to
     _need(tuple(out.shape) == shape and out.dtype in dtypes and out.device == device and
           (shape[-1] <= 1 or out.stride(-1) == 1),
           f"out must be {list(shape)} of {list(dtypes)} on {device} with unit stride along its last axis")
-    lo, hi = _extent(out)
     for t in inputs:
-        a, b = _extent(t)
-        _need(hi <= a or b <= lo, "out overlaps an input")
+        _need(_apart(out, t), "out overlaps an input")
     return out
 
 
@@ -384,14 +397,15 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor, out: torch.
 
     x bf16 / fp16 [T, K], w the same type [E, N, K], ends int32 [E] on the device (cumulative row counts; empty
     segments allowed, E <= 1024) -> [T, N] of the input type or fp32.  No segment is padded and nothing is read back
-    to the host.  Rows behind ``ends[-1]`` are zero in an output allocated here and left alone in ``out``.  Rows of x
-    and w are a multiple of 16 bytes apart and 16-byte aligned.  ``status`` (``new_status``) records ends that are
-    out of order, which are otherwise taken as the nearest ones in order, and waits that ran out of their limit and left
-    the output unfinished; a backward pass records both in the same word.
+    to the host.  Rows behind ``ends[-1]`` are zero in an output allocated here and left alone in ``out``, which may
+    lie beside an input in one buffer (columns next to its columns) but not on it.  Rows of x and w are a multiple of
+    16 bytes apart and 16-byte aligned.  ``status`` (``new_status``) records ends that are out of order, which are
+    otherwise taken as the nearest ones in order, and waits that ran out of their limit and left the output
+    unfinished; a backward pass records both in the same word.
 
-    Differentiable (in reverse mode, once) in x and w without ``out`` and ``out_dtype``; a weight gradient covers every expert (zero where a
-    segment is empty).  As with any autograd function, a backward pass is captured into a CUDA graph only when no
-    graph of the same leaves that was recorded outside the capture is still alive."""
+    Differentiable (in reverse mode, once) in x and w without ``out`` and ``out_dtype``; a weight gradient covers every
+    expert (zero where a segment is empty).  As with any autograd function, a backward pass is captured into a CUDA
+    graph only when no graph of the same leaves that was recorded outside the capture is still alive."""
     if forward_ad._current_level >= 0:
         _no_tangent("grouped_mm", x, w)
     if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
@@ -492,15 +506,12 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
         ldq, _ = _operand(q, "q", 2, torch.int8, device)
         ldq = ldq if rows > 1 else cols
         _need(tuple(q.shape) == (rows, cols) and ldq >= cols, "bad q buffer")
-        (lo, hi), (a, b) = _extent(q), _extent(x)
-        _need(hi <= a or b <= lo, "q overlaps x")
+        _need(_apart(q, x), "q overlaps x")
     if scale is None:
         scale = x.new_empty(rows, dtype=torch.float32)
     else:
         _vector(scale, "scale", (rows,), torch.float32, device)
-        lo, hi = _extent(scale)
-        for a, b in (_extent(x), _extent(q)):
-            _need(hi <= a or b <= lo, "scale overlaps x or q")
+        _need(_apart(scale, x) and _apart(scale, q), "scale overlaps x or q")
     _launch(device, "b2m_quant_i8", x.data_ptr(), code, rows, cols, strides[0] if rows > 1 else cols, q.data_ptr(), ldq,
             scale.data_ptr(), None if status is None else _status_word(status, device))
     return q, scale

@@ -162,3 +162,44 @@ def test_compiled_callers_and_dispatch_modes_work():
     x = inputs[0].clone().requires_grad_()
     dy = torch.ones_like(want)
     assert torch.equal(torch.autograd.grad(compiled(x, inputs[1]), x, dy)[0], torch.autograd.grad(call(x, inputs[1]), x, dy)[0])
+
+
+# ---------------------------------------------------------------- outputs beside an input
+@pytest.mark.parametrize("rows,n,k", [(6, 32, 64), (300, 264, 136), (1, 8, 16)])
+def test_outputs_beside_an_input_in_one_buffer(rows, n, k):
+    """Columns next to an input's columns are an output like any other; nothing else of the buffer changes."""
+    counts = [rows - rows // 3, rows // 3]
+    ends, w = _ends(counts), _randn(2, n, k, seed=1)
+    buf = torch.full((rows, k + n + 24), 7.0, device=DEV, dtype=torch.bfloat16)
+    x, out, dy = buf[:, :k], buf[:, k + 8:k + 8 + n], _randn(rows, n, seed=2)
+    x.copy_(_randn(rows, k, seed=3))
+    plain, kept = x.clone(), x.clone()
+    assert torch.equal(ops.grouped_mm(x, w, ends, out=out), ops.grouped_mm(plain, w, ends))
+    assert torch.equal(x, kept) and (buf[:, k:k + 8] == 7).all() and (buf[:, k + 8 + n:] == 7).all()
+    # dx beside dy
+    both = torch.full((rows, n + k), 7.0, device=DEV, dtype=torch.bfloat16)
+    both[:, :n] = dy
+    assert torch.equal(ops.grouped_mm_dx(both[:, :n], w, ends, out=both[:, n:]), ops.grouped_mm_dx(dy, w, ends))
+    assert torch.equal(both[:, :n], dy)
+    for bad in (buf[:, k - 1:k - 1 + n], buf[:, :n]):
+        with pytest.raises(ValueError, match="overlaps"):
+            ops.grouped_mm(x, w, ends, out=bad)
+
+
+@pytest.mark.parametrize("rows,n,k", [(6, 32, 64), (300, 264, 144), (1, 8, 16)])
+def test_integer_outputs_beside_an_input_in_one_buffer(rows, n, k):
+    """Codes beside their rows, and integer products beside the codes."""
+    ends, w = _ends([rows - rows // 3, rows // 3]), _randn(2 * n, k, seed=1)
+    plain = _randn(rows, k, seed=3)
+    want, want_s = ops.quant_int8(plain)
+    buf = torch.full((rows, 2 * k + 8), 7.0, device=DEV, dtype=torch.bfloat16)
+    buf[:, :k] = plain
+    q, s = ops.quant_int8(buf[:, :k], q=buf.view(torch.int8)[:, 2 * k + 16:3 * k + 16])
+    assert torch.equal(q, want) and torch.equal(s, want_s) and torch.equal(buf[:, :k], plain)
+    wq, sw = ops.quant_int8(w)
+    wide = torch.full((rows, k + 4 * n), 5, device=DEV, dtype=torch.int8)
+    wide[:, :k] = want
+    got = ops.int8_grouped_mm(wide[:, :k], s, wq.view(2, n, k), sw.view(2, n), ends,
+                              out=wide[:, k:].view(torch.float32))
+    assert torch.equal(got, ops.int8_grouped_mm(want, s, wq.view(2, n, k), sw.view(2, n), ends, out_dtype=torch.float32))
+    assert torch.equal(wide[:, :k], want)

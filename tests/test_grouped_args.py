@@ -102,3 +102,42 @@ def test_every_wrapper_takes_a_status_word(name):
     from td_benchmark_b200 import ops
 
     assert inspect.signature(getattr(ops, name)).parameters["status"].default is None
+
+
+def _bytes_of(t):
+    import itertools
+
+    at = {sum(i * s for i, s in zip(index, t.stride())) for index in itertools.product(*map(range, t.shape))}
+    return {t.data_ptr() + i * t.element_size() + b for i in at for b in range(t.element_size())}
+
+
+def test_tensors_that_share_no_byte():
+    """Never called apart when they share one, and called apart when they are parts of one buffer's rows."""
+    import random
+
+    import torch
+
+    from td_benchmark_b200 import ops
+
+    buf = torch.zeros((6, 40), dtype=torch.bfloat16)
+    cube = torch.zeros((3, 8, 20), dtype=torch.bfloat16)
+    for a, b in [(buf[:, :16], buf[:, 16:]), (buf[:, 24:], buf[1:4, 8:24]), (buf[0], buf[2:]), (buf[:3], buf[3:]),
+                 (cube[:, :4], cube[:, 4:]), (cube[..., :8], cube[..., 8:16]), (buf[:, :8], buf.view(torch.int8)[:, 64:]),
+                 (buf[::2], buf[1::2]), (buf[:, :0], buf)]:
+        assert ops._apart(a, b) and ops._apart(b, a) and not _bytes_of(a) & _bytes_of(b)
+    for a, b in [(buf, buf), (buf[:, :17], buf[:, 16:]), (buf[:3], buf[2:]), (buf.view(-1)[:4], buf), (buf[0], buf[:1]),
+                 (cube[0], cube[:, 4]), (buf[:1].expand(6, 40), buf[:, 39:])]:
+        assert not ops._apart(a, b) and not ops._apart(b, a)
+    rng = random.Random(1)
+    flat, apart = torch.zeros(120, dtype=torch.int16), 0
+    for _ in range(3000):
+        views = []
+        for _ in range(2):
+            shape = [rng.randrange(1, 4) for _ in range(rng.randrange(1, 4))]
+            strides = [rng.choice([0, 1, 2, 5, 8, 10, 16, 20]) for _ in shape[1:]] + [1]
+            room = 119 - sum((n - 1) * s for n, s in zip(shape, strides))
+            views.append(flat.as_strided(shape, strides, rng.randrange(0, room)))
+        if ops._apart(*views):
+            apart += 1
+            assert not _bytes_of(views[0]) & _bytes_of(views[1]), views
+    assert apart > 500
