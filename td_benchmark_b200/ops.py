@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -360,6 +361,7 @@ def _output(out: torch.Tensor | None, shape: tuple, dtypes: tuple, out_dtype: to
           f"out must be {list(shape)} of {list(dtypes)} on {device} with unit stride along its last axis")
     for t in inputs:
         _need(_apart(out, t), "out overlaps an input")
+    increment_version(out)          # a graph that saved its old values must not use the new ones
     return out
 
 
@@ -507,11 +509,13 @@ def quant_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tens
         ldq = ldq if rows > 1 else cols
         _need(tuple(q.shape) == (rows, cols) and ldq >= cols, "bad q buffer")
         _need(_apart(q, x), "q overlaps x")
+        increment_version(q)
     if scale is None:
         scale = x.new_empty(rows, dtype=torch.float32)
     else:
         _vector(scale, "scale", (rows,), torch.float32, device)
         _need(_apart(scale, x) and _apart(scale, q), "scale overlaps x or q")
+        increment_version(scale)
     _launch(device, "b2m_quant_i8", x.data_ptr(), code, rows, cols, strides[0] if rows > 1 else cols, q.data_ptr(), ldq,
             scale.data_ptr(), None if status is None else _status_word(status, device))
     return q, scale

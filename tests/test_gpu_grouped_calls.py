@@ -203,3 +203,26 @@ def test_integer_outputs_beside_an_input_in_one_buffer(rows, n, k):
                               out=wide[:, k:].view(torch.float32))
     assert torch.equal(got, ops.int8_grouped_mm(want, s, wq.view(2, n, k), sw.view(2, n), ends, out_dtype=torch.float32))
     assert torch.equal(wide[:, :k], want)
+
+
+# ---------------------------------------------------------------- outputs that a graph has saved
+@pytest.mark.parametrize("name", NAMES)
+def test_a_graph_notices_that_its_saved_values_were_overwritten(name):
+    call, inputs, out = _all_calls()[name]
+    v = torch.ones(out.shape, device=DEV, dtype=out.dtype, requires_grad=True)
+    loss = (out * v).sum()                                   # saves out for v's gradient
+    loss.backward(retain_graph=True)
+    call(*inputs, out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():                             # tensors without a version
+        kept = torch.empty_like(out)
+        assert torch.equal(call(*inputs, kept), out)
+
+
+def test_codes_count_as_modified_too():
+    x = _randn(6, 64)
+    q = torch.zeros((6, 64), device=DEV, dtype=torch.int8)
+    before = q._version
+    ops.quant_int8(x, q=q)
+    assert q._version > before
