@@ -25,6 +25,7 @@ int require_sm100(int* num_sms);
 int driver_entry(const char* name, void** fn);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 }  // namespace b2m
 

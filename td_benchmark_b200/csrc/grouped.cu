@@ -1407,6 +1407,14 @@ int check_out(const char* what, const void* out, int64_t cols, int64_t ldo, int3
   return B2M_OK;
 }
 
+// What the kernels read or write as 32-bit words; any of them may be null here.
+int check_words(const char* what, const int32_t* ends, const int32_t* status, const float* a_scale = nullptr,
+                const float* w_scale = nullptr) {
+  if (!aligned4(ends) || !aligned4(status) || !aligned4(a_scale) || !aligned4(w_scale))
+    return fail(B2M_ERR_ARG, "%s: ends, scales and status must be 4-byte aligned", what);
+  return B2M_OK;
+}
+
 // kFwd and kDx: `rows` (x, dy or integer codes) times each segment's weights.
 template <int kMode, bool kI8>
 int rows_times_weights(const char* what, const Matrix& x, const Weights& w, const int32_t* ends, int32_t in_type,
@@ -1524,6 +1532,7 @@ extern "C" int b2m_grouped_mm(const void* x, int64_t rows, int64_t ldx, const vo
   B2M_TRY(check_weights("grouped_mm", mw, 2));
   B2M_TRY(check_matrix("grouped_mm", "x", mx, 2));
   if (!ends) return fail(B2M_ERR_ARG, "grouped_mm: null ends");
+  B2M_TRY(check_words("grouped_mm", ends, dev_status));
   if (rows > 0) B2M_TRY(check_out("grouped_mm", out, n, ldo, out_type, in_type));
   return rows_times_weights<kFwd, false>("grouped_mm", mx, mw, ends, in_type, out, ldo, out_type, clear_rest, nullptr,
                                          nullptr, dev_status, stream);
@@ -1539,6 +1548,7 @@ extern "C" int b2m_grouped_mm_dx(const void* dy, int64_t rows, int64_t lddy, con
   B2M_TRY(check_weights("grouped_mm_dx", mw, 2));
   B2M_TRY(check_matrix("grouped_mm_dx", "dy", mdy, 2));
   if (!ends) return fail(B2M_ERR_ARG, "grouped_mm_dx: null ends");
+  B2M_TRY(check_words("grouped_mm_dx", ends, dev_status));
   if (rows > 0) B2M_TRY(check_out("grouped_mm_dx", out, k, ldo, out_type, in_type));
   return rows_times_weights<kDx, false>("grouped_mm_dx", mdy, mw, ends, in_type, out, ldo, out_type, clear_rest,
                                         nullptr, nullptr, dev_status, stream);
@@ -1556,6 +1566,7 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   if (experts < 1 || experts > kMaxExperts)
     return fail(B2M_ERR_ARG, "%s: need 1 <= experts <= %d (%d)", what, kMaxExperts, experts);
   if (!ends) return fail(B2M_ERR_ARG, "%s: null ends", what);
+  B2M_TRY(check_words(what, ends, dev_status));
   B2M_TRY(check_out(what, out, k, ldo, out_type, in_type));
   if (out_stride < (n - 1) * ldo + k) return fail(B2M_ERR_ARG, "%s: experts of the output overlap", what);
   Params p{};
@@ -1626,6 +1637,7 @@ extern "C" int b2m_int8_mm(const void* a, const float* a_scale, int64_t rows, in
   B2M_TRY(check_matrix("int8_mm", "a", ma, 1));
   if (k > 131071) return fail(B2M_ERR_ARG, "int8_mm: k=%lld; sums of more than 131071 products can pass 32 bits", (long long)k);
   if (!w_scale || (rows > 0 && !a_scale)) return fail(B2M_ERR_ARG, "int8_mm: null scales");
+  B2M_TRY(check_words("int8_mm", ends, dev_status, a_scale, w_scale));
   if (!ends && experts != 1) return fail(B2M_ERR_ARG, "int8_mm: ends may be null for one expert only");
   if (out_type != B2M_BF16 && out_type != B2M_FP16 && out_type != B2M_FP32)
     return fail(B2M_ERR_ARG, "int8_mm: unknown output type %d", out_type);

@@ -380,6 +380,8 @@ extern "C" int b2m_quant_i8(const void* x, int32_t in_type, int64_t rows, int64_
   if (rows > 0 && (!x || !q || !scale)) return fail(B2M_ERR_ARG, "quant_i8: null pointer");
   if (reinterpret_cast<uintptr_t>(x) % (in_type == B2M_FP32 ? 4 : 2))
     return fail(B2M_ERR_ARG, "quant_i8: misaligned input");
+  if (!aligned4(scale) || !aligned4(dev_status))
+    return fail(B2M_ERR_ARG, "quant_i8: scale and status must be 4-byte aligned");
   int num_sms = 0;
   B2M_TRY(require_sm100(&num_sms));
   if (rows == 0) return B2M_OK;

@@ -141,3 +141,15 @@ def test_tensors_that_share_no_byte():
             apart += 1
             assert not _bytes_of(views[0]) & _bytes_of(views[1]), views
     assert apart > 500
+
+
+@pytest.mark.parametrize("fn,base,names", [("b2m_grouped_mm", MM, ("ends", "status")),
+                                           ("b2m_grouped_mm_dx", dict(MM, ldx=32), ("ends", "status")),
+                                           ("b2m_grouped_mm_dw", DW, ("ends", "status")),
+                                           ("b2m_quant_i8", QUANT, ("scale", "status")),
+                                           ("b2m_int8_mm", INT8, ("ends", "a_scale", "w_scale", "status"))])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_words_that_start_anywhere_are_refused(fn, base, names, off):
+    """A 32-bit access at such an address would fault."""
+    for name in names:
+        _refused(fn, base, {name: P + off}, "4-byte aligned")
