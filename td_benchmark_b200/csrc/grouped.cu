@@ -1328,6 +1328,7 @@ int launch(const Maps& maps, const Params& p, int64_t tiles_bound, int num_sms, 
 }
 
 constexpr int64_t kMaxDim = int64_t(1) << 30;
+constexpr int64_t kMaxStride = int64_t(1) << 38;  // elements: more than any memory holds
 constexpr int64_t kMaxTiles = int64_t(1) << 30;
 
 uint32_t magic(int64_t d) { return static_cast<uint32_t>(((uint64_t(1) << 32) + d - 1) / d); }
@@ -1377,7 +1378,7 @@ int check_matrix(const char* what, const char* name, const Matrix& m, int elem) 
   if (m.rows < 0 || m.rows > kMaxDim || m.cols < 1 || m.cols > kMaxDim)
     return fail(B2M_ERR_ARG, "%s: %s is [%lld, %lld]; each extent is at most 2^30 and it has columns", what, name,
                 (long long)m.rows, (long long)m.cols);
-  if (m.ld < m.cols || m.ld * elem % 16 || m.ld > (int64_t(1) << 38))
+  if (m.ld < m.cols || m.ld > kMaxStride || m.ld * elem % 16)
     return fail(B2M_ERR_ARG, "%s: rows of %s must be at least %lld elements and a multiple of 16 bytes apart (%lld)",
                 what, name, (long long)m.cols, (long long)m.ld);
   if (m.rows > 0 && (!m.ptr || !aligned16(m.ptr)))
@@ -1390,7 +1391,7 @@ int check_weights(const char* what, const Weights& w, int elem) {
     return fail(B2M_ERR_ARG, "%s: need 1 <= experts <= %d (%lld)", what, kMaxExperts, (long long)w.experts);
   B2M_TRY(check_matrix(what, "w", Matrix{w.ptr, w.n, w.k, w.ld}, elem));
   if (w.n < 1) return fail(B2M_ERR_ARG, "%s: w has no rows", what);
-  if (w.expert_stride < 1 || w.expert_stride * elem % 16 || w.expert_stride > (int64_t(1) << 38))
+  if (w.expert_stride < 1 || w.expert_stride > kMaxStride || w.expert_stride * elem % 16)
     return fail(B2M_ERR_ARG, "%s: experts of w must be a multiple of 16 bytes apart (%lld elements)", what,
                 (long long)w.expert_stride);
   return B2M_OK;
@@ -1400,6 +1401,7 @@ int check_out(const char* what, const void* out, int64_t cols, int64_t ldo, int3
   if (!out) return fail(B2M_ERR_ARG, "%s: null output", what);
   if (ldo < cols) return fail(B2M_ERR_ARG, "%s: output rows are %lld elements apart, need %lld", what, (long long)ldo,
                               (long long)cols);
+  if (ldo > kMaxStride) return fail(B2M_ERR_ARG, "%s: output rows are more than 2^38 elements apart", what);
   if (out_type != B2M_FP32 && out_type != in_type)
     return fail(B2M_ERR_ARG, "%s: output type %d must be the input type or fp32", what, out_type);
   if (reinterpret_cast<uintptr_t>(out) % (out_type == B2M_FP32 ? 4 : 2))
@@ -1568,7 +1570,9 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   if (!ends) return fail(B2M_ERR_ARG, "%s: null ends", what);
   B2M_TRY(check_words(what, ends, dev_status));
   B2M_TRY(check_out(what, out, k, ldo, out_type, in_type));
-  if (out_stride < (n - 1) * ldo + k) return fail(B2M_ERR_ARG, "%s: experts of the output overlap", what);
+  // up to 2^30 rows, up to 2^38 elements apart: the product needs 128 bits
+  if (out_stride > kMaxStride || out_stride < static_cast<__int128>(n - 1) * ldo + k)
+    return fail(B2M_ERR_ARG, "%s: experts of the output overlap, or are more than 2^38 elements apart", what);
   Params p{};
   p.ends = ends;
   p.experts = experts;

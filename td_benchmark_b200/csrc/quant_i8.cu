@@ -372,7 +372,8 @@ int launch_quant(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q
 extern "C" int b2m_quant_i8(const void* x, int32_t in_type, int64_t rows, int64_t cols, int64_t ldx, void* q,
                             int64_t ldq, float* scale, int32_t* dev_status, void* stream) {
   using namespace b2m;
-  if (rows < 0 || cols < 1 || cols > (int64_t(1) << 30) || ldx < cols || ldq < cols)
+  if (rows < 0 || cols < 1 || cols > (int64_t(1) << 30) || ldx < cols || ldq < cols ||
+      ldx > (int64_t(1) << 38) || ldq > (int64_t(1) << 38))
     return fail(B2M_ERR_ARG, "quant_i8: bad shape [%lld, %lld], row strides %lld and %lld", (long long)rows,
                 (long long)cols, (long long)ldx, (long long)ldq);
   if (in_type != B2M_BF16 && in_type != B2M_FP16 && in_type != B2M_FP32)

@@ -153,3 +153,15 @@ def test_words_that_start_anywhere_are_refused(fn, base, names, off):
     """A 32-bit access at such an address would fault."""
     for name in names:
         _refused(fn, base, {name: P + off}, "4-byte aligned")
+
+
+@pytest.mark.parametrize("far", [(1 << 38) + 8, 1 << 59, 1 << 61, (1 << 62) - 16, 1 << 62, (1 << 63) - 16])
+def test_strides_whose_products_pass_64_bits_are_refused(far):
+    """Offsets are row times stride in 64 bits: a stride that no memory holds must not wrap into one that looks right."""
+    for fn, base, names in [("b2m_grouped_mm", MM, ("ldx", "ldw", "w_stride", "ldo")),
+                            ("b2m_grouped_mm_dx", dict(MM, ldx=32), ("ldx", "ldw", "w_stride", "ldo")),
+                            ("b2m_grouped_mm_dw", DW, ("lddy", "ldx", "ldo", "out_stride")),
+                            ("b2m_quant_i8", QUANT, ("ldx", "ldq")), ("b2m_int8_mm", INT8, ("lda", "ldw", "w_stride", "ldo"))]:
+        for name in names:
+            _refused(fn, base, {name: far}, "apart|bad shape")
+    _refused("b2m_grouped_mm_dw", DW, dict(n=5, ldo=1 << 62, lddy=32), "apart")
