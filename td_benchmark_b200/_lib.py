@@ -76,6 +76,8 @@ class B2MError(RuntimeError):
 def load(path: Path | None = None) -> ctypes.CDLL:
     """Load (once) and type the library; raise if it is absent."""
     global _lib
+    if path is None and _lib is not None:    # every call comes here, and only complete libraries are kept
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib
@@ -95,13 +97,8 @@ def load(path: Path | None = None) -> ctypes.CDLL:
         return lib
 
 
-_bound: dict[str, object] = {}   # entry points of the loaded library, by name
-
-
 def call(name: str, *args) -> None:
-    fn = _bound.get(name)
-    if fn is None:
-        fn = _bound.setdefault(name, getattr(load(), name))
-    rc = fn(*args)
+    lib = load()
+    rc = getattr(lib, name)(*args)
     if rc != 0:
-        raise B2MError(name, rc, load().b2m_last_error().decode(errors="replace"))
+        raise B2MError(name, rc, lib.b2m_last_error().decode(errors="replace"))
