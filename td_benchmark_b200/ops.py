@@ -461,12 +461,14 @@ def grouped_mm_dw(dy: torch.Tensor, x: torch.Tensor, ends: torch.Tensor, out: to
 
 def _kernel_rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself when the kernels can read its rows, else a copy whose rows are (a gradient that torch hands over
-    may be expanded, transposed or of a width that is no multiple of 16 bytes)."""
-    rows, cols = t.shape
-    if (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or (t.stride(0) >= cols and t.stride(0) % 8 == 0)) and \
-            t.data_ptr() % 16 == 0:
+    may be expanded, transposed or of a width that is no multiple of 16 bytes; saved tensors come back in another layout
+    when hooks kept them elsewhere)."""
+    cols = t.shape[-1]
+    if (cols <= 1 or t.stride(-1) == 1) and t.data_ptr() % 16 == 0 and \
+            (t.shape[-2] <= 1 or (t.stride(-2) >= cols and t.stride(-2) % 8 == 0)) and \
+            (t.dim() == 2 or t.shape[0] <= 1 or (t.stride(0) > 0 and t.stride(0) % 8 == 0)):
         return t
-    return torch.empty((rows, (cols + 7) // 8 * 8), dtype=t.dtype, device=t.device)[:, :cols].copy_(t)
+    return torch.empty((*t.shape[:-1], (cols + 7) // 8 * 8), dtype=t.dtype, device=t.device)[..., :cols].copy_(t)
 
 
 class _GroupedMM(torch.autograd.Function):
@@ -481,7 +483,7 @@ class _GroupedMM(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, w, ends = ctx.saved_tensors
-        dy = _kernel_rows(dy)
+        x, w, dy = _kernel_rows(x), _kernel_rows(w), _kernel_rows(dy)
         dx = grouped_mm_dx(dy, w, ends, status=ctx.status) if ctx.needs_input_grad[0] else None
         dw = grouped_mm_dw(dy, x, ends, status=ctx.status) if ctx.needs_input_grad[1] else None
         return dx, dw, None, None

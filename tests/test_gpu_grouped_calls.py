@@ -226,3 +226,20 @@ def test_codes_count_as_modified_too():
     before = q._version
     ops.quant_int8(x, q=q)
     assert q._version > before
+
+
+# ---------------------------------------------------------------- saved tensors
+@pytest.mark.parametrize("k", [61, 64])
+def test_saved_tensors_that_come_back_in_another_layout(k):
+    """Hooks that keep saved tensors on the host bring rows back that lie next to each other, whatever they were."""
+    counts, n = [4, 0, 9], 40
+    x = torch.full((13, 72), float("nan"), device=DEV, dtype=torch.bfloat16)[:, :k]
+    w = torch.full((3, n, 72), float("nan"), device=DEV, dtype=torch.bfloat16)[..., :k]
+    x.copy_(_randn(13, k)), w.copy_(_randn(3, n, k, seed=1))
+    x.requires_grad_(), w.requires_grad_()
+    dy = _randn(13, n, seed=2)
+    want = torch.autograd.grad(ops.grouped_mm(x, w, _ends(counts)), (x, w), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = ops.grouped_mm(x, w, _ends(counts))
+    for got, ref in zip(torch.autograd.grad(y, (x, w), dy), want):
+        assert torch.equal(got, ref)
