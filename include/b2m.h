@@ -396,8 +396,9 @@ int b2m_route_topk(const float* logits, int64_t tokens, int32_t experts, int32_t
  * Operands: type codes below; unit stride along the last axis; ld*, w_stride in elements,
  * multiples of 16 bytes (the extents need not be); base pointers 16-byte aligned; ends, scales and
  * dev_status 4-byte aligned.
- * Outputs: the input type or fp32, any row stride.  Sums are fp32 over the whole axis
- * and rounded once.  Extents <= 2^30. */
+ * Outputs: the input type or fp32, any row stride.  Sums are fp32; parts of a long sum may
+ * be added up in fp32, in a fixed order.  The output is rounded once.  Extents <= 2^30,
+ * strides <= 2^38 elements. */
 #define B2M_BF16 0
 #define B2M_FP16 1
 #define B2M_FP32 2
@@ -422,8 +423,8 @@ int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, 
  *   scale[r] = max(amax(|x[r, :]|) / 127, 1e-12)            (IEEE fp32 division)
  *   q[r, c]  = rne(x[r, c] / scale[r]) clamped to +-127      (IEEE fp32 division)
  * A NaN in a row makes its scale NaN, an infinity makes it infinite; the codes of such values
- * are 0, so whatever is multiplied with the row becomes NaN.  Any strides; x and q as their elements are aligned, scale
- * and dev_status 4-byte aligned. */
+ * are 0, so whatever is multiplied with the row becomes NaN.  Any strides up to 2^38
+ * elements; x and q as their elements are aligned, scale and dev_status 4-byte aligned. */
 int b2m_quant_i8(const void* x, int32_t in_type, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
                  float* scale, int32_t* dev_status, void* stream);
 

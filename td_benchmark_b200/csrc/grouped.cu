@@ -16,8 +16,9 @@
 // Persistent CTAs, in pairs (M = 256 over both), or single ones where segments are short:
 // warp 0 feeds a ring of TMA stages, warp 1 issues tcgen05.mma into one of two TMEM
 // accumulators, warps 4 and following turn the other one into output rows.
-// Every sum is one fp32 (or exact int32) accumulator in TMEM from the first product to
-// the last, rounded once.
+// A sum is one fp32 (or exact int32) accumulator in TMEM from the first product to the
+// last; where a cluster shares it, two to eight of them, added up in fp32 (int32) in the order
+// of its parts.  The output is rounded once.
 //
 // Rows that a tile loads beyond its segment are other output rows in kFwd and kDx, computed
 // and never stored.  In kDw they would enter the sum: the last warp clears them (in both operands,
@@ -494,9 +495,10 @@ struct Where {
 // find the same tiles each for itself: handing them over needs releases at cluster scope, which
 // wait for the epilogue's output stores, 3000 cycles a tile.)
 //
-// A wide launch walks its segments from the longest to the shortest, all pairs side by side on
-// the same one, and deals every second round of tiles out backwards, which evens the shares
-// out.  Long segments are limited by the tensor cores and short ones by memory, but doing both
+// A wide launch of up to 256 segments walks them from long classes of length to short ones (all
+// below 32 rows are one class, all from 6144 on another), with more segments as they come; all
+// pairs go side by side on the same segment, and every second round of tiles is dealt out
+// backwards, which evens the shares out.  Long segments are limited by the tensor cores and short ones by memory, but doing both
 // at once lost more than it gave: pairs that share weights or rows drift apart and read them
 // again (16384 rows over 32 experts of 4096 x 7168, lengths by Zipf 1.2: 3.6 GB instead of
 // 2.1 GB, 862 us instead of 800), and stores wait behind the others' loads (weight gradient:
@@ -1454,8 +1456,10 @@ int rows_times_weights(const char* what, const Matrix& x, const Weights& w, cons
   // and four times as many CTAs share them out (E=32, 4096 x 7168, forward: 280 us narrow, 288
   // wide at 8 rows each).  The mean is all that the host knows of the lengths.  Under Zipf 1.2 the
   // longest segments cost a narrow launch more than it saves from 16 rows on average (299
-  // narrow, 292 wide; 377 and 311 at 32), and not yet at 12 (278, 292).  One segment alone has the
-  // length that the host sees: up to one narrow tile.
+  // narrow, 292 wide; 377 and 311 at 32), and not yet at 12 (278, 292).  Nor does one segment that has a
+  // quarter of 12 rows an expert (E=256, 1536 x 2048: 243 narrow, 250 wide; E=1024, 768 x 2048: 496, 491);
+  // half of them on one cost 249 and 250 (508, 491), all of them 41 and 31 (85, 34).  One segment alone
+  // has the length that the host sees: up to one narrow tile.
   //
   // Few tiles for the SMs: clusters of two to eight CTAs share each one along its sum.  So a
   // launch is narrow whenever that makes no more than 64 tiles (bf16, one segment of 96 rows, 2048 x

@@ -127,9 +127,10 @@ __device__ __forceinline__ void round_two(float x0, float x1, float inv, float& 
 
 // The code (plus kRound) of an x whose product with 1 / scale lies `d` from the integer m, close
 // to the tie t = m +- 1/2.  e = x - t scale is exact: t has eight bits, so both terms are multiples
-// of 2^-25 of scale's power of two, and they differ by less than 2^11 of those.  The IEEE quotient is t
-// itself when x / scale is within half a step of it.  (Only at t = 1/2, a power of two, is the
-// step below it shorter; both answers are 0 there.)
+// of 2^-25 of scale's power of two P, and they differ by less than 2^12 of those (kNearTie and the
+// product's error make 6e-5 of scale, which is below 2 P).  The IEEE quotient is t itself when
+// x / scale is within half a step of it.  (Only at t = 1/2, a power of two, is the step below it
+// shorter; both answers are 0 there.)
 __device__ __forceinline__ float code_near_tie(float x, float scale, float m, float d) {
   const float t = m + copysignf(0.5f, d);
   const float e = __fmaf_rn(-t, scale, x);
