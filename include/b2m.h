@@ -414,7 +414,8 @@ int b2m_grouped_mm_dx(const void* dy, int64_t rows, int64_t lddy, const void* w,
                       int32_t out_type, int32_t clear_rest, int32_t* dev_status, void* stream);
 
 /* Gradient of the weights: out[e] = dy[segment e]^T x[segment e], zero for an empty segment.
- * dy [rows, n], x [rows, k], out [experts, n, k] (out_stride elements between experts). */
+ * dy [rows, n], x [rows, k], out [experts, n, k] (out_stride elements between experts, which lie
+ * behind each other or, with rows far enough apart, between each other's rows). */
 int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, int64_t ldx, int64_t rows, int64_t n, int64_t k,
                       const int32_t* ends, int32_t experts, int32_t in_type, void* out, int64_t ldo,
                       int64_t out_stride, int32_t out_type, int32_t* dev_status, void* stream);

@@ -1574,8 +1574,11 @@ extern "C" int b2m_grouped_mm_dw(const void* dy, int64_t lddy, const void* x, in
   if (!ends) return fail(B2M_ERR_ARG, "%s: null ends", what);
   B2M_TRY(check_words(what, ends, dev_status));
   B2M_TRY(check_out(what, out, k, ldo, out_type, in_type));
-  // up to 2^30 rows, up to 2^38 elements apart: the product needs 128 bits
-  if (out_stride > kMaxStride || out_stride < static_cast<__int128>(n - 1) * ldo + k)
+  // One expert behind the other, or row by row between the others'.  (Up to 2^30 rows, up to 2^38 elements apart: the
+  // products need 128 bits.)
+  const bool apart = out_stride >= static_cast<__int128>(n - 1) * ldo + k;
+  const bool between = out_stride >= k && ldo >= static_cast<__int128>(experts - 1) * out_stride + k;
+  if (out_stride > kMaxStride || (!apart && !between))
     return fail(B2M_ERR_ARG, "%s: experts of the output overlap, or are more than 2^38 elements apart", what);
   Params p{};
   p.ends = ends;

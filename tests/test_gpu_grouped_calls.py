@@ -243,3 +243,40 @@ def test_saved_tensors_that_come_back_in_another_layout(k):
         y = ops.grouped_mm(x, w, _ends(counts))
     for got, ref in zip(torch.autograd.grad(y, (x, w), dy), want):
         assert torch.equal(got, ref)
+
+
+# ---------------------------------------------------------------- orders and distances of the experts
+def _experts(kind, experts, rows, cols, dtype, fill):
+    """[experts, rows, cols] laid out one behind the other with a gap, or row by row between the others."""
+    if kind == "gap":
+        base = torch.full((experts * (rows * cols + 48),), fill, device=DEV, dtype=dtype)
+        return base, base.as_strided((experts, rows, cols), (rows * cols + 48, cols, 1))
+    base = torch.full((rows, experts, cols), fill, device=DEV, dtype=dtype)
+    return base, base.transpose(0, 1)
+
+
+@pytest.mark.parametrize("kind", ["gap", "between"])
+@pytest.mark.parametrize("counts,n,k", [([4, 0, 2], 32, 64), ([300, 1, 70], 264, 144), ([5, 0, 9], 264, 4112)])
+def test_experts_in_another_order(kind, counts, n, k):
+    """Weights and their gradients of any expert stride give what contiguous ones give."""
+    rows, ends = sum(counts), _ends(counts)
+    x, dy, w = _randn(rows, k), _randn(rows, n, seed=1), _randn(3, n, k, seed=2)
+    _, wide = _experts(kind, 3, n, k, torch.bfloat16, float("nan"))
+    wide.copy_(w)
+    assert torch.equal(ops.grouped_mm(x, wide, ends), ops.grouped_mm(x, w, ends))
+    assert torch.equal(ops.grouped_mm_dx(dy, wide, ends), ops.grouped_mm_dx(dy, w, ends))
+    a, sa = ops.quant_int8(x)
+    q, sw = ops.quant_int8(w.view(-1, k))
+    _, wide = _experts(kind, 3, n, k, torch.int8, 77)
+    wide.copy_(q.view(3, n, k))
+    want = ops.int8_grouped_mm(a, sa, q.view(3, n, k), sw.view(3, n), ends)
+    assert torch.equal(ops.int8_grouped_mm(a, sa, wide, sw.view(3, n), ends), want)
+    for dtype in (torch.bfloat16, torch.float32):
+        base, out = _experts(kind, 3, n, k, dtype, 7.0)
+        got = ops.grouped_mm_dw(dy, x, ends, out=out)
+        assert torch.equal(got, ops.grouped_mm_dw(dy, x, ends, out_dtype=dtype))
+        out.fill_(7.0)
+        assert (base == 7).all()                             # nothing between the experts was written
+    xr, wr = x.clone().requires_grad_(), _experts(kind, 3, n, k, torch.bfloat16, 0.0)[1].copy_(w).requires_grad_()
+    gx, gw = torch.autograd.grad(ops.grouped_mm(xr, wr, ends), (xr, wr), dy)
+    assert torch.equal(gx, ops.grouped_mm_dx(dy, w, ends)) and torch.equal(gw, ops.grouped_mm_dw(dy, x, ends))

@@ -165,3 +165,10 @@ def test_strides_whose_products_pass_64_bits_are_refused(far):
         for name in names:
             _refused(fn, base, {name: far}, "apart|bad shape")
     _refused("b2m_grouped_mm_dw", DW, dict(n=5, ldo=1 << 62, lddy=32), "apart")
+
+
+@pytest.mark.parametrize("change", [dict(out_stride=32, ldo=128), dict(out_stride=64, ldo=255), dict(out_stride=63, ldo=4096),
+                                    dict(out_stride=2047, ldo=64)])
+def test_weight_gradients_whose_experts_overlap_are_refused(change):
+    """Neither one behind the other nor row by row between the others."""
+    _refused("b2m_grouped_mm_dw", DW, change, "overlap")
